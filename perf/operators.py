@@ -221,9 +221,10 @@ def _run_int8(state):
         return int8_linear(state["x"], state["weight"], state["scale"], bias=state["bias"])
     x = state["x"].float()
     amax = x.abs().amax(-1, keepdim=True).clamp_min(2.0 ** -100)
-    q = torch.round(x * (127 / amax))
+    full = torch.full_like(amax, 127)  # tensor by tensor, so that both quotients are correctly rounded
+    q = torch.round(x * (full / amax))
     acc = (q.double() @ state["weight"].double().t()).float()  # integers past 2^24: summed in 64 bits
-    y = acc * ((amax / 127) * state["scale"])
+    y = acc * ((amax / full) * state["scale"])
     if state["bias"] is not None:
         y = y + state["bias"].float()
     return y.to(state["x"].dtype)
@@ -260,8 +261,9 @@ def exact(case, seed):
         # the quantised values are float32 by definition; what is made of them is in 64 bits
         x = st["x"].float()
         top = torch.maximum(x.max(-1).values, -x.min(-1).values).clamp(min=2.0 ** -100)
-        q = (x * (127 / top).unsqueeze(1)).round()
-        left = q.double() * (top / 127).double().unsqueeze(1)
+        top = top.unsqueeze(1)
+        steps = torch.full_like(top, 127)
+        left = (x * (steps / top)).round().double() * (top / steps).double()
         y = torch.einsum("mk,nk->mn", left, st["weight"].double() * st["scale"].double().unsqueeze(1))
         return [y if st["bias"] is None else y + st["bias"].double()]
 
