@@ -27,6 +27,9 @@ ATS_ETIMEOUT = -4
 ATS_F32 = 0
 ATS_BF16 = 1
 
+ATS_ROPE_MAX_PAIRS = 256
+ATS_POS_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}  # types of rotary positions
+
 ATS_MOE_PACKED = 0
 ATS_MOE_SLOTS = 1
 ATS_ROUTER_BWD_DW, ATS_ROUTER_BWD_DX, ATS_ROUTER_BWD_ALL = 1, 2, 3  # stages of ats_moe_router_bwd_staged
@@ -78,6 +81,21 @@ SIGNATURES: dict[str, tuple] = {
     "ats_rope_apply": (c_int, [c_void_p, c_void_p, c_int64, POINTER(c_int64), POINTER(c_int64),
                                c_void_p, c_void_p, c_int64, POINTER(c_int64), POINTER(c_int64),
                                c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int, c_int, c_void_p]),
+    "ats_sandwich_norm_fwd": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int64,
+                                      c_float, c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
+                                      c_void_p]),
+    "ats_sandwich_norm_bwd_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64]),
+    "ats_sandwich_norm_bwd": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int,
+                                      c_void_p, c_int, c_int64, c_float, c_void_p, c_void_p, c_void_p, c_void_p,
+                                      c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_int64, c_int64, c_void_p]),
+    "ats_rope_axes_apply": (c_int, [c_void_p, c_void_p, c_int64, POINTER(c_int64), POINTER(c_int64),
+                                    c_void_p, c_void_p, c_int64, POINTER(c_int64), POINTER(c_int64),
+                                    c_void_p, c_int, POINTER(c_int64), c_int, c_void_p, c_char_p, c_int,
+                                    c_int64, c_int64, c_int64, c_int, c_int, c_void_p]),
+    "ats_int8_quantize": (c_int, [c_void_p, c_int64, c_int, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p]),
+    "ats_int8_linear_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64]),
+    "ats_int8_linear": (c_int, [c_void_p, c_int64, c_int, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p,
+                                c_int64, c_int64, c_int64, c_void_p, c_size_t, c_void_p]),
     "ats_moe_status": (c_int, [c_void_p, c_size_t, c_int64, c_int, c_int, c_int64, c_int, POINTER(c_int)]),
     "ats_moe_plan_export": (c_int, [c_void_p, c_size_t, c_int64, c_int, c_int, c_int64, c_int, c_void_p, c_void_p,
                                     c_void_p, c_void_p]),
@@ -255,6 +273,15 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 def stream_of(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def device_of(t: torch.Tensor):
+    """Context in which ``t``'s device is the current one: the library launches on
+    the current device, which need not be that of the tensors."""
+    return _SAME_DEVICE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 def strides3(*s: int):

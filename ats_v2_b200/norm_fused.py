@@ -166,3 +166,116 @@ def fused_add_rmsnorm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Ten
         s = residual + x
         return rms_norm(s, weight, eps), s
     return _AddRMSNormFn.apply(x, residual, weight, eps)
+
+
+class _SandwichNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, post_weight, pre_weight, gate, rows_per_gate, residual_scale, eps):
+        ctx.set_materialize_grads(False)  # an unused result's gradient arrives as None and is not read
+        H = x.shape[-1]
+        x2, r2 = x.reshape(-1, H).contiguous(), residual.reshape(-1, H).contiguous()
+        wp, wn = post_weight.contiguous(), pre_weight.contiguous()
+        g = gate.contiguous() if gate is not None else None
+        rows = x2.shape[0]
+        s, h = torch.empty_like(x2), torch.empty_like(x2)
+        train = any(ctx.needs_input_grad)
+        rstd = torch.empty((2, rows), dtype=torch.float32, device=x.device) if train else None
+        with _lib.device_of(x):
+            _lib.call("ats_sandwich_norm_fwd", x2.data_ptr(), r2.data_ptr(), _lib.dtype_code(x2.dtype), wp.data_ptr(),
+                      wn.data_ptr(), _lib.dtype_code(wp.dtype), _lib.ptr(g),
+                      _lib.dtype_code(g.dtype) if g is not None else 0, rows_per_gate, residual_scale, eps,
+                      s.data_ptr(), h.data_ptr(), rstd[0].data_ptr() if train else None,
+                      rstd[1].data_ptr() if train else None, rows, H, _lib.stream_of(x))
+        if train:
+            ctx.save_for_backward(x2, r2, wp, wn, g, rstd)
+            ctx.meta = rows_per_gate, residual_scale, x.shape, gate.shape if gate is not None else None
+        return h.view(x.shape), s.view(x.shape)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dh, ds):
+        if dh is None and ds is None:
+            return (None,) * 8
+        x, r, wp, wn, g, rstd = ctx.saved_tensors
+        rows_per_gate, residual_scale, shape, gate_shape = ctx.meta
+        rows, H = x.shape
+        if rows == 0:
+            zero = x.new_zeros(shape)
+            return (zero, zero.clone(), torch.zeros_like(wp), torch.zeros_like(wn),
+                    torch.zeros(gate_shape, dtype=g.dtype, device=g.device) if g is not None else None,
+                    None, None, None)
+        dh, ds = (t.reshape(rows, H).to(x.dtype).contiguous() if t is not None else None for t in (dh, ds))
+        dx, dr = torch.empty_like(x), torch.empty_like(r)
+        dwp, dwn = torch.empty_like(wp), torch.empty_like(wn)
+        dg = torch.empty_like(g) if g is not None else None
+        with _lib.device_of(x):
+            wsb = _lib.query("ats_sandwich_norm_bwd_workspace_bytes", rows, H, rows_per_gate if g is not None else 0)
+            ws = torch.empty(wsb, dtype=torch.uint8, device=x.device)
+            _lib.call("ats_sandwich_norm_bwd", _lib.ptr(dh), _lib.ptr(ds), x.data_ptr(), r.data_ptr(),
+                      _lib.dtype_code(x.dtype), wp.data_ptr(), wn.data_ptr(), _lib.dtype_code(wp.dtype), _lib.ptr(g),
+                      _lib.dtype_code(g.dtype) if g is not None else 0, rows_per_gate, residual_scale,
+                      rstd[0].data_ptr(), rstd[1].data_ptr(), dx.data_ptr(), dr.data_ptr(), dwp.data_ptr(),
+                      dwn.data_ptr(), _lib.ptr(dg), ws.data_ptr(), wsb, rows, H, _lib.stream_of(x))
+        return (dx.view(shape), dr.view(shape), dwp, dwn, dg.view(gate_shape) if dg is not None else None,
+                None, None, None)
+
+
+def _rows_per_gate(shape: torch.Size, gate: torch.Tensor) -> int:
+    """How many consecutive rows of x share a gate row: gate is [H], or x's shape with
+    1 in place of the last axes before H (none of them, some or all)."""
+    if gate.dim() == 1 and gate.shape[0] == shape[-1]:
+        return max(1, shape[:-1].numel())
+    if gate.dim() == len(shape) and gate.shape[-1] == shape[-1]:
+        lead = len(shape) - 1
+        while lead > 0 and gate.shape[lead - 1] == 1:
+            lead -= 1
+        if gate.shape[:lead] == shape[:lead]:
+            return max(1, shape[lead:-1].numel())
+    raise ValueError(f"fused_sandwich_norm: gate shape {tuple(gate.shape)} must be ({shape[-1]},) or x's shape "
+                     f"{tuple(shape)} with 1 in place of the last axes before hidden, e.g. [batch, 1, hidden].")
+
+
+def _torch_sandwich_norm(x, residual, post_weight, pre_weight, gate, residual_scale, eps):
+    """The operator in torch operations (float32, rounded once): what CPU tensors run."""
+    def norm(v, w):
+        return v * torch.rsqrt(v.square().mean(-1, keepdim=True) + eps) * w.float()
+
+    p = norm(x.float(), post_weight)
+    s = residual_scale * residual.float() + (p if gate is None else gate.float() * p)
+    return norm(s, pre_weight).to(x.dtype), s.to(x.dtype)
+
+
+def fused_sandwich_norm(x: torch.Tensor, residual: torch.Tensor, post_weight: torch.Tensor, pre_weight: torch.Tensor,
+                        gate: torch.Tensor | None = None, residual_scale: float = 1.0,
+                        eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor]:
+    """The end of a transformer block whose output ``x`` is normalised before it joins the
+    residual stream, with the next block's norm:
+
+        s = residual_scale * residual + gate * (rms_norm(x) * post_weight)
+        h = rms_norm(s) * pre_weight
+
+    Returns (h, s): the next block's input and its residual.  ``x`` and ``residual``
+    share shape [..., hidden] and dtype (float32 or bfloat16); the weights [hidden]
+    share a dtype (float32 or bfloat16); ``gate`` (optional, float32 or bfloat16) is
+    [hidden] (per channel), x's shape (per token) or x's shape with 1 in place of the
+    last axes before hidden, e.g. [batch, 1, hidden] (per sequence).  The arithmetic is
+    float32 and each result is rounded once.  CUDA tensors run one kernel forward and
+    two or three backward; differentiable once, in every tensor argument."""
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"fused_sandwich_norm expected x of shape [..., hidden], got {tuple(x.shape)}.")
+    if x.shape != residual.shape:
+        raise ValueError(f"fused_sandwich_norm: x shape {tuple(x.shape)} must match residual shape "
+                         f"{tuple(residual.shape)}.")
+    for name, w in (("post_weight", post_weight), ("pre_weight", pre_weight)):
+        if w.shape != (x.shape[-1],):
+            raise ValueError(f"fused_sandwich_norm: {name} shape {tuple(w.shape)} must be ({x.shape[-1]},).")
+    if residual.dtype != x.dtype:
+        raise TypeError(f"fused_sandwich_norm: residual dtype {residual.dtype} must equal x dtype {x.dtype}")
+    if pre_weight.dtype != post_weight.dtype:
+        raise TypeError(f"fused_sandwich_norm: pre_weight dtype {pre_weight.dtype} must equal post_weight dtype "
+                        f"{post_weight.dtype}")
+    rows_per_gate = _rows_per_gate(x.shape, gate) if gate is not None else 0
+    residual_scale, eps = float(residual_scale), float(eps)
+    if _lib.on_cpu("fused_sandwich_norm", x, residual, post_weight, pre_weight, gate):
+        return _torch_sandwich_norm(x, residual, post_weight, pre_weight, gate, residual_scale, eps)
+    return _SandwichNormFn.apply(x, residual, post_weight, pre_weight, gate, rows_per_gate, residual_scale, eps)

@@ -13,9 +13,17 @@ ats/model/rope.py.
   writes outputs with the inputs' strides; its backward is the adjoint
   rotation, again one launch.
 * ``rotate_half`` is kept for API compatibility (rope.py:65-68).
+
+Not in the reference: positions with several axes (time, height and width of
+images and video).  ``apply_multi_axis_rotary(q, k, positions, inv_freq,
+sections)`` rotates each pair of a head by its own axis's position, and
+``MultiAxisRotaryEmbedding`` holds the frequencies.
 """
 
 from __future__ import annotations
+
+import functools
+from collections.abc import Sequence
 
 import torch
 from torch import nn
@@ -171,3 +179,138 @@ def apply_rotary_pos_emb(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor,
         raise ValueError(f"apply_rotary_pos_emb: q must be [batch, heads, seq_len, head_dim], got {tuple(q.shape)}")
     q, k, cos, sin, cs = _prepare(q, k, cos, sin, "apply_rotary_pos_emb")
     return _RopeFn.apply(q, k, cos, sin, cs)
+
+
+@functools.lru_cache(maxsize=64)
+def axis_of_pairs(sections: tuple[int, ...], interleaved: bool = False) -> bytes:
+    """The position axis of each rotated pair.  ``sections[a]`` pairs follow axis a:
+    section after section, or (``interleaved``) dealt out one by one to the axes that
+    have pairs left."""
+    if not sections or any(not isinstance(n, int) or n < 0 for n in sections) or len(sections) > 256 or \
+            not 1 <= sum(sections) <= _lib.ATS_ROPE_MAX_PAIRS:
+        raise ValueError(f"multi-axis rotary: sections {sections} must be counts of pairs, one per axis, 1 to "
+                         f"{_lib.ATS_ROPE_MAX_PAIRS} pairs in all.")
+    pairs = [(i, a) for a, n in enumerate(sections) for i in range(n)]
+    return bytes(a for _, a in (sorted(pairs) if interleaved else pairs))
+
+
+def _strides(t: torch.Tensor):
+    return _lib.strides3(t.stride(0), t.stride(1), t.stride(2))
+
+
+def _launch_axes(q, q_out, k, k_out, positions, inv_freq, axes: bytes, n_axes: int, backward: bool) -> None:
+    t = q if q is not None else k
+    B, _, S, D = t.shape
+    ps = (positions.stride(0), positions.stride(1) if positions.dim() == 3 else 0, positions.stride(-1))
+    if q is None:
+        q, q_out, k, k_out = k, k_out, None, None
+    with _lib.device_of(t):
+        _lib.call("ats_rope_axes_apply", q.data_ptr(), q_out.data_ptr(), q.shape[1], _strides(q), _strides(q_out),
+                  _lib.ptr(k), _lib.ptr(k_out), k.shape[1] if k is not None else 0,
+                  _strides(k) if k is not None else None, _strides(k_out) if k is not None else None,
+                  positions.data_ptr(), _lib.ATS_POS_TYPES[positions.dtype], _lib.strides3(*ps), n_axes,
+                  inv_freq.data_ptr(), axes, len(axes), B, S, D, _lib.dtype_code(t.dtype), 1 if backward else 0,
+                  _lib.stream_of(t))
+
+
+class _MultiAxisRotaryFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, positions, inv_freq, axes, n_axes):
+        ctx.set_materialize_grads(False)  # an unused output's gradient arrives as None, not zeros
+        q_out = torch.empty_like(q)
+        k_out = torch.empty_like(k) if k is not None else None
+        _launch_axes(q, q_out, k, k_out, positions, inv_freq, axes, n_axes, False)
+        ctx.save_for_backward(positions, inv_freq)
+        ctx.axes = axes, n_axes
+        return q_out, k_out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dq_out, dk_out):
+        positions, inv_freq = ctx.saved_tensors
+        dq_out, dk_out = (_last_dim_contig(t) if t is not None else None for t in (dq_out, dk_out))
+        dq, dk = (torch.empty_like(t) if t is not None else None for t in (dq_out, dk_out))
+        if dq is not None or dk is not None:
+            _launch_axes(dq_out, dq, dk_out, dk, positions, inv_freq, *ctx.axes, True)
+        return dq, dk, None, None, None, None
+
+
+def _torch_multi_axis(x: torch.Tensor, positions, inv_freq, axes: bytes) -> torch.Tensor:
+    """The rotation in torch operations (angles in 64 bits, float32 arithmetic): what CPU tensors run."""
+    n = len(axes)
+    pos = positions if positions.dim() == 3 else positions[:, None]
+    angle = pos.double()[list(axes)].permute(1, 2, 0) * inv_freq.double()  # [B, S, pairs]
+    cos, sin = angle.cos().float()[:, None], angle.sin().float()[:, None]
+    f = x.float()
+    a, b = f[..., :n], f[..., n:2 * n]
+    return torch.cat([a * cos - b * sin, b * cos + a * sin, f[..., 2 * n:]], -1).to(x.dtype)
+
+
+def apply_multi_axis_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv_freq: torch.Tensor,
+                            sections: Sequence[int], interleaved: bool = False
+                            ) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """Rotary embedding of q and k (optional) [batch, heads, seq_len, head_dim] whose positions
+    have several axes.  ``positions`` is [axes, batch, seq_len] or [axes, seq_len] (int32, int64
+    or float32); ``sections[a]`` pairs of each head follow axis a, consecutive or
+    (``interleaved``) dealt out in turn to the axes with pairs left; pair j joins columns j and
+    j + sum(sections) and turns by ``positions[axis] * inv_freq[j]`` radians (``inv_freq``
+    float32 [sum(sections)]).  Columns from 2*sum(sections) on pass unchanged.  The angles are
+    reduced in 64 bits, so far positions keep their accuracy; the rest is float32, rounded once.
+    Any batch, head and sequence strides; outputs are laid out like the inputs.  One launch each
+    way on CUDA tensors; differentiable once, in q and k."""
+    axes = axis_of_pairs(tuple(sections), bool(interleaved))
+    n_axes = len(sections)
+    if q.dim() != 4 or q.shape[-1] < 2 * len(axes):
+        raise ValueError(f"apply_multi_axis_rotary: q must be [batch, heads, seq_len, head_dim >= {2 * len(axes)}], "
+                         f"got {tuple(q.shape)}.")
+    B, _, S, D = q.shape
+    if k is not None:
+        if k.dim() != 4 or k.shape[0] != B or k.shape[2:] != q.shape[2:]:
+            raise ValueError(f"apply_multi_axis_rotary: k shape {tuple(k.shape)} incompatible with q {tuple(q.shape)}.")
+        if k.dtype != q.dtype:
+            raise TypeError(f"apply_multi_axis_rotary: q and k must share a dtype ({q.dtype} vs {k.dtype})")
+    if tuple(positions.shape) not in ((n_axes, B, S), (n_axes, S)):
+        raise ValueError(f"apply_multi_axis_rotary: positions must be [{n_axes}, {B}, {S}] or [{n_axes}, {S}], got "
+                         f"{tuple(positions.shape)}.")
+    if positions.dtype not in _lib.ATS_POS_TYPES:
+        raise TypeError(f"apply_multi_axis_rotary: positions must be int32, int64 or float32, got {positions.dtype}")
+    if inv_freq.shape != (len(axes),) or inv_freq.dtype != torch.float32:
+        raise ValueError(f"apply_multi_axis_rotary: inv_freq must be float32 [{len(axes)}], got {inv_freq.dtype} "
+                         f"{tuple(inv_freq.shape)}.")
+    if positions.requires_grad or inv_freq.requires_grad:
+        raise NotImplementedError("apply_multi_axis_rotary: gradients w.r.t. positions and inv_freq are not supported")
+    if _lib.on_cpu("apply_multi_axis_rotary", q, k, positions, inv_freq):
+        return (_torch_multi_axis(q, positions, inv_freq, axes),
+                _torch_multi_axis(k, positions, inv_freq, axes) if k is not None else None)
+    q = _last_dim_contig(q)
+    k = _last_dim_contig(k) if k is not None else None
+    return _MultiAxisRotaryFn.apply(q, k, positions, inv_freq.contiguous(), axes, n_axes)
+
+
+class MultiAxisRotaryEmbedding(nn.Module):
+    """Rotary embedding over several position axes, as ``RotaryEmbedding`` is over one: pair j of
+    the ``dim`` rotated columns has frequency theta^(-2j/dim) and follows the axis that
+    ``sections`` (pairs per axis, summing to dim/2) gives it.  With the same position on every
+    axis it is the rotation of ``RotaryEmbedding``."""
+
+    def __init__(self, dim: int, sections: Sequence[int], theta: float = 10000.0, interleaved: bool = False) -> None:
+        super().__init__()
+        if dim % 2 != 0 or 2 * len(axis_of_pairs(tuple(sections), bool(interleaved))) != dim:
+            raise ValueError(f"MultiAxisRotaryEmbedding: sections {tuple(sections)} must sum to dim / 2, got dim {dim}.")
+        self.dim = dim
+        self.sections = tuple(sections)
+        self.theta = theta
+        self.interleaved = bool(interleaved)
+        self.inv_freq: torch.Tensor
+        self.register_buffer("inv_freq", 1.0 / (theta ** (torch.arange(0, dim, 2, dtype=torch.float32) / dim)),
+                             persistent=False)
+
+    def _apply(self, fn, recurse=True):  # .to(dtype) must not round the frequencies
+        inv_freq = self.inv_freq
+        super()._apply(fn, recurse)
+        self.inv_freq = inv_freq.to(device=self.inv_freq.device)
+        return self
+
+    def forward(self, q: torch.Tensor, k: torch.Tensor | None,
+                positions: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor | None]:
+        return apply_multi_axis_rotary(q, k, positions, self.inv_freq, self.sections, self.interleaved)

@@ -182,6 +182,34 @@ ATS_API int ats_add_rmsnorm_bwd(const void* dy, const void* sum, const void* dsu
                                 size_t workspace_bytes, int64_t rows, int64_t hidden, float eps,
                                 void* stream);
 
+/* End of a transformer block with a norm after it and the next block's norm:
+ *   p = x * rstd(x) * w_post; sum = residual_scale * residual + gate * p;
+ *   h = sum * rstd(sum) * w_pre,   rstd(v) = 1 / sqrt(mean(v^2) + eps)
+ * in float32, sum and h each rounded once to dtype (h from the unrounded sum).
+ * x, residual, sum, h: rows x hidden contiguous; w_post, w_pre: [hidden] in
+ * w_dtype.  gate (may be NULL: 1) is [rows / rows_per_gate, hidden] in
+ * gate_dtype, each of its rows shared by rows_per_gate consecutive rows.
+ * rstd_x, rstd_sum: [rows] float32 kept for the backward (both or neither NULL).
+ * Any hidden below 2^30.  No reference counterpart (its block has the norms before only,
+ * ats/model/transformer.py:192-220). */
+ATS_API int ats_sandwich_norm_fwd(const void* x, const void* residual, ats_dtype dtype, const void* w_post,
+                                  const void* w_pre, ats_dtype w_dtype, const void* gate, ats_dtype gate_dtype,
+                                  int64_t rows_per_gate, float residual_scale, float eps, void* sum, void* h,
+                                  float* rstd_x, float* rstd_sum, int64_t rows, int64_t hidden, void* stream);
+
+/* Backward: dh and dsum (each may be NULL: zero) are the gradients of h and
+ * sum; dx, dresidual in dtype, dw_post and dw_pre in w_dtype, dgate in gate_dtype
+ * with the gate's shape.  Sums over rows are float32 in a fixed order.
+ * workspace: ats_sandwich_norm_bwd_workspace_bytes(rows, hidden, rows_per_gate), 16-byte aligned,
+ * with rows_per_gate 0 where there is no gate.  rows > 0. */
+ATS_API size_t ats_sandwich_norm_bwd_workspace_bytes(int64_t rows, int64_t hidden, int64_t rows_per_gate);
+ATS_API int ats_sandwich_norm_bwd(const void* dh, const void* dsum, const void* x, const void* residual,
+                                  ats_dtype dtype, const void* w_post, const void* w_pre, ats_dtype w_dtype,
+                                  const void* gate, ats_dtype gate_dtype, int64_t rows_per_gate,
+                                  float residual_scale, const float* rstd_x, const float* rstd_sum, void* dx,
+                                  void* dresidual, void* dw_post, void* dw_pre, void* dgate, void* workspace,
+                                  size_t workspace_bytes, int64_t rows, int64_t hidden, void* stream);
+
 /* ------------------------------------------------------------------- RoPE
  * Rotate-half RoPE on q [B,Hq,S,D] and k [B,Hk,S,D] in one launch:
  *   out = round(round(x*cos) + round(rotate_half(x)*sin)),
@@ -199,6 +227,27 @@ ATS_API int ats_rope_apply(const void* q_in, void* q_out, int64_t Hq,
                    const void* cos, const void* sin, int64_t cs_row_stride,
                    int64_t B, int64_t S, int64_t D, ats_dtype x_dtype,
                    int backward, void* stream);
+
+/* Rotary embedding with several position axes, forward (backward = 0) or
+ * adjoint, for q and optionally k in one launch.  Pair j (columns j and
+ * j + pairs of a head, j < pairs <= ATS_ROPE_MAX_PAIRS) of the token (b, s) is
+ * rotated by positions[axis_of_pair[j]][b][s] * inv_freq[j] radians; columns
+ * from 2*pairs on are copied.  float32 arithmetic, rounded once; the angle is
+ * reduced in double precision.  Tensors [B, heads, S, D] by strides as in
+ * ats_rope_apply; positions by element strides (axis, b, s), any of them 0, in
+ * the type pos_type; inv_freq [pairs] on the device; axis_of_pair [pairs] is a
+ * HOST array, read before the call returns.  The reference's embedding has one axis
+ * (ats/model/rope.py:17-87). */
+#define ATS_ROPE_MAX_PAIRS 256
+#define ATS_POS_I32 0
+#define ATS_POS_I64 1
+#define ATS_POS_F32 2
+ATS_API int ats_rope_axes_apply(const void* q_in, void* q_out, int64_t Hq, const int64_t q_in_strides[3],
+                                const int64_t q_out_strides[3], const void* k_in, void* k_out, int64_t Hk,
+                                const int64_t k_in_strides[3], const int64_t k_out_strides[3],
+                                const void* positions, int pos_type, const int64_t pos_strides[3], int axes,
+                                const float* inv_freq, const uint8_t* axis_of_pair, int pairs, int64_t B,
+                                int64_t S, int64_t D, ats_dtype x_dtype, int backward, void* stream);
 
 /* --------------------------------------------------------------- MoE router
  * Softmax over E experts in float32, top-k (descending; exact ties -> lower
@@ -536,6 +585,27 @@ ATS_API int ats_moe_router_bwd_staged(const float* dlogits, const void* x, const
 /* Device status of the router GEMMs run with this workspace (as ats_moe_status). */
 ATS_API int ats_moe_router_status(const void* workspace, size_t workspace_bytes, int64_t T, int64_t hidden,
                           int E, int* status);
+
+/* --------------------------------------------------- 8-bit integer projection
+ * ats_int8_quantize: rows of x [rows, K] to int8 with a float32 scale each,
+ *   amax = max(max|x|, 2^-100); q = rint(x * (127 / amax)); scale = amax / 127
+ * in float32, round half to even; a row with an infinity or NaN gets q = 0 and a NaN
+ * scale.  q rows are q_row_stride >= K bytes apart; bytes past K are set to 0.
+ * 1 <= K <= 131072.
+ * ats_int8_linear: x [M, K] quantised so, per token, then
+ *   y[m][n] = (sum_k q[m][k] w[n][k]) * (scale[m] * w_scale[n]) + bias[n]
+ * the sum exact in int32, the rest float32, rounded once to dtype.  w: int8
+ * [N, K], 16-byte aligned rows (w_row_stride a multiple of 16 bytes); bytes past K are not used.  bias
+ * [N] may be NULL.  y [M, N] contiguous.  workspace: 16-byte aligned,
+ * ats_int8_linear_workspace_bytes(M, N, K).  The reference's quantized Linear
+ * (ats/model/quantization.py:40-193) only imitates int8 in float. */
+ATS_API int ats_int8_quantize(const void* x, int64_t x_row_stride, ats_dtype dtype, void* q, int64_t q_row_stride,
+                              float* scale, int64_t rows, int64_t K, void* stream);
+ATS_API size_t ats_int8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K);
+ATS_API int ats_int8_linear(const void* x, int64_t x_row_stride, ats_dtype dtype, const void* w,
+                            int64_t w_row_stride, const float* w_scale, const void* bias, ats_dtype bias_dtype,
+                            void* y, int64_t M, int64_t N, int64_t K, void* workspace, size_t workspace_bytes,
+                            void* stream);
 
 #ifdef __cplusplus
 }
