@@ -88,13 +88,16 @@ int ats_gemm_pairs(void) { return ats::g_gemm_pairs.load(std::memory_order_relax
 
 int ats_set_wait_budget(int64_t cycles) {
   ATS_TRY(ats::gemm_set_wait_budget((long long)cycles));
+  ATS_TRY(ats::int8_set_wait_budget((long long)cycles));
   return ats::ring_set_wait_budget((long long)cycles);
 }
 
 int ats_device_status(int* status) {
   if (status == nullptr) return ats::fail(ATS_EBADARG, "device_status: null output");
-  int g = 0, r = 0, x = 0;
+  int g = 0, i8 = 0, r = 0, x = 0;
   ATS_TRY(ats::gemm_take_status(&g));
+  ATS_TRY(ats::int8_take_status(&i8));
+  if (g == 0) g = i8;
   ATS_TRY(ats::ring_take_status(&r));
   ATS_TRY(ats::ep_take_status(&x));
   *status = g != 0 ? g : r;

@@ -10,18 +10,32 @@
 // in float32 (a row with an infinity or NaN gets a NaN scale, so its outputs
 // are NaN).  The sum is exact in int32: K <= 131072 keeps 127 * 128 * K below
 // 2^31.  The scales and the bias are applied in float32, rounded once.
+#include <cudaTypedefs.h>
+
+#include <mutex>
+
 #include "common.cuh"
+#include "tc_ptx.cuh"
 
 namespace ats {
 namespace {
 
-constexpr int kQuantThreads = 256;
 constexpr int kMaxK = 131072;
+constexpr int64_t kMaxRows = 1 << 30;  // tokens and channels
+constexpr long long kWaitBudget = 4000000000LL;  // SM cycles, about 2 s
+// Budget of the main-loop waits and the first wait that gave up on this device (0: none), as for the other
+// tensor-core GEMMs; the waits that drain copies and MMAs always keep kWaitBudget.
+__device__ long long g_int8_wait_budget = kWaitBudget;
+__device__ int g_int8_status;
 
+__device__ __forceinline__ void give_up(volatile int* abort, int code) {
+  *abort = 1;
+  atomicCAS(&g_int8_status, 0, code);
+}
+
+// ------------------------------------------------------------- quantisation
 // |v| as an unsigned integer orders like |v|, and puts NaN above infinity above every number.
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
-
-__device__ __forceinline__ uint32_t warp_max_u(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
 
 // scale and 127 / amax of a row from the largest |x|'s bits
 __device__ __forceinline__ float row_scale(uint32_t bits, float& inv) {
@@ -39,89 +53,765 @@ __device__ __forceinline__ int quant(float v, float inv) {
   return r == r ? (int)fminf(fmaxf(r, -127.f), 127.f) : 0;
 }
 
-template <typename T>
+// 16 consecutive values of a row from element k; those at or past K are zero.
+template <typename T, bool VEC>
+__device__ __forceinline__ void load16(const T* row, int k, int K, float (&v)[16]) {
+  if (VEC && k + 16 <= K) {
+    load_n<T, 16>(row + k, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = k + i < K ? Cvt<T>::to_f(row[k + i]) : 0.f;
+  }
+}
+
+__device__ __forceinline__ uint32_t max16(const float (&v)[16], uint32_t m) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) m = max(m, abs_bits(v[i]));
+  return m;
+}
+
+__device__ __forceinline__ uint4 quant16(const float (&v)[16], float inv) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    w[i] = (uint32_t)(quant(v[4 * i], inv) & 255) | (uint32_t)(quant(v[4 * i + 1], inv) & 255) << 8 |
+           (uint32_t)(quant(v[4 * i + 2], inv) & 255) << 16 | (uint32_t)(quant(v[4 * i + 3], inv) & 255) << 24;
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// G threads to a row (a warp, or the whole block of 256), each with 16 consecutive values per step and the first
+// kKeep steps held in registers; a longer row is read again.  q rows are written in 16-byte pieces where they are
+// aligned for it (Q16), zeros up to the next multiple of 16 at most ldq.
+constexpr int kQuantThreads = 256, kKeep = 2;
+
+template <typename T, int G, bool VEC, bool Q16>
 __global__ void __launch_bounds__(kQuantThreads) int8_quantize_kernel(const T* __restrict__ x, int64_t ldx,
                                                                      int8_t* __restrict__ q, int64_t ldq,
                                                                      float* __restrict__ scale, int64_t rows, int K) {
+  tc::launch_dependents();
   __shared__ uint32_t red[kQuantThreads / 32];
-  const int64_t row = blockIdx.x;
+  const int64_t row = (int64_t)blockIdx.x * (kQuantThreads / G) + threadIdx.x / G;
+  const int t = threadIdx.x % G;
+  if (G == 32 && row >= rows) return;
   const T* xr = x + row * ldx;
+  float v[kKeep][16];
   uint32_t m = 0;
-  for (int k = threadIdx.x; k < K; k += kQuantThreads) {
-    const uint32_t b = abs_bits(Cvt<T>::to_f(xr[k]));
-    m = b > m ? b : m;
+#pragma unroll
+  for (int j = 0; j < kKeep; ++j) {
+    const int k = (j * G + t) * 16;
+    if (k < K) {
+      load16<T, VEC>(xr, k, K, v[j]);
+      m = max16(v[j], m);
+    }
   }
-  m = warp_max_u(m);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
-  __syncthreads();
-  for (int i = 0; i < kQuantThreads / 32; ++i) m = red[i] > m ? red[i] : m;
+  for (int k = (kKeep * G + t) * 16; k < K; k += G * 16) {
+    float u[16];
+    load16<T, VEC>(xr, k, K, u);
+    m = max16(u, m);
+  }
+  m = __reduce_max_sync(0xffffffffu, m);
+  if (G > 32) {
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kQuantThreads / 32; ++i) m = max(m, red[i]);
+  }
   float inv;
   const float s = row_scale(m, inv);
-  if (threadIdx.x == 0) scale[row] = s;
-  for (int k = threadIdx.x; k < K; k += kQuantThreads) q[row * ldq + k] = (int8_t)quant(Cvt<T>::to_f(xr[k]), inv);
-  for (int64_t k = K + threadIdx.x; k < ldq; k += kQuantThreads) q[row * ldq + k] = 0;
+  if (t == 0) scale[row] = s;
+  int8_t* qr = q + row * ldq;
+  auto put = [&](int k, const float (&u)[16]) {
+    const uint4 w = quant16(u, inv);
+    if (Q16) {
+      *reinterpret_cast<uint4*>(qr + k) = w;
+    } else {
+      const int8_t* e = reinterpret_cast<const int8_t*>(&w);
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (k + i < ldq) qr[k + i] = e[i];
+    }
+  };
+#pragma unroll
+  for (int j = 0; j < kKeep; ++j) {
+    const int k = (j * G + t) * 16;
+    if (k < K) put(k, v[j]);
+  }
+  for (int k = (kKeep * G + t) * 16; k < K; k += G * 16) {
+    float u[16];
+    load16<T, VEC>(xr, k, K, u);
+    put(k, u);
+  }
+  for (int64_t k = (K + 15) / 16 * 16 + t; k < ldq; k += G) qr[k] = 0;
 }
 
-// A warp per output channel and kTok tokens.
-constexpr int kTok = 4, kDotWarps = 8;
+template <typename T, int G>
+int quantize_g(const T* x, int64_t ldx, int8_t* q, int64_t ldq, float* scale, int64_t rows, int K, cudaStream_t st) {
+  const bool vec = aligned16(x) && ldx % Chunk<T>::N == 0, q16 = aligned16(q) && ldq % 16 == 0;
+  const int64_t per = kQuantThreads / G;
+  const unsigned grid = (unsigned)((rows + per - 1) / per);
+  if (vec && q16) int8_quantize_kernel<T, G, true, true><<<grid, kQuantThreads, 0, st>>>(x, ldx, q, ldq, scale, rows, K);
+  else if (vec) int8_quantize_kernel<T, G, true, false><<<grid, kQuantThreads, 0, st>>>(x, ldx, q, ldq, scale, rows, K);
+  else if (q16) int8_quantize_kernel<T, G, false, true><<<grid, kQuantThreads, 0, st>>>(x, ldx, q, ldq, scale, rows, K);
+  else int8_quantize_kernel<T, G, false, false><<<grid, kQuantThreads, 0, st>>>(x, ldx, q, ldq, scale, rows, K);
+  return check_launch("int8_quantize");
+}
 
+// A warp per row where the row fits its registers, a block per row beyond.
 template <typename T>
-__global__ void __launch_bounds__(32 * kDotWarps) int8_dot_kernel(const int8_t* __restrict__ q, int64_t ldq,
-                                                                 const float* __restrict__ sx,
-                                                                 const int8_t* __restrict__ w, int64_t ldw,
-                                                                 const float* __restrict__ sw, const void* bias,
-                                                                 int bias_bf16, T* __restrict__ y, int64_t M,
-                                                                 int64_t N, int K) {
-  const int lane = threadIdx.x & 31;
-  const int64_t n = (int64_t)blockIdx.x * kDotWarps + (threadIdx.x >> 5);
-  if (n >= N) return;
-  for (int64_t m0 = (int64_t)blockIdx.y * kTok; m0 < M; m0 += (int64_t)gridDim.y * kTok) {
-    const int nt = M - m0 < kTok ? (int)(M - m0) : kTok;
-    int acc[kTok] = {};
-    const int full = K / 16;
-    for (int c = lane; c < full; c += 32) {
-      const uint4 wv = *reinterpret_cast<const uint4*>(w + n * ldw + (int64_t)c * 16);
+int quantize_t(const void* x, int64_t ldx, void* q, int64_t ldq, float* scale, int64_t rows, int64_t K,
+               cudaStream_t st) {
+  auto* xp = static_cast<const T*>(x);
+  auto* qp = static_cast<int8_t*>(q);
+  return K <= 32 * 16 * kKeep ? quantize_g<T, 32>(xp, ldx, qp, ldq, scale, rows, (int)K, st)
+                              : quantize_g<T, kQuantThreads>(xp, ldx, qp, ldq, scale, rows, (int)K, st);
+}
+
+// ------------------------------------------------------------------ epilogue
+struct Out {
+  void* y;
+  const float* sx;
+  const float* sw;
+  const void* bias;
+  int bias_bf16;
+  int M, N;
+};
+
+__device__ __forceinline__ float bias_at(const Out& o, int n) {
+  if (o.bias == nullptr) return 0.f;
+  return o.bias_bf16 ? __bfloat162float(static_cast<const bf16*>(o.bias)[n]) : static_cast<const float*>(o.bias)[n];
+}
+
+// ------------------------------------------------------- one to kDotTokens tokens
+// One launch: every block quantises the tokens into its shared memory (they come from L2), with the first weights
+// of its warps already in flight, then a warp takes an output channel at a time: 16 weights per lane and step
+// against the tokens' integers.  The weights are read once, at full width; they bound it.
+constexpr int kDotTokens = 4, kDotThreads = 256, kDotStep = 8;
+constexpr int kDotSmem = 96 * 1024;
+
+template <typename T, int MT>
+__global__ void __launch_bounds__(kDotThreads) int8_dot_kernel(const T* __restrict__ x, int64_t ldx,
+                                                              const int8_t* __restrict__ w, int64_t ldw, Out o, int K,
+                                                              int vec) {
+  extern __shared__ __align__(16) int8_t qs[];  // [MT][Kp]
+  __shared__ uint32_t red[MT][kDotThreads / 32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int full = K / 16, Kp = (K + 15) / 16 * 16;
+  const int64_t stride = (int64_t)gridDim.x * (kDotThreads / 32);
+  int64_t n = (int64_t)blockIdx.x * (kDotThreads / 32) + warp;
+  uint4 wv[kDotStep];
+  auto load = [&](int64_t row, int c0) {
+    const int8_t* p = w + row * ldw;
 #pragma unroll
-      for (int t = 0; t < kTok; ++t)
-        if (t < nt) {
-          const uint4 qv = *reinterpret_cast<const uint4*>(q + (m0 + t) * ldq + (int64_t)c * 16);
-          acc[t] = __dp4a((int)wv.x, (int)qv.x, acc[t]);
-          acc[t] = __dp4a((int)wv.y, (int)qv.y, acc[t]);
-          acc[t] = __dp4a((int)wv.z, (int)qv.z, acc[t]);
-          acc[t] = __dp4a((int)wv.w, (int)qv.w, acc[t]);
+    for (int j = 0; j < kDotStep; ++j) {
+      const int c = c0 + j * 32 + lane;
+      if (c < full) wv[j] = __ldcs(reinterpret_cast<const uint4*>(p + (int64_t)c * 16));
+    }
+  };
+  if (n < o.N) load(n, 0);
+
+  uint32_t m[MT] = {};
+  for (int k = threadIdx.x * 16; k < K; k += kDotThreads * 16)
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+      if (t < o.M) {
+        float v[16];
+        if (vec) load16<T, true>(x + t * ldx, k, K, v);
+        else load16<T, false>(x + t * ldx, k, K, v);
+        m[t] = max16(v, m[t]);
+      }
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+    m[t] = __reduce_max_sync(0xffffffffu, m[t]);
+    if (lane == 0) red[t][warp] = m[t];
+  }
+  __syncthreads();
+  float sx[MT], inv[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+#pragma unroll
+    for (int i = 0; i < kDotThreads / 32; ++i) m[t] = max(m[t], red[t][i]);
+    sx[t] = row_scale(m[t], inv[t]);
+  }
+  for (int k = threadIdx.x * 16; k < K; k += kDotThreads * 16)
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      float v[16] = {};
+      if (t < o.M) {
+        if (vec) load16<T, true>(x + t * ldx, k, K, v);
+        else load16<T, false>(x + t * ldx, k, K, v);
+      }
+      *reinterpret_cast<uint4*>(qs + t * Kp + k) = quant16(v, inv[t]);
+    }
+  __syncthreads();
+
+  for (; n < o.N; n += stride) {
+    int acc[MT] = {};
+    for (int c0 = 0; c0 < full; c0 += kDotStep * 32) {
+      uint4 cur[kDotStep];
+#pragma unroll
+      for (int j = 0; j < kDotStep; ++j) cur[j] = wv[j];
+      // the next weights of this channel, or the first of the warp's next one
+      if (c0 + kDotStep * 32 < full) load(n, c0 + kDotStep * 32);
+      else if (n + stride < o.N) load(n + stride, 0);
+#pragma unroll
+      for (int j = 0; j < kDotStep; ++j) {
+        const int c = c0 + j * 32 + lane;
+        if (c < full) {
+#pragma unroll
+          for (int t = 0; t < MT; ++t) {
+            const uint4 qv = *reinterpret_cast<const uint4*>(qs + t * Kp + c * 16);
+            acc[t] = __dp4a((int)cur[j].x, (int)qv.x, acc[t]);
+            acc[t] = __dp4a((int)cur[j].y, (int)qv.y, acc[t]);
+            acc[t] = __dp4a((int)cur[j].z, (int)qv.z, acc[t]);
+            acc[t] = __dp4a((int)cur[j].w, (int)qv.w, acc[t]);
+          }
         }
+      }
     }
     const int k = full * 16 + lane;
     if (lane < 16 && k < K)
 #pragma unroll
-      for (int t = 0; t < kTok; ++t)
-        if (t < nt) acc[t] += (int)w[n * ldw + k] * (int)q[(m0 + t) * ldq + k];
+      for (int t = 0; t < MT; ++t) acc[t] += (int)w[n * ldw + k] * (int)qs[t * Kp + k];
 #pragma unroll
-    for (int t = 0; t < kTok; ++t) {
+    for (int t = 0; t < MT; ++t) {
       const int a = warp_sum_i(acc[t]);
-      if (lane == 0 && t < nt) {
-        float v = (float)a * (sx[m0 + t] * sw[n]);
-        if (bias != nullptr)
-          v += bias_bf16 ? __bfloat162float(static_cast<const bf16*>(bias)[n]) : static_cast<const float*>(bias)[n];
-        y[(m0 + t) * N + n] = Cvt<T>::from_f(v);
+      if (lane == t && t < o.M) {
+        float v = (float)a * (sx[t] * o.sw[n]);
+        if (o.bias != nullptr) v += bias_at(o, (int)n);
+        static_cast<T*>(o.y)[(int64_t)t * o.N + n] = Cvt<T>::from_f(v);
       }
     }
   }
 }
 
-template <typename T>
-int quantize_t(const void* x, int64_t ldx, void* q, int64_t ldq, float* scale, int64_t rows, int64_t K,
-               cudaStream_t st) {
-  int8_quantize_kernel<T><<<(unsigned)rows, kQuantThreads, 0, st>>>(static_cast<const T*>(x), ldx,
-                                                                   static_cast<int8_t*>(q), ldq, scale, rows, (int)K);
-  return check_launch("int8_quantize");
+// ------------------------------------------------- tensor cores, many tokens
+// tcgen05.mma kind::i8 on 128 tokens x BN channels, K in blocks of 128 bytes: one persistent CTA per SM, a TMA
+// producer warp, an MMA warp with two accumulators in TMEM, eight epilogue warps (two per TMEM lane quadrant, half
+// of the columns each) that scale, round and store through swizzled boxes.
+constexpr int BM = 128, BKB = 128;
+constexpr int kEpiWarps = 8, kTileThreads = 64 + 32 * kEpiWarps;
+constexpr int kBox = 32 * 64, kBoxesPerWarp = 2;  // a box: 32 rows of 64 bytes
+constexpr int kBandM = 16;                        // M tiles per band of the tile order
+
+__host__ __device__ constexpr int tile_stage_bytes(int bn) { return (BM + bn) * BKB; }
+__host__ __device__ constexpr int tile_stages(int bn) { return 4 * tile_stage_bytes(256) / tile_stage_bytes(bn); }
+
+struct TileArgs {
+  Out o;
+  int kb;       // K blocks
+  int mt, nt;   // tiles
+  int tma_out;  // rows of y are 16-byte multiples: boxes leave by TMA
+};
+
+// Tile t: bands of kBandM M tiles, M fastest inside a band, so that the CTAs that run together share weights and
+// the band's tokens in L2.
+__device__ __forceinline__ void tile_of(const TileArgs& p, int t, int& m, int& n) {
+  const int band = t / (kBandM * p.nt), m0 = band * kBandM;
+  const int gm = p.mt - m0 < kBandM ? p.mt - m0 : kBandM;
+  const int r = t - band * kBandM * p.nt;
+  n = r / gm;
+  m = m0 + (r - n * gm);
 }
 
+template <typename T, int BN>
+__global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid_constant__ CUtensorMap tmA,
+                                                                   const __grid_constant__ CUtensorMap tmB,
+                                                                   const __grid_constant__ CUtensorMap tmO,
+                                                                   TileArgs p) {
+  constexpr int STAGE = tile_stage_bytes(BN), NST = tile_stages(BN);
+  constexpr uint32_t IDESC = tc::idesc_i8(BM, BN);
+  constexpr int BOX_COLS = 64 / (int)sizeof(T);
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* staging = ring + NST * STAGE;
+  __shared__ __align__(8) uint64_t full_bar[NST], empty_bar[NST], tfull_bar[2], tempty_bar[2], done_bar;
+  __shared__ uint32_t tmem_base_s;
+  __shared__ volatile int abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long budget = g_int8_wait_budget;
+  const int total = p.mt * p.nt;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < NST; ++s) {
+      tc::mbar_init(&full_bar[s], 1);
+      tc::mbar_init(&empty_bar[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      tc::mbar_init(&tfull_bar[a], 1);
+      tc::mbar_init(&tempty_bar[a], kEpiWarps);
+    }
+    tc::mbar_init(&done_bar, 1);
+    tc::fence_barrier_init();
+    tc::fence_proxy_async_smem();
+    abort_flag = 0;
+  }
+  if (warp == 1) {
+    tc::tmem_alloc(&tmem_base_s, 2 * BN);
+    tc::tmem_relinquish();
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tmem_base = tmem_base_s;
+  tc::wait_prerequisites();  // the quantised tokens and their scales
+
+  if (warp == 0) {
+    if (lane == 0) {
+      tc::prefetch_tensormap(&tmA);
+      tc::prefetch_tensormap(&tmB);
+      int stage = 0, issued = 0;
+      uint32_t phase = 0;
+      for (int t = blockIdx.x; t < total && !abort_flag; t += gridDim.x) {
+        int m, n;
+        tile_of(p, t, m, n);
+        for (int kb = 0; kb < p.kb; ++kb) {
+          if (!tc::mbar_wait(&empty_bar[stage], phase ^ 1u, &abort_flag, budget)) {
+            give_up(&abort_flag, 31);
+            break;
+          }
+          uint8_t* sa = ring + stage * STAGE;
+          tc::mbar_arrive_expect_tx(&full_bar[stage], STAGE);
+          tc::tma_load_2d(sa, &tmA, kb * BKB, m * BM, &full_bar[stage]);
+          tc::tma_load_2d(sa + BM * BKB, &tmB, kb * BKB, n * BN, &full_bar[stage]);
+          ++issued;
+          if (++stage == NST) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      // every load issued lands before the CTA may exit
+      for (int s = 0; s < NST && s < issued; ++s) {
+        const int last = s + (issued - 1 - s) / NST * NST;
+        if (!tc::mbar_wait(&full_bar[s], (uint32_t)((last / NST) & 1), nullptr, kWaitBudget))
+          atomicCAS(&g_int8_status, 0, 35);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      int stage = 0, i = 0;
+      uint32_t phase = 0;
+      bool issued = false;
+      for (int t = blockIdx.x; t < total && !abort_flag; t += gridDim.x, ++i) {
+        const int acc = i & 1;
+        if (!tc::mbar_wait(&tempty_bar[acc], ((uint32_t)(i >> 1) & 1u) ^ 1u, &abort_flag, budget)) {
+          give_up(&abort_flag, 32);
+          break;
+        }
+        tc::tc_fence_after();
+        bool ok = true;
+        for (int kb = 0; kb < p.kb; ++kb) {
+          if (!tc::mbar_wait(&full_bar[stage], phase, &abort_flag, budget)) {
+            give_up(&abort_flag, 33);
+            ok = false;
+            break;
+          }
+          tc::tc_fence_after();
+          const uint32_t sa = tc::smem_u32(ring + stage * STAGE), sb = sa + BM * BKB;
+#pragma unroll
+          for (int k = 0; k < BKB / 32; ++k)
+            tc::mma_i8(tmem_base + (uint32_t)(acc * BN), tc::smem_desc(sa + k * 32, 16u, 1024u, tc::kLayoutSW128),
+                       tc::smem_desc(sb + k * 32, 16u, 1024u, tc::kLayoutSW128), IDESC, (kb > 0 || k > 0) ? 1u : 0u);
+          tc::mma_commit(&empty_bar[stage]);
+          issued = true;
+          if (++stage == NST) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (!ok) break;
+        tc::mma_commit(&tfull_bar[acc]);
+      }
+      if (issued) {  // all MMAs complete before TMEM is freed
+        tc::mma_commit(&done_bar);
+        if (!tc::mbar_wait(&done_bar, 0u, nullptr, kWaitBudget)) atomicCAS(&g_int8_status, 0, 36);
+      }
+    }
+  } else {
+    const int quad = warp & 3, chalf = (warp - 2) >> 2;
+    uint8_t* boxes = staging + (warp - 2) * kBoxesPerWarp * kBox;
+    int puts = 0, i = 0;
+    for (int t = blockIdx.x; t < total && !abort_flag; t += gridDim.x, ++i) {
+      int m, n;
+      tile_of(p, t, m, n);
+      const int acc = i & 1;
+      const int row0 = m * BM + quad * 32, row = row0 + lane;
+      const float sx = row < p.o.M ? p.o.sx[row] : 0.f;
+      if (!tc::mbar_wait(&tfull_bar[acc], (uint32_t)(i >> 1) & 1u, &abort_flag, budget)) {
+        give_up(&abort_flag, 34);
+        break;
+      }
+      tc::tc_fence_after();
+      const uint32_t t_row = tmem_base + (uint32_t)(acc * BN + chalf * (BN / 2)) + ((uint32_t)(quad * 32) << 16);
+#pragma unroll 1
+      for (int c = 0; c < BN / 2; c += BOX_COLS) {
+        const int col0 = n * BN + chalf * (BN / 2) + c;
+        float v[BOX_COLS];
+#pragma unroll
+        for (int h = 0; h < BOX_COLS; h += 16) {
+          uint32_t r[16];
+          tc::tmem_ld16(t_row + c + h, r);
+          const int colw = col0 + h + (lane & 15);
+          const float sw = colw < p.o.N ? p.o.sw[colw] : 0.f;
+          const float bw = colw < p.o.N ? bias_at(p.o, colw) : 0.f;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            v[h + j] = (float)(int)r[j] * (sx * __shfl_sync(0xffffffffu, sw, j));
+            if (p.o.bias != nullptr) v[h + j] += __shfl_sync(0xffffffffu, bw, j);
+          }
+        }
+        uint8_t* box = boxes + (puts % kBoxesPerWarp) * kBox;
+        if (lane == 0) tc::bulk_wait_read<kBoxesPerWarp - 1>();
+        __syncwarp();
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {  // row `lane`, 16-byte piece q at its swizzled place (conflict-free)
+          float u[Chunk<T>::N];
+#pragma unroll
+          for (int j = 0; j < Chunk<T>::N; ++j) u[j] = v[q * Chunk<T>::N + j];
+          uint4 w;
+          pack_chunk<T>(u, w);
+          *reinterpret_cast<uint4*>(box + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4)) = w;
+        }
+        if (p.tma_out) {
+          tc::fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            if (col0 < p.o.N && row0 < p.o.M) tc::tma_store_2d(&tmO, box, col0, row0);
+            tc::bulk_commit();
+          }
+        } else {  // rows of y that are not 16-byte multiples: element by element, along the rows
+          __syncwarp();
+          constexpr int ROWS = 32 / BOX_COLS;  // rows a warp writes at once
+          const int cc = lane % BOX_COLS, byte = cc * (int)sizeof(T);
+          for (int r = lane / BOX_COLS; r < 32; r += ROWS)
+            if (row0 + r < p.o.M && col0 + cc < p.o.N)
+              static_cast<T*>(p.o.y)[(int64_t)(row0 + r) * p.o.N + col0 + cc] = *reinterpret_cast<const T*>(
+                  box + r * 64 + (((byte >> 4) ^ ((r >> 1) & 3)) << 4) + (byte & 15));
+          __syncwarp();
+        }
+        ++puts;
+      }
+      tc::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&tempty_bar[acc]);
+    }
+    if (lane == 0) tc::bulk_wait<0>();
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  if (warp == 1) tc::tmem_dealloc(tmem_base, 2 * BN);
+}
+
+// -------------------------------------------------- tensor cores, few tokens
+// The weights take the MMA's 128 rows and TN tokens its columns, and a cluster of `split` CTAs shares K: each sums
+// its part of K in TMEM, puts its int32 tile into its shared memory, and every CTA adds the parts of its share of
+// the tokens through distributed shared memory.  So a decoding batch reads the weights with every SM, and no
+// workspace or atomics are needed.  The weights' loads start before the quantisation has ended.
+constexpr int kPartThreads = 192;
+
+__host__ __device__ constexpr int part_stage_bytes(int tn) { return (BM + tn) * BKB; }
+__host__ __device__ constexpr int part_stages(int tn) { return 200 * 1024 / part_stage_bytes(tn) < 8 ? 200 * 1024 / part_stage_bytes(tn) : 8; }
+
+template <typename T, int TN>
+__global__ void __launch_bounds__(kPartThreads, 1) int8_part_kernel(const __grid_constant__ CUtensorMap tmW,
+                                                                   const __grid_constant__ CUtensorMap tmX, Out o,
+                                                                   int kb_all) {
+  constexpr int STAGE = part_stage_bytes(TN), NST = part_stages(TN);
+  constexpr int TCOLS = TN < 32 ? 32 : TN;
+  constexpr uint32_t IDESC = tc::idesc_i8(BM, TN);
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ __align__(8) uint64_t full_bar[NST], empty_bar[NST], tfull_bar;
+  __shared__ uint32_t tmem_base_s;
+  __shared__ volatile int abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long budget = g_int8_wait_budget;
+  const int split = (int)gridDim.z, part = (int)blockIdx.z;  // the cluster is all of z
+  const int kb0 = (int)((int64_t)kb_all * part / split), kb1 = (int)((int64_t)kb_all * (part + 1) / split);
+  const int n0 = blockIdx.x * BM, m0 = blockIdx.y * TN;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < NST; ++s) {
+      tc::mbar_init(&full_bar[s], 1);
+      tc::mbar_init(&empty_bar[s], 1);
+    }
+    tc::mbar_init(&tfull_bar, 1);
+    tc::fence_barrier_init();
+    tc::fence_proxy_async_smem();
+    abort_flag = 0;
+  }
+  if (warp == 1) {
+    tc::tmem_alloc(&tmem_base_s, TCOLS);
+    tc::tmem_relinquish();
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tmem_base = tmem_base_s;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      const int nkb = kb1 - kb0;
+      const int ahead = nkb < NST ? nkb : NST;
+      for (int s = 0; s < ahead; ++s) {
+        tc::mbar_arrive_expect_tx(&full_bar[s], STAGE);
+        tc::tma_load_2d(ring + s * STAGE, &tmW, (kb0 + s) * BKB, n0, &full_bar[s]);
+      }
+      tc::wait_prerequisites();
+      for (int s = 0; s < ahead; ++s)
+        tc::tma_load_2d(ring + s * STAGE + BM * BKB, &tmX, (kb0 + s) * BKB, m0, &full_bar[s]);
+      int issued = ahead;
+      for (int i = ahead; i < nkb; ++i) {
+        const int s = i % NST;
+        if (!tc::mbar_wait(&empty_bar[s], (uint32_t)((i / NST) & 1) ^ 1u, &abort_flag, budget)) {
+          give_up(&abort_flag, 41);
+          break;
+        }
+        tc::mbar_arrive_expect_tx(&full_bar[s], STAGE);
+        tc::tma_load_2d(ring + s * STAGE, &tmW, (kb0 + i) * BKB, n0, &full_bar[s]);
+        tc::tma_load_2d(ring + s * STAGE + BM * BKB, &tmX, (kb0 + i) * BKB, m0, &full_bar[s]);
+        ++issued;
+      }
+      for (int s = 0; s < NST && s < issued; ++s) {  // every load issued lands before the CTA may exit
+        const int last = s + (issued - 1 - s) / NST * NST;
+        if (!tc::mbar_wait(&full_bar[s], (uint32_t)((last / NST) & 1), nullptr, kWaitBudget))
+          atomicCAS(&g_int8_status, 0, 45);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const int nkb = kb1 - kb0;
+      for (int i = 0; i < nkb; ++i) {
+        const int s = i % NST;
+        if (!tc::mbar_wait(&full_bar[s], (uint32_t)((i / NST) & 1), &abort_flag, budget)) {
+          give_up(&abort_flag, 43);
+          break;
+        }
+        tc::tc_fence_after();
+        const uint32_t sa = tc::smem_u32(ring + s * STAGE), sb = sa + BM * BKB;
+#pragma unroll
+        for (int k = 0; k < BKB / 32; ++k)
+          tc::mma_i8(tmem_base, tc::smem_desc(sa + k * 32, 16u, 1024u, tc::kLayoutSW128),
+                     tc::smem_desc(sb + k * 32, 16u, 1024u, tc::kLayoutSW128), IDESC, (i > 0 || k > 0) ? 1u : 0u);
+        tc::mma_commit(&empty_bar[s]);
+      }
+      tc::mma_commit(&tfull_bar);  // also after a wait that gave up: the MMAs issued complete before TMEM is freed
+    }
+  }
+  __syncwarp();
+  tc::wait_prerequisites();  // the scales
+  if (!tc::mbar_wait(&tfull_bar, 0u, nullptr, kWaitBudget)) atomicCAS(&g_int8_status, 0, 44);
+  tc::tc_fence_after();
+  const int n_here = warp >= 2 ? n0 + (warp & 3) * 32 + lane : 0;
+  if (split == 1) {
+    if (warp >= 2) {  // thread = channel, columns = tokens: a warp's stores run along the channels
+      const float sw = n_here < o.N ? o.sw[n_here] : 0.f, bw = n_here < o.N ? bias_at(o, n_here) : 0.f;
+#pragma unroll 1
+      for (int c = 0; c < TN; c += 16) {
+        uint32_t r[16];
+        tc::tmem_ld16(tmem_base + (uint32_t)c + ((uint32_t)((warp & 3) * 32) << 16), r);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const int m = m0 + c + j;
+          if (m < o.M && n_here < o.N) {
+            float v = (float)(int)r[j] * (o.sx[m] * sw);
+            if (o.bias != nullptr) v += bw;
+            static_cast<T*>(o.y)[(int64_t)m * o.N + n_here] = Cvt<T>::from_f(v);
+          }
+        }
+      }
+    }
+  } else {
+    int* tile = reinterpret_cast<int*>(ring);  // [TN][128]: the ring is no longer read or written
+    if (warp >= 2) {
+#pragma unroll 1
+      for (int c = 0; c < TN; c += 16) {
+        uint32_t r[16];
+        tc::tmem_ld16(tmem_base + (uint32_t)c + ((uint32_t)((warp & 3) * 32) << 16), r);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) tile[(c + j) * BM + (warp & 3) * 32 + lane] = (int)r[j];
+      }
+    }
+    __syncwarp();
+    tc::cluster_sync();
+    const int share = TN / split;  // tokens of this CTA
+    for (int i = threadIdx.x; i < share * (BM / 4); i += kPartThreads) {
+      const int t = part * share + i / (BM / 4), r4 = i % (BM / 4) * 4;
+      const int m = m0 + t, n = n0 + r4;
+      if (m >= o.M || n >= o.N) continue;
+      int4 a = make_int4(0, 0, 0, 0);
+      const uint32_t mine = tc::smem_u32(tile + t * BM + r4);
+      for (int z = 0; z < split; ++z) {
+        const int4 b = tc::ld_cluster_v4(tc::cluster_addr(mine, (uint32_t)z));
+        a.x += b.x, a.y += b.y, a.z += b.z, a.w += b.w;
+      }
+      const float sx = o.sx[m];
+      const int e[4] = {a.x, a.y, a.z, a.w};
+      T* y = static_cast<T*>(o.y) + (int64_t)m * o.N + n;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (n + j < o.N) {
+          float v = (float)e[j] * (sx * o.sw[n + j]);
+          if (o.bias != nullptr) v += bias_at(o, n + j);
+          y[j] = Cvt<T>::from_f(v);
+        }
+    }
+    tc::cluster_sync();  // no CTA leaves while another reads its tile
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  if (warp == 1) tc::tmem_dealloc(tmem_base, TCOLS);
+}
+
+// ---------------------------------------------------------------------- host
 int64_t padded_k(int64_t K) { return (K + 15) / 16 * 16; }
 
 size_t q_bytes(int64_t M, int64_t K) { return align_up((size_t)(M * padded_k(K)), 256); }
 
+PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
+std::once_flag g_encode_once;
+
+int encode(CUtensorMap* m, CUtensorMapDataType type, const void* base, uint64_t inner, uint64_t outer,
+           uint64_t row_bytes, uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle swz) {
+  std::call_once(g_encode_once, [] {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      g_encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+  });
+  if (g_encode == nullptr) return fail(ATS_ECUDA, "int8_linear: cuTensorMapEncodeTiled unavailable");
+  cuuint64_t dims[2] = {inner, outer};
+  cuuint64_t strides[1] = {row_bytes};
+  cuuint32_t box[2] = {box_inner, box_outer};
+  cuuint32_t es[2] = {1, 1};
+  CUresult r = g_encode(m, type, 2, const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        swz, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(ATS_ECUDA, "int8_linear: cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return ATS_OK;
+}
+
+// Operand of int8 rows: boxes of 128 bytes x `rows`, 128-byte swizzle; bytes past K and rows past the end read as 0.
+int operand_map(CUtensorMap* m, const void* base, int64_t K, int64_t rows, int64_t ld, int box_rows) {
+  return encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, (uint64_t)K, (uint64_t)rows, (uint64_t)ld, BKB,
+                (uint32_t)box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+// Launch after a kernel whose launch_dependents() lets this one's prologue start early; z is one cluster.
+template <typename K, typename... A>
+int launch_after(K kernel, dim3 grid, int threads, int smem, int cluster_z, cudaStream_t st, const char* what, A... args) {
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return fail(ATS_ECUDA, "%s: %s", what, cudaGetErrorString(e));
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 1;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = (unsigned)cluster_z;
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster_z > 1 ? 2 : 1;
+  e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  if (e != cudaSuccess) return fail(ATS_ECUDA, "%s: %s", what, cudaGetErrorString(e));
+  return check_launch(what);
+}
+
+template <typename T>
+int dot(const void* x, int64_t ldx, const int8_t* w, int64_t ldw, const Out& o, int K, cudaStream_t st) {
+  const int warps = kDotThreads / 32;
+  const int64_t want = (o.N + warps - 1) / warps, cap = (int64_t)num_sms() * 4;
+  const unsigned grid = (unsigned)(want < cap ? want : cap);
+  const int mt = o.M == 1 ? 1 : o.M == 2 ? 2 : 4;
+  const int smem = mt * (int)padded_k(K);
+  auto* xp = static_cast<const T*>(x);
+  const int vec = aligned16(x) && ldx % Chunk<T>::N == 0;
+  auto go = [&](auto kernel) {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kDotSmem);
+    if (e != cudaSuccess) return fail(ATS_ECUDA, "int8_dot: %s", cudaGetErrorString(e));
+    kernel<<<grid, kDotThreads, smem, st>>>(xp, ldx, w, ldw, o, K, vec);
+    return check_launch("int8_dot");
+  };
+  return mt == 1 ? go(int8_dot_kernel<T, 1>) : mt == 2 ? go(int8_dot_kernel<T, 2>) : go(int8_dot_kernel<T, 4>);
+}
+
+template <typename T, int BN>
+int tiles(const int8_t* q, int64_t ldq, const int8_t* w, int64_t ldw, const Out& o, int K, cudaStream_t st) {
+  CUtensorMap ma, mb, mo;
+  ATS_TRY(operand_map(&ma, q, K, o.M, ldq, BM));
+  ATS_TRY(operand_map(&mb, w, K, o.N, ldw, BN));
+  TileArgs p{o, (K + BKB - 1) / BKB, (o.M + BM - 1) / BM, (o.N + BN - 1) / BN, 0};
+  const int64_t row_bytes = (int64_t)o.N * (int64_t)sizeof(T);
+  p.tma_out = row_bytes % 16 == 0 && aligned16(o.y);
+  if (p.tma_out)
+    ATS_TRY(encode(&mo, sizeof(T) == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, o.y,
+                   (uint64_t)o.N, (uint64_t)o.M, (uint64_t)row_bytes, 64 / sizeof(T), 32, CU_TENSOR_MAP_SWIZZLE_64B));
+  else
+    mo = ma;
+  const int64_t total = (int64_t)p.mt * p.nt;
+  if (total > 0x7fffffff - 4096) return fail(ATS_EUNSUPPORTED, "int8_linear: too many tiles");
+  const int grid = total < gemm_ctas() ? (int)total : gemm_ctas();
+  const int smem = 1024 + tile_stages(BN) * tile_stage_bytes(BN) + kEpiWarps * kBoxesPerWarp * kBox;
+  return launch_after(int8_tile_kernel<T, BN>, dim3((unsigned)grid), kTileThreads, smem, 1, st, "int8_tile", ma, mb, mo, p);
+}
+
+template <typename T, int TN>
+int parts(const int8_t* q, int64_t ldq, const int8_t* w, int64_t ldw, const Out& o, int K, int split, cudaStream_t st) {
+  CUtensorMap mw, mx;
+  ATS_TRY(operand_map(&mw, w, K, o.N, ldw, BM));
+  ATS_TRY(operand_map(&mx, q, K, o.M, ldq, TN));
+  const dim3 grid((unsigned)((o.N + BM - 1) / BM), (unsigned)((o.M + TN - 1) / TN), (unsigned)split);
+  const int smem = 1024 + part_stages(TN) * part_stage_bytes(TN);
+  return launch_after(int8_part_kernel<T, TN>, grid, kPartThreads, smem, split, st, "int8_part", mw, mx, o,
+                      (K + BKB - 1) / BKB);
+}
+
+template <typename T>
+int linear(const void* x, int64_t ldx, const int8_t* w, int64_t ldw, Out o, int64_t K, int8_t* q, float* sx,
+           cudaStream_t st) {
+  if (o.M <= kDotTokens && o.M * padded_k(K) <= kDotSmem / 2) return dot<T>(x, ldx, w, ldw, o, (int)K, st);
+  const int64_t ldq = padded_k(K);
+  ATS_TRY(quantize_t<T>(x, ldx, q, ldq, sx, o.M, K, st));
+  o.sx = sx;
+  const int64_t nt = (o.N + BM - 1) / BM;
+  const int kb = (int)((K + BKB - 1) / BKB);
+  // Few tokens: as many columns as hold them, and K split until the SMs are busy (each part keeps 2 blocks).
+  const int tn = o.M <= 16 ? 16 : o.M <= 32 ? 32 : o.M <= 64 ? 64 : 128;
+  const int64_t part_tiles = nt * ((o.M + tn - 1) / tn);
+  if (part_tiles <= num_sms() && (o.M + tn - 1) / tn <= 65535) {
+    int split = 1;
+    while (split < 8 && part_tiles * split * 2 <= num_sms() && kb >= split * 4) split *= 2;
+    switch (tn) {
+      case 16: return parts<T, 16>(q, ldq, w, ldw, o, (int)K, split, st);
+      case 32: return parts<T, 32>(q, ldq, w, ldw, o, (int)K, split, st);
+      case 64: return parts<T, 64>(q, ldq, w, ldw, o, (int)K, split, st);
+      default: return parts<T, 128>(q, ldq, w, ldw, o, (int)K, split, st);
+    }
+  }
+  return o.N > 128 ? tiles<T, 256>(q, ldq, w, ldw, o, (int)K, st) : tiles<T, 128>(q, ldq, w, ldw, o, (int)K, st);
+}
+
 }  // namespace
+
+int int8_set_wait_budget(long long cycles) {
+  const long long v = cycles > 0 ? cycles : kWaitBudget;
+  cudaError_t e = cudaMemcpyToSymbol(g_int8_wait_budget, &v, sizeof(v));
+  if (e != cudaSuccess) return fail(ATS_ECUDA, "set_wait_budget (int8): %s", cudaGetErrorString(e));
+  return ATS_OK;
+}
+
+int int8_take_status(int* code) {
+  const int zero = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(code, g_int8_status, sizeof(int));
+  if (e == cudaSuccess && *code != 0) e = cudaMemcpyToSymbol(g_int8_status, &zero, sizeof(int));
+  if (e != cudaSuccess) return fail(ATS_ECUDA, "device_status (int8): %s", cudaGetErrorString(e));
+  return ATS_OK;
+}
+
 }  // namespace ats
 
 using namespace ats;
@@ -131,7 +821,7 @@ extern "C" {
 int ats_int8_quantize(const void* x, int64_t x_row_stride, ats_dtype dtype, void* q, int64_t q_row_stride,
                       float* scale, int64_t rows, int64_t K, void* stream) {
   if (dtype != ATS_F32 && dtype != ATS_BF16) return fail(ATS_EBADARG, "int8_quantize: dtype");
-  if (rows < 0 || rows > 0x7fffffff || K < 1 || K > kMaxK || q_row_stride < K || x_row_stride < 0)
+  if (rows < 0 || rows > kMaxRows || K < 1 || K > kMaxK || q_row_stride < K || x_row_stride < 0)
     return fail(ATS_EBADARG, "int8_quantize: rows=%lld K=%lld (at most %d) row stride %lld", (long long)rows,
                 (long long)K, kMaxK, (long long)q_row_stride);
   if (rows == 0) return ATS_OK;
@@ -152,7 +842,7 @@ int ats_int8_linear(const void* x, int64_t x_row_stride, ats_dtype dtype, const 
   if (dtype != ATS_F32 && dtype != ATS_BF16) return fail(ATS_EBADARG, "int8_linear: dtype");
   if (bias != nullptr && bias_dtype != ATS_F32 && bias_dtype != ATS_BF16)
     return fail(ATS_EBADARG, "int8_linear: bias dtype");
-  if (M < 0 || M > 0x7fffffff || N < 1 || N > 0x7fffffff || K < 1 || K > kMaxK || x_row_stride < 0)
+  if (M < 0 || M > kMaxRows || N < 1 || N > kMaxRows || K < 1 || K > kMaxK || x_row_stride < 0)
     return fail(ATS_EBADARG, "int8_linear: M=%lld N=%lld K=%lld (K at most %d)", (long long)M, (long long)N,
                 (long long)K, kMaxK);
   if (w_row_stride < K || w_row_stride % 16 != 0 || !aligned16(w))
@@ -165,19 +855,11 @@ int ats_int8_linear(const void* x, int64_t x_row_stride, ats_dtype dtype, const 
     return fail(ATS_EBADARG, "int8_linear: workspace too small");
   int8_t* q = static_cast<int8_t*>(workspace);
   float* sx = reinterpret_cast<float*>(q + q_bytes(M, K));
-  const int64_t ldq = padded_k(K);
-  cudaStream_t st = (cudaStream_t)stream;
-  ATS_TRY(ats_int8_quantize(x, x_row_stride, dtype, q, ldq, sx, M, K, stream));
-  const int64_t mt = (M + kTok - 1) / kTok;
-  const dim3 grid((unsigned)((N + kDotWarps - 1) / kDotWarps), (unsigned)(mt < 65535 ? mt : 65535));
   const int8_t* wp = static_cast<const int8_t*>(w);
-  if (dtype == ATS_BF16)
-    int8_dot_kernel<bf16><<<grid, 32 * kDotWarps, 0, st>>>(q, ldq, sx, wp, w_row_stride, w_scale, bias,
-                                                         bias_dtype == ATS_BF16, static_cast<bf16*>(y), M, N, (int)K);
-  else
-    int8_dot_kernel<float><<<grid, 32 * kDotWarps, 0, st>>>(q, ldq, sx, wp, w_row_stride, w_scale, bias,
-                                                          bias_dtype == ATS_BF16, static_cast<float*>(y), M, N, (int)K);
-  return check_launch("int8_dot");
+  const Out o{y, nullptr, w_scale, bias, bias_dtype == ATS_BF16, (int)M, (int)N};
+  cudaStream_t st = (cudaStream_t)stream;
+  return dtype == ATS_BF16 ? linear<bf16>(x, x_row_stride, wp, w_row_stride, o, K, q, sx, st)
+                           : linear<float>(x, x_row_stride, wp, w_row_stride, o, K, q, sx, st);
 }
 
 }  // extern "C"
