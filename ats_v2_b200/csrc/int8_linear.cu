@@ -53,75 +53,110 @@ __device__ __forceinline__ int quant(float v, float inv) {
   return r == r ? (int)fminf(fmaxf(r, -127.f), 127.f) : 0;
 }
 
-// 16 consecutive values of a row from element k; those at or past K are zero.
+// 16 consecutive values of a row from element k, as they are stored; those at or past K are zero.
 template <typename T, bool VEC>
-__device__ __forceinline__ void load16(const T* row, int k, int K, float (&v)[16]) {
+__device__ __forceinline__ void load16(const T* row, int k, int K, uint4 (&v)[sizeof(T)]) {
   if (VEC && k + 16 <= K) {
-    load_n<T, 16>(row + k, v);
-  } else {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = k + i < K ? Cvt<T>::to_f(row[k + i]) : 0.f;
+    for (int i = 0; i < (int)sizeof(T); ++i) v[i] = reinterpret_cast<const uint4*>(row + k)[i];
+  } else {
+    T e[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) e[i] = k + i < K ? row[k + i] : Cvt<T>::from_f(0.f);
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T); ++i) v[i] = reinterpret_cast<const uint4*>(e)[i];
   }
 }
 
-__device__ __forceinline__ uint32_t max16(const float (&v)[16], uint32_t m) {
+template <typename T>
+__device__ __forceinline__ uint32_t max16(const uint4 (&v)[sizeof(T)], uint32_t m) {
+  const T* e = reinterpret_cast<const T*>(v);
 #pragma unroll
-  for (int i = 0; i < 16; ++i) m = max(m, abs_bits(v[i]));
+  for (int i = 0; i < 16; ++i) m = max(m, abs_bits(Cvt<T>::to_f(e[i])));
   return m;
 }
 
-__device__ __forceinline__ uint4 quant16(const float (&v)[16], float inv) {
+__device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d, float inv) {
+  return (uint32_t)(quant(a, inv) & 255) | (uint32_t)(quant(b, inv) & 255) << 8 |
+         (uint32_t)(quant(c, inv) & 255) << 16 | (uint32_t)(quant(d, inv) & 255) << 24;
+}
+
+template <typename T>
+__device__ __forceinline__ uint4 quant16(const uint4 (&v)[sizeof(T)], float inv) {
+  const T* e = reinterpret_cast<const T*>(v);
   uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    w[i] = (uint32_t)(quant(v[4 * i], inv) & 255) | (uint32_t)(quant(v[4 * i + 1], inv) & 255) << 8 |
-           (uint32_t)(quant(v[4 * i + 2], inv) & 255) << 16 | (uint32_t)(quant(v[4 * i + 3], inv) & 255) << 24;
+    w[i] = pack4(Cvt<T>::to_f(e[4 * i]), Cvt<T>::to_f(e[4 * i + 1]), Cvt<T>::to_f(e[4 * i + 2]),
+                 Cvt<T>::to_f(e[4 * i + 3]), inv);
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// G threads to a row (a warp, or the whole block of 256), each with 16 consecutive values per step and the first
-// kKeep steps held in registers; a longer row is read again.  q rows are written in 16-byte pieces where they are
-// aligned for it (Q16), zeros up to the next multiple of 16 at most ldq.
-constexpr int kQuantThreads = 256, kKeep = 2;
+// 4 values from element k, zero at or past K; vec: the row is aligned to 4 elements.
+template <typename T>
+__device__ __forceinline__ void load4(const T* row, int k, int K, int vec, float (&v)[4]) {
+  if (vec && k + 4 <= K) {
+    if constexpr (sizeof(T) == 2) {
+      const uint2 raw = *reinterpret_cast<const uint2*>(row + k);
+      const T* e = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = Cvt<T>::to_f(e[i]);
+    } else {
+      load_n<T, 4>(row + k, v);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = k + i < K ? Cvt<T>::to_f(row[k + i]) : 0.f;
+  }
+}
+
+// G threads to a row (a warp, or all of a block), each with 16 consecutive values per step and the first kKeep steps
+// held in registers; a longer row is read again.  q rows are written in 16-byte pieces where they are aligned for it
+// (Q16), zeros up to the next multiple of 16 at most ldq.
+constexpr int kKeep = 4;
 
 template <typename T, int G, bool VEC, bool Q16>
-__global__ void __launch_bounds__(kQuantThreads) int8_quantize_kernel(const T* __restrict__ x, int64_t ldx,
-                                                                     int8_t* __restrict__ q, int64_t ldq,
-                                                                     float* __restrict__ scale, int64_t rows, int K) {
+__global__ void __launch_bounds__(G < 128 ? 128 : G) int8_quantize_kernel(const T* __restrict__ x, int64_t ldx,
+                                                                         int8_t* __restrict__ q, int64_t ldq,
+                                                                         float* __restrict__ scale, int64_t rows,
+                                                                         int K) {
+  constexpr int THREADS = G < 128 ? 128 : G;
+  // In this order: a dependent kernel reads its weights before its own wait, and what wrote them has ended by now.
+  tc::wait_prerequisites();
   tc::launch_dependents();
-  __shared__ uint32_t red[kQuantThreads / 32];
-  const int64_t row = (int64_t)blockIdx.x * (kQuantThreads / G) + threadIdx.x / G;
+  __shared__ uint32_t red[THREADS / 32];
+  const int64_t row = (int64_t)blockIdx.x * (THREADS / G) + threadIdx.x / G;
   const int t = threadIdx.x % G;
   if (G == 32 && row >= rows) return;
   const T* xr = x + row * ldx;
-  float v[kKeep][16];
+  uint4 raw[kKeep][sizeof(T)];  // 16 values of T
   uint32_t m = 0;
 #pragma unroll
   for (int j = 0; j < kKeep; ++j) {
     const int k = (j * G + t) * 16;
-    if (k < K) {
-      load16<T, VEC>(xr, k, K, v[j]);
-      m = max16(v[j], m);
-    }
+    if (k < K) load16<T, VEC>(xr, k, K, raw[j]);
   }
+#pragma unroll
+  for (int j = 0; j < kKeep; ++j)
+    if ((j * G + t) * 16 < K) m = max16<T>(raw[j], m);
   for (int k = (kKeep * G + t) * 16; k < K; k += G * 16) {
-    float u[16];
+    uint4 u[sizeof(T)];
     load16<T, VEC>(xr, k, K, u);
-    m = max16(u, m);
+    m = max16<T>(u, m);
   }
   m = __reduce_max_sync(0xffffffffu, m);
   if (G > 32) {
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kQuantThreads / 32; ++i) m = max(m, red[i]);
+    for (int i = 0; i < G / 32; ++i) m = max(m, red[i]);
   }
   float inv;
   const float s = row_scale(m, inv);
   if (t == 0) scale[row] = s;
   int8_t* qr = q + row * ldq;
-  auto put = [&](int k, const float (&u)[16]) {
-    const uint4 w = quant16(u, inv);
+  auto put = [&](int k, const uint4 (&u)[sizeof(T)]) {
+    const uint4 w = quant16<T>(u, inv);
     if (Q16) {
       *reinterpret_cast<uint4*>(qr + k) = w;
     } else {
@@ -134,36 +169,69 @@ __global__ void __launch_bounds__(kQuantThreads) int8_quantize_kernel(const T* _
 #pragma unroll
   for (int j = 0; j < kKeep; ++j) {
     const int k = (j * G + t) * 16;
-    if (k < K) put(k, v[j]);
+    if (k < K) put(k, raw[j]);
   }
   for (int k = (kKeep * G + t) * 16; k < K; k += G * 16) {
-    float u[16];
+    uint4 u[sizeof(T)];
     load16<T, VEC>(xr, k, K, u);
     put(k, u);
   }
   for (int64_t k = (K + 15) / 16 * 16 + t; k < ldq; k += G) qr[k] = 0;
 }
 
+// Launch whose prologue may start before the stream's previous kernel has ended (every kernel here waits for it with
+// wait_prerequisites); cluster_z CTAs along z are one cluster.
+template <typename F, typename... A>
+int launch_after(F kernel, dim3 grid, int threads, int smem, int cluster_z, cudaStream_t st, const char* what,
+                 A... args) {
+  // All with one shared-memory split: an SM that has to change it between two kernels first drains.
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                       cudaSharedmemCarveoutMaxShared);
+  if (e == cudaSuccess && smem > 48 * 1024)
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return fail(ATS_ECUDA, "%s: %s", what, cudaGetErrorString(e));
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 1;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = (unsigned)cluster_z;
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster_z > 1 ? 2 : 1;
+  e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  if (e != cudaSuccess) return fail(ATS_ECUDA, "%s: %s", what, cudaGetErrorString(e));
+  return check_launch(what);
+}
+
 template <typename T, int G>
 int quantize_g(const T* x, int64_t ldx, int8_t* q, int64_t ldq, float* scale, int64_t rows, int K, cudaStream_t st) {
   const bool vec = aligned16(x) && ldx % Chunk<T>::N == 0, q16 = aligned16(q) && ldq % 16 == 0;
-  const int64_t per = kQuantThreads / G;
+  constexpr int THREADS = G < 128 ? 128 : G;
+  const int64_t per = THREADS / G;
   const unsigned grid = (unsigned)((rows + per - 1) / per);
-  if (vec && q16) int8_quantize_kernel<T, G, true, true><<<grid, kQuantThreads, 0, st>>>(x, ldx, q, ldq, scale, rows, K);
-  else if (vec) int8_quantize_kernel<T, G, true, false><<<grid, kQuantThreads, 0, st>>>(x, ldx, q, ldq, scale, rows, K);
-  else if (q16) int8_quantize_kernel<T, G, false, true><<<grid, kQuantThreads, 0, st>>>(x, ldx, q, ldq, scale, rows, K);
-  else int8_quantize_kernel<T, G, false, false><<<grid, kQuantThreads, 0, st>>>(x, ldx, q, ldq, scale, rows, K);
-  return check_launch("int8_quantize");
+  auto go = [&](auto kernel) {
+    return launch_after(kernel, dim3(grid), THREADS, 0, 1, st, "int8_quantize", x, ldx, q, ldq, scale, rows, K);
+  };
+  if (vec) return q16 ? go(int8_quantize_kernel<T, G, true, true>) : go(int8_quantize_kernel<T, G, true, false>);
+  return q16 ? go(int8_quantize_kernel<T, G, false, true>) : go(int8_quantize_kernel<T, G, false, false>);
 }
 
-// A warp per row where the row fits its registers, a block per row beyond.
+// As many threads as hold the row in their registers: 32, 128 or 512 (8192x2048 bf16: 9.0 us with a warp a row,
+// 18.4 us with 256 threads).
 template <typename T>
 int quantize_t(const void* x, int64_t ldx, void* q, int64_t ldq, float* scale, int64_t rows, int64_t K,
                cudaStream_t st) {
   auto* xp = static_cast<const T*>(x);
   auto* qp = static_cast<int8_t*>(q);
-  return K <= 32 * 16 * kKeep ? quantize_g<T, 32>(xp, ldx, qp, ldq, scale, rows, (int)K, st)
-                              : quantize_g<T, kQuantThreads>(xp, ldx, qp, ldq, scale, rows, (int)K, st);
+  if (K <= 32 * 16 * kKeep) return quantize_g<T, 32>(xp, ldx, qp, ldq, scale, rows, (int)K, st);
+  if (K <= 128 * 16 * kKeep) return quantize_g<T, 128>(xp, ldx, qp, ldq, scale, rows, (int)K, st);
+  return quantize_g<T, 512>(xp, ldx, qp, ldq, scale, rows, (int)K, st);
 }
 
 // ------------------------------------------------------------------ epilogue
@@ -181,24 +249,25 @@ __device__ __forceinline__ float bias_at(const Out& o, int n) {
   return o.bias_bf16 ? __bfloat162float(static_cast<const bf16*>(o.bias)[n]) : static_cast<const float*>(o.bias)[n];
 }
 
-// ------------------------------------------------------- one to kDotTokens tokens
-// One launch: every block quantises the tokens into its shared memory (they come from L2), with the first weights
-// of its warps already in flight, then a warp takes an output channel at a time: 16 weights per lane and step
-// against the tokens' integers.  The weights are read once, at full width; they bound it.
-constexpr int kDotTokens = 4, kDotThreads = 256, kDotStep = 8;
-constexpr int kDotSmem = 96 * 1024;
+// --------------------------------------------------------------- one token
+// One launch: every block quantises the token into its shared memory (it comes from L2), with the first weights of
+// its warps already in flight, then a warp takes an output channel at a time: 16 weights per lane and step against
+// the token's integers.  The weights are read once; they bound it.
+constexpr int kDotThreads = 256, kDotStep = 8;
+constexpr int kDotSmem = 48 * 1024;  // longest token, in bytes
 
-template <typename T, int MT>
-__global__ void __launch_bounds__(kDotThreads) int8_dot_kernel(const T* __restrict__ x, int64_t ldx,
-                                                              const int8_t* __restrict__ w, int64_t ldw, Out o, int K,
-                                                              int vec) {
-  extern __shared__ __align__(16) int8_t qs[];  // [MT][Kp]
-  __shared__ uint32_t red[MT][kDotThreads / 32];
+template <typename T>
+__global__ void __launch_bounds__(kDotThreads, 4) int8_dot_kernel(const T* __restrict__ x,
+                                                                 const int8_t* __restrict__ w, int64_t ldw, Out o,
+                                                                 int K, int vec) {
+  extern __shared__ __align__(16) int8_t qs[];  // [Kp]
+  __shared__ uint32_t red[kDotThreads / 32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int full = K / 16, Kp = (K + 15) / 16 * 16;
   const int64_t stride = (int64_t)gridDim.x * (kDotThreads / 32);
   int64_t n = (int64_t)blockIdx.x * (kDotThreads / 32) + warp;
   uint4 wv[kDotStep];
+  tc::wait_prerequisites();
   auto load = [&](int64_t row, int c0) {
     const int8_t* p = w + row * ldw;
 #pragma unroll
@@ -209,77 +278,54 @@ __global__ void __launch_bounds__(kDotThreads) int8_dot_kernel(const T* __restri
   };
   if (n < o.N) load(n, 0);
 
-  uint32_t m[MT] = {};
-  for (int k = threadIdx.x * 16; k < K; k += kDotThreads * 16)
+  uint32_t m = 0;
+#pragma unroll 4
+  for (int k = threadIdx.x * 4; k < K; k += kDotThreads * 4) {
+    float v[4];
+    load4<T>(x, k, K, vec, v);
 #pragma unroll
-    for (int t = 0; t < MT; ++t)
-      if (t < o.M) {
-        float v[16];
-        if (vec) load16<T, true>(x + t * ldx, k, K, v);
-        else load16<T, false>(x + t * ldx, k, K, v);
-        m[t] = max16(v, m[t]);
-      }
-#pragma unroll
-  for (int t = 0; t < MT; ++t) {
-    m[t] = __reduce_max_sync(0xffffffffu, m[t]);
-    if (lane == 0) red[t][warp] = m[t];
+    for (int i = 0; i < 4; ++i) m = max(m, abs_bits(v[i]));
   }
+  m = __reduce_max_sync(0xffffffffu, m);
+  if (lane == 0) red[warp] = m;
   __syncthreads();
-  float sx[MT], inv[MT];
 #pragma unroll
-  for (int t = 0; t < MT; ++t) {
-#pragma unroll
-    for (int i = 0; i < kDotThreads / 32; ++i) m[t] = max(m[t], red[t][i]);
-    sx[t] = row_scale(m[t], inv[t]);
+  for (int i = 0; i < kDotThreads / 32; ++i) m = max(m, red[i]);
+  float inv;
+  const float sx = row_scale(m, inv);
+#pragma unroll 4
+  for (int k = threadIdx.x * 4; k < Kp; k += kDotThreads * 4) {
+    float v[4];
+    load4<T>(x, k, K, vec, v);
+    *reinterpret_cast<uint32_t*>(qs + k) = pack4(v[0], v[1], v[2], v[3], inv);
   }
-  for (int k = threadIdx.x * 16; k < K; k += kDotThreads * 16)
-#pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      float v[16] = {};
-      if (t < o.M) {
-        if (vec) load16<T, true>(x + t * ldx, k, K, v);
-        else load16<T, false>(x + t * ldx, k, K, v);
-      }
-      *reinterpret_cast<uint4*>(qs + t * Kp + k) = quant16(v, inv[t]);
-    }
   __syncthreads();
 
   for (; n < o.N; n += stride) {
-    int acc[MT] = {};
+    int acc = 0;
     for (int c0 = 0; c0 < full; c0 += kDotStep * 32) {
-      uint4 cur[kDotStep];
-#pragma unroll
-      for (int j = 0; j < kDotStep; ++j) cur[j] = wv[j];
-      // the next weights of this channel, or the first of the warp's next one
-      if (c0 + kDotStep * 32 < full) load(n, c0 + kDotStep * 32);
-      else if (n + stride < o.N) load(n + stride, 0);
 #pragma unroll
       for (int j = 0; j < kDotStep; ++j) {
         const int c = c0 + j * 32 + lane;
         if (c < full) {
-#pragma unroll
-          for (int t = 0; t < MT; ++t) {
-            const uint4 qv = *reinterpret_cast<const uint4*>(qs + t * Kp + c * 16);
-            acc[t] = __dp4a((int)cur[j].x, (int)qv.x, acc[t]);
-            acc[t] = __dp4a((int)cur[j].y, (int)qv.y, acc[t]);
-            acc[t] = __dp4a((int)cur[j].z, (int)qv.z, acc[t]);
-            acc[t] = __dp4a((int)cur[j].w, (int)qv.w, acc[t]);
-          }
+          const uint4 qv = *reinterpret_cast<const uint4*>(qs + c * 16);
+          acc = __dp4a((int)wv[j].x, (int)qv.x, acc);
+          acc = __dp4a((int)wv[j].y, (int)qv.y, acc);
+          acc = __dp4a((int)wv[j].z, (int)qv.z, acc);
+          acc = __dp4a((int)wv[j].w, (int)qv.w, acc);
         }
       }
+      // the next weights of this channel, or the first of the warp's next one
+      if (c0 + kDotStep * 32 < full) load(n, c0 + kDotStep * 32);
+      else if (n + stride < o.N) load(n + stride, 0);
     }
     const int k = full * 16 + lane;
-    if (lane < 16 && k < K)
-#pragma unroll
-      for (int t = 0; t < MT; ++t) acc[t] += (int)w[n * ldw + k] * (int)qs[t * Kp + k];
-#pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      const int a = warp_sum_i(acc[t]);
-      if (lane == t && t < o.M) {
-        float v = (float)a * (sx[t] * o.sw[n]);
-        if (o.bias != nullptr) v += bias_at(o, (int)n);
-        static_cast<T*>(o.y)[(int64_t)t * o.N + n] = Cvt<T>::from_f(v);
-      }
+    if (lane < 16 && k < K) acc += (int)w[n * ldw + k] * (int)qs[k];
+    acc = warp_sum_i(acc);
+    if (lane == 0) {
+      float v = (float)acc * (sx * o.sw[n]);
+      if (o.bias != nullptr) v += bias_at(o, (int)n);
+      static_cast<T*>(o.y)[n] = Cvt<T>::from_f(v);
     }
   }
 }
@@ -436,13 +482,20 @@ __global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid
       const int acc = i & 1;
       const int row0 = m * BM + quad * 32, row = row0 + lane;
       const float sx = row < p.o.M ? p.o.sx[row] : 0.f;
+      float sw[BN / 64], bw[BN / 64];  // of column lane + 32 j of the warp's half, in flight during the wait
+#pragma unroll
+      for (int j = 0; j < BN / 64; ++j) {
+        const int col = n * BN + chalf * (BN / 2) + j * 32 + lane;
+        sw[j] = col < p.o.N ? p.o.sw[col] : 0.f;
+        bw[j] = col < p.o.N ? bias_at(p.o, col) : 0.f;
+      }
       if (!tc::mbar_wait(&tfull_bar[acc], (uint32_t)(i >> 1) & 1u, &abort_flag, budget)) {
         give_up(&abort_flag, 34);
         break;
       }
       tc::tc_fence_after();
       const uint32_t t_row = tmem_base + (uint32_t)(acc * BN + chalf * (BN / 2)) + ((uint32_t)(quad * 32) << 16);
-#pragma unroll 1
+#pragma unroll
       for (int c = 0; c < BN / 2; c += BOX_COLS) {
         const int col0 = n * BN + chalf * (BN / 2) + c;
         float v[BOX_COLS];
@@ -450,13 +503,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid
         for (int h = 0; h < BOX_COLS; h += 16) {
           uint32_t r[16];
           tc::tmem_ld16(t_row + c + h, r);
-          const int colw = col0 + h + (lane & 15);
-          const float sw = colw < p.o.N ? p.o.sw[colw] : 0.f;
-          const float bw = colw < p.o.N ? bias_at(p.o, colw) : 0.f;
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
-            v[h + j] = (float)(int)r[j] * (sx * __shfl_sync(0xffffffffu, sw, j));
-            if (p.o.bias != nullptr) v[h + j] += __shfl_sync(0xffffffffu, bw, j);
+            v[h + j] = (float)(int)r[j] * (sx * __shfl_sync(0xffffffffu, sw[(c + h) / 32], (c + h) % 32 + j));
+            if (p.o.bias != nullptr) v[h + j] += __shfl_sync(0xffffffffu, bw[(c + h) / 32], (c + h) % 32 + j);
           }
         }
         uint8_t* box = boxes + (puts % kBoxesPerWarp) * kBox;
@@ -507,15 +557,72 @@ __global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid
 // its part of K in TMEM, puts its int32 tile into its shared memory, and every CTA adds the parts of its share of
 // the tokens through distributed shared memory.  So a decoding batch reads the weights with every SM, and no
 // workspace or atomics are needed.  The weights' loads start before the quantisation has ended.
-constexpr int kPartThreads = 192;
+constexpr int kPartThreads = 64 + 32 * kEpiWarps, kMaxSplit = 8;
 
+// Two CTAs of a part kernel share an SM: about 100 KB of ring each.
 __host__ __device__ constexpr int part_stage_bytes(int tn) { return (BM + tn) * BKB; }
-__host__ __device__ constexpr int part_stages(int tn) { return 200 * 1024 / part_stage_bytes(tn) < 8 ? 200 * 1024 / part_stage_bytes(tn) : 8; }
+__host__ __device__ constexpr int part_stages(int tn) { return 100 * 1024 / part_stage_bytes(tn); }
+
+struct PartOut {
+  const int* tile;                     // [TN][128] sums of this CTA's part of K
+  const float *sx_s, *sw_s, *bw_s;
+  int n0, m0, first, share, vec_out;  // tokens [first, first + share) of the tile are this CTA's
+};
+
+// Add the S parts of this CTA's tokens and write them: a warp takes tokens, a lane four channels, with 8 reads in
+// flight (a read of another CTA's shared memory takes hundreds of cycles).
+template <typename T, int S>
+__device__ __forceinline__ void reduce_parts(const Out& o, const PartOut& p) {
+  constexpr int U = kMaxSplit / S, W = kPartThreads / 32;
+  const int warp = threadIdx.x >> 5, r4 = (threadIdx.x & 31) * 4, n = p.n0 + r4;
+  const float4 sw = *reinterpret_cast<const float4*>(p.sw_s + r4), bw = *reinterpret_cast<const float4*>(p.bw_s + r4);
+  const bool whole = p.vec_out && n + 4 <= o.N;
+  uint32_t base[S];
+#pragma unroll
+  for (int z = 0; z < S; ++z) {
+    const uint32_t mine = tc::smem_u32(p.tile + p.first * BM + r4);
+    base[z] = S == 1 ? mine : tc::cluster_addr(mine, (uint32_t)z);
+  }
+  const int left = o.M - p.m0 - p.first;
+  const int share = p.share < left ? p.share : left;
+  for (int i0 = warp; i0 < share; i0 += U * W) {
+    int4 b[U][S];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * W < share ? i0 + u * W : i0;
+#pragma unroll
+      for (int z = 0; z < S; ++z)
+        b[u][z] = S == 1 ? *reinterpret_cast<const int4*>(p.tile + (p.first + i) * BM + r4)
+                         : tc::ld_cluster_v4(base[z] + (uint32_t)i * BM * 4u);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * W;
+      int4 a = b[u][0];
+#pragma unroll
+      for (int z = 1; z < S; ++z) a.x += b[u][z].x, a.y += b[u][z].y, a.z += b[u][z].z, a.w += b[u][z].w;
+      const float sx = i < share ? p.sx_s[p.first + i] : 0.f;
+      float v[4] = {(float)a.x * (sx * sw.x), (float)a.y * (sx * sw.y), (float)a.z * (sx * sw.z),
+                    (float)a.w * (sx * sw.w)};
+      if (o.bias != nullptr) v[0] += bw.x, v[1] += bw.y, v[2] += bw.z, v[3] += bw.w;
+      T* y = static_cast<T*>(o.y) + (int64_t)(p.m0 + p.first + i) * o.N + n;
+      if (whole && i < share) {
+        T e[4] = {Cvt<T>::from_f(v[0]), Cvt<T>::from_f(v[1]), Cvt<T>::from_f(v[2]), Cvt<T>::from_f(v[3])};
+        if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(y) = *reinterpret_cast<const uint2*>(e);
+        else *reinterpret_cast<uint4*>(y) = *reinterpret_cast<const uint4*>(e);
+      } else if (i < share) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (n + j < o.N) y[j] = Cvt<T>::from_f(v[j]);
+      }
+    }
+  }
+}
 
 template <typename T, int TN>
-__global__ void __launch_bounds__(kPartThreads, 1) int8_part_kernel(const __grid_constant__ CUtensorMap tmW,
+__global__ void __launch_bounds__(kPartThreads, 2) int8_part_kernel(const __grid_constant__ CUtensorMap tmW,
                                                                    const __grid_constant__ CUtensorMap tmX, Out o,
-                                                                   int kb_all) {
+                                                                   int kb_all, int vec_out) {
   constexpr int STAGE = part_stage_bytes(TN), NST = part_stages(TN);
   constexpr int TCOLS = TN < 32 ? 32 : TN;
   constexpr uint32_t IDESC = tc::idesc_i8(BM, TN);
@@ -524,6 +631,8 @@ __global__ void __launch_bounds__(kPartThreads, 1) int8_part_kernel(const __grid
   __shared__ __align__(8) uint64_t full_bar[NST], empty_bar[NST], tfull_bar;
   __shared__ uint32_t tmem_base_s;
   __shared__ volatile int abort_flag;
+  __shared__ float sx_s[TN];
+  __shared__ __align__(16) float sw_s[BM], bw_s[BM];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long budget = g_int8_wait_budget;
   const int split = (int)gridDim.z, part = (int)blockIdx.z;  // the cluster is all of z
@@ -598,65 +707,35 @@ __global__ void __launch_bounds__(kPartThreads, 1) int8_part_kernel(const __grid
     }
   }
   __syncwarp();
-  tc::wait_prerequisites();  // the scales
+  if (warp >= 2 && warp < 6) {
+    const int r = threadIdx.x - 64, n = n0 + r;
+    sw_s[r] = n < o.N ? o.sw[n] : 0.f;
+    bw_s[r] = n < o.N ? bias_at(o, n) : 0.f;
+    tc::wait_prerequisites();  // the tokens' scales
+    if (r < TN) sx_s[r] = m0 + r < o.M ? o.sx[m0 + r] : 0.f;
+  }
   if (!tc::mbar_wait(&tfull_bar, 0u, nullptr, kWaitBudget)) atomicCAS(&g_int8_status, 0, 44);
   tc::tc_fence_after();
-  const int n_here = warp >= 2 ? n0 + (warp & 3) * 32 + lane : 0;
-  if (split == 1) {
-    if (warp >= 2) {  // thread = channel, columns = tokens: a warp's stores run along the channels
-      const float sw = n_here < o.N ? o.sw[n_here] : 0.f, bw = n_here < o.N ? bias_at(o, n_here) : 0.f;
-#pragma unroll 1
-      for (int c = 0; c < TN; c += 16) {
-        uint32_t r[16];
-        tc::tmem_ld16(tmem_base + (uint32_t)c + ((uint32_t)((warp & 3) * 32) << 16), r);
+  int* tile = reinterpret_cast<int*>(ring);  // [TN][128]: the ring is no longer read or written
+  if (warp >= 2) {
+#pragma unroll 2
+    for (int c = (warp - 2) / 4 * 16; c < TN; c += 32) {  // two warps per TMEM lane quadrant
+      uint32_t r[16];
+      tc::tmem_ld16(tmem_base + (uint32_t)c + ((uint32_t)((warp & 3) * 32) << 16), r);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const int m = m0 + c + j;
-          if (m < o.M && n_here < o.N) {
-            float v = (float)(int)r[j] * (o.sx[m] * sw);
-            if (o.bias != nullptr) v += bw;
-            static_cast<T*>(o.y)[(int64_t)m * o.N + n_here] = Cvt<T>::from_f(v);
-          }
-        }
-      }
+      for (int j = 0; j < 16; ++j) tile[(c + j) * BM + (warp & 3) * 32 + lane] = (int)r[j];
     }
-  } else {
-    int* tile = reinterpret_cast<int*>(ring);  // [TN][128]: the ring is no longer read or written
-    if (warp >= 2) {
-#pragma unroll 1
-      for (int c = 0; c < TN; c += 16) {
-        uint32_t r[16];
-        tc::tmem_ld16(tmem_base + (uint32_t)c + ((uint32_t)((warp & 3) * 32) << 16), r);
-#pragma unroll
-        for (int j = 0; j < 16; ++j) tile[(c + j) * BM + (warp & 3) * 32 + lane] = (int)r[j];
-      }
-    }
-    __syncwarp();
-    tc::cluster_sync();
-    const int share = TN / split;  // tokens of this CTA
-    for (int i = threadIdx.x; i < share * (BM / 4); i += kPartThreads) {
-      const int t = part * share + i / (BM / 4), r4 = i % (BM / 4) * 4;
-      const int m = m0 + t, n = n0 + r4;
-      if (m >= o.M || n >= o.N) continue;
-      int4 a = make_int4(0, 0, 0, 0);
-      const uint32_t mine = tc::smem_u32(tile + t * BM + r4);
-      for (int z = 0; z < split; ++z) {
-        const int4 b = tc::ld_cluster_v4(tc::cluster_addr(mine, (uint32_t)z));
-        a.x += b.x, a.y += b.y, a.z += b.z, a.w += b.w;
-      }
-      const float sx = o.sx[m];
-      const int e[4] = {a.x, a.y, a.z, a.w};
-      T* y = static_cast<T*>(o.y) + (int64_t)m * o.N + n;
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (n + j < o.N) {
-          float v = (float)e[j] * (sx * o.sw[n + j]);
-          if (o.bias != nullptr) v += bias_at(o, n + j);
-          y[j] = Cvt<T>::from_f(v);
-        }
-    }
-    tc::cluster_sync();  // no CTA leaves while another reads its tile
   }
+  __syncwarp();
+  if (split > 1) tc::cluster_sync();
+  else __syncthreads();
+  const PartOut po{tile, sx_s, sw_s, bw_s, n0, m0, part * (TN / split), TN / split, vec_out};
+  if (split == 1) reduce_parts<T, 1>(o, po);
+  else if (split == 2) reduce_parts<T, 2>(o, po);
+  else if (split == 4) reduce_parts<T, 4>(o, po);
+  else reduce_parts<T, 8>(o, po);
+  __syncwarp();
+  if (split > 1) tc::cluster_sync();  // no CTA leaves while another reads its tile
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
@@ -697,46 +776,13 @@ int operand_map(CUtensorMap* m, const void* base, int64_t K, int64_t rows, int64
                 (uint32_t)box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-// Launch after a kernel whose launch_dependents() lets this one's prologue start early; z is one cluster.
-template <typename K, typename... A>
-int launch_after(K kernel, dim3 grid, int threads, int smem, int cluster_z, cudaStream_t st, const char* what, A... args) {
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return fail(ATS_ECUDA, "%s: %s", what, cudaGetErrorString(e));
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = 1;
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = (unsigned)cluster_z;
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3((unsigned)threads);
-  cfg.dynamicSmemBytes = (size_t)smem;
-  cfg.stream = st;
-  cfg.attrs = attr;
-  cfg.numAttrs = cluster_z > 1 ? 2 : 1;
-  e = cudaLaunchKernelEx(&cfg, kernel, args...);
-  if (e != cudaSuccess) return fail(ATS_ECUDA, "%s: %s", what, cudaGetErrorString(e));
-  return check_launch(what);
-}
-
 template <typename T>
-int dot(const void* x, int64_t ldx, const int8_t* w, int64_t ldw, const Out& o, int K, cudaStream_t st) {
+int dot(const void* x, const int8_t* w, int64_t ldw, const Out& o, int K, cudaStream_t st) {
   const int warps = kDotThreads / 32;
   const int64_t want = (o.N + warps - 1) / warps, cap = (int64_t)num_sms() * 4;
   const unsigned grid = (unsigned)(want < cap ? want : cap);
-  const int mt = o.M == 1 ? 1 : o.M == 2 ? 2 : 4;
-  const int smem = mt * (int)padded_k(K);
-  auto* xp = static_cast<const T*>(x);
-  const int vec = aligned16(x) && ldx % Chunk<T>::N == 0;
-  auto go = [&](auto kernel) {
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kDotSmem);
-    if (e != cudaSuccess) return fail(ATS_ECUDA, "int8_dot: %s", cudaGetErrorString(e));
-    kernel<<<grid, kDotThreads, smem, st>>>(xp, ldx, w, ldw, o, K, vec);
-    return check_launch("int8_dot");
-  };
-  return mt == 1 ? go(int8_dot_kernel<T, 1>) : mt == 2 ? go(int8_dot_kernel<T, 2>) : go(int8_dot_kernel<T, 4>);
+  return launch_after(int8_dot_kernel<T>, dim3(grid), kDotThreads, (int)padded_k(K), 1, st, "int8_dot",
+                      static_cast<const T*>(x), w, ldw, o, K, aligned16(x) ? 1 : 0);
 }
 
 template <typename T, int BN>
@@ -767,24 +813,24 @@ int parts(const int8_t* q, int64_t ldq, const int8_t* w, int64_t ldw, const Out&
   const dim3 grid((unsigned)((o.N + BM - 1) / BM), (unsigned)((o.M + TN - 1) / TN), (unsigned)split);
   const int smem = 1024 + part_stages(TN) * part_stage_bytes(TN);
   return launch_after(int8_part_kernel<T, TN>, grid, kPartThreads, smem, split, st, "int8_part", mw, mx, o,
-                      (K + BKB - 1) / BKB);
+                      (K + BKB - 1) / BKB, o.N % 4 == 0 && aligned16(o.y) ? 1 : 0);
 }
 
 template <typename T>
 int linear(const void* x, int64_t ldx, const int8_t* w, int64_t ldw, Out o, int64_t K, int8_t* q, float* sx,
            cudaStream_t st) {
-  if (o.M <= kDotTokens && o.M * padded_k(K) <= kDotSmem / 2) return dot<T>(x, ldx, w, ldw, o, (int)K, st);
+  if (o.M == 1 && padded_k(K) <= kDotSmem - 1024) return dot<T>(x, w, ldw, o, (int)K, st);
   const int64_t ldq = padded_k(K);
   ATS_TRY(quantize_t<T>(x, ldx, q, ldq, sx, o.M, K, st));
   o.sx = sx;
   const int64_t nt = (o.N + BM - 1) / BM;
   const int kb = (int)((K + BKB - 1) / BKB);
-  // Few tokens: as many columns as hold them, and K split until the SMs are busy (each part keeps 2 blocks).
+  // Few tokens: as many columns as hold them, and K split until two CTAs share each SM (a part keeps 2 blocks).
   const int tn = o.M <= 16 ? 16 : o.M <= 32 ? 32 : o.M <= 64 ? 64 : 128;
   const int64_t part_tiles = nt * ((o.M + tn - 1) / tn);
-  if (part_tiles <= num_sms() && (o.M + tn - 1) / tn <= 65535) {
+  if (part_tiles <= 2 * num_sms() && (o.M + tn - 1) / tn <= 65535) {
     int split = 1;
-    while (split < 8 && part_tiles * split * 2 <= num_sms() && kb >= split * 4) split *= 2;
+    while (split < kMaxSplit && part_tiles * split * 2 <= 2 * num_sms() && kb >= split * 4) split *= 2;
     switch (tn) {
       case 16: return parts<T, 16>(q, ldq, w, ldw, o, (int)K, split, st);
       case 32: return parts<T, 32>(q, ldq, w, ldw, o, (int)K, split, st);
@@ -792,7 +838,10 @@ int linear(const void* x, int64_t ldx, const int8_t* w, int64_t ldw, Out o, int6
       default: return parts<T, 128>(q, ldq, w, ldw, o, (int)K, split, st);
     }
   }
-  return o.N > 128 ? tiles<T, 256>(q, ldq, w, ldw, o, (int)K, st) : tiles<T, 128>(q, ldq, w, ldw, o, (int)K, st);
+  // 256 columns read fewer bytes per product; 128 where they leave fewer SMs idle.
+  const int64_t mt = (o.M + BM - 1) / BM;
+  return mt * ((o.N + 255) / 256) > num_sms() * 3 / 4 ? tiles<T, 256>(q, ldq, w, ldw, o, (int)K, st)
+                                                      : tiles<T, 128>(q, ldq, w, ldw, o, (int)K, st);
 }
 
 }  // namespace
