@@ -401,76 +401,77 @@ __global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid
   tc::wait_prerequisites();  // the quantised tokens and their scales
 
   if (warp == 0) {
-    if (lane == 0) {
-      tc::prefetch_tensormap(&tmA);
-      tc::prefetch_tensormap(&tmB);
-      int stage = 0, issued = 0;
-      uint32_t phase = 0;
-      for (int t = blockIdx.x; t < total && !abort_flag; t += gridDim.x) {
-        int m, n;
-        tile_of(p, t, m, n);
-        for (int kb = 0; kb < p.kb; ++kb) {
-          if (!tc::mbar_wait(&empty_bar[stage], phase ^ 1u, &abort_flag, budget)) {
-            give_up(&abort_flag, 31);
-            break;
-          }
+    int stage = 0, issued = 0;
+    uint32_t phase = 0;
+    for (int t = blockIdx.x; t < total; t += gridDim.x) {
+      int m, n;
+      tile_of(p, t, m, n);
+      bool ok = true;
+      for (int kb = 0; kb < p.kb; ++kb) {
+        ok = tc::mbar_wait_warp(&empty_bar[stage], phase ^ 1u, &abort_flag, budget);
+        if (!ok) break;
+        if (tc::elect_one()) {
           uint8_t* sa = ring + stage * STAGE;
           tc::mbar_arrive_expect_tx(&full_bar[stage], STAGE);
           tc::tma_load_2d(sa, &tmA, kb * BKB, m * BM, &full_bar[stage]);
           tc::tma_load_2d(sa + BM * BKB, &tmB, kb * BKB, n * BN, &full_bar[stage]);
-          ++issued;
-          if (++stage == NST) {
-            stage = 0;
-            phase ^= 1u;
-          }
+        }
+        ++issued;
+        if (++stage == NST) {
+          stage = 0;
+          phase ^= 1u;
         }
       }
-      // every load issued lands before the CTA may exit
-      for (int s = 0; s < NST && s < issued; ++s) {
-        const int last = s + (issued - 1 - s) / NST * NST;
-        if (!tc::mbar_wait(&full_bar[s], (uint32_t)((last / NST) & 1), nullptr, kWaitBudget))
-          atomicCAS(&g_int8_status, 0, 35);
+      if (!ok) {
+        give_up(&abort_flag, 31);
+        break;
       }
     }
+    // every load issued lands before the CTA may exit
+    for (int s = 0; s < NST && s < issued; ++s) {
+      const int last = s + (issued - 1 - s) / NST * NST;
+      if (!tc::mbar_wait(&full_bar[s], (uint32_t)((last / NST) & 1), nullptr, kWaitBudget))
+        atomicCAS(&g_int8_status, 0, 35);
+    }
   } else if (warp == 1) {
-    if (lane == 0) {
-      int stage = 0, i = 0;
-      uint32_t phase = 0;
-      bool issued = false;
-      for (int t = blockIdx.x; t < total && !abort_flag; t += gridDim.x, ++i) {
-        const int acc = i & 1;
-        if (!tc::mbar_wait(&tempty_bar[acc], ((uint32_t)(i >> 1) & 1u) ^ 1u, &abort_flag, budget)) {
-          give_up(&abort_flag, 32);
+    const uint64_t desc = tc::smem_desc(tc::smem_u32(ring), 16u, 1024u, tc::kLayoutSW128);
+    int stage = 0, i = 0;
+    uint32_t phase = 0;
+    bool issued = false, ok = true;
+    for (int t = blockIdx.x; t < total && ok; t += gridDim.x, ++i) {
+      const int acc = i & 1;
+      ok = tc::mbar_wait_warp(&tempty_bar[acc], ((uint32_t)(i >> 1) & 1u) ^ 1u, &abort_flag, budget);
+      if (!ok) {
+        give_up(&abort_flag, 32);
+        break;
+      }
+      tc::tc_fence_after();
+      for (int kb = 0; kb < p.kb; ++kb) {
+        ok = tc::mbar_wait_warp(&full_bar[stage], phase, &abort_flag, budget);
+        if (!ok) {
+          give_up(&abort_flag, 33);
           break;
         }
         tc::tc_fence_after();
-        bool ok = true;
-        for (int kb = 0; kb < p.kb; ++kb) {
-          if (!tc::mbar_wait(&full_bar[stage], phase, &abort_flag, budget)) {
-            give_up(&abort_flag, 33);
-            ok = false;
-            break;
-          }
-          tc::tc_fence_after();
-          const uint32_t sa = tc::smem_u32(ring + stage * STAGE), sb = sa + BM * BKB;
+        // the start address of a descriptor is in units of 16 bytes; the ring ends below 2^18
+        const uint64_t da = desc + (uint64_t)(stage * (STAGE / 16)), db = da + BM * BKB / 16;
+        if (tc::elect_one()) {
 #pragma unroll
           for (int k = 0; k < BKB / 32; ++k)
-            tc::mma_i8(tmem_base + (uint32_t)(acc * BN), tc::smem_desc(sa + k * 32, 16u, 1024u, tc::kLayoutSW128),
-                       tc::smem_desc(sb + k * 32, 16u, 1024u, tc::kLayoutSW128), IDESC, (kb > 0 || k > 0) ? 1u : 0u);
+            tc::mma_i8(tmem_base + (uint32_t)(acc * BN), da + k * 2, db + k * 2, IDESC, (kb > 0 || k > 0) ? 1u : 0u);
           tc::mma_commit(&empty_bar[stage]);
-          issued = true;
-          if (++stage == NST) {
-            stage = 0;
-            phase ^= 1u;
-          }
+          if (kb == p.kb - 1) tc::mma_commit(&tfull_bar[acc]);
         }
-        if (!ok) break;
-        tc::mma_commit(&tfull_bar[acc]);
+        issued = true;
+        if (++stage == NST) {
+          stage = 0;
+          phase ^= 1u;
+        }
       }
-      if (issued) {  // all MMAs complete before TMEM is freed
-        tc::mma_commit(&done_bar);
-        if (!tc::mbar_wait(&done_bar, 0u, nullptr, kWaitBudget)) atomicCAS(&g_int8_status, 0, 36);
-      }
+    }
+    if (issued) {  // all MMAs complete before TMEM is freed
+      if (tc::elect_one()) tc::mma_commit(&done_bar);
+      if (!tc::mbar_wait(&done_bar, 0u, nullptr, kWaitBudget)) atomicCAS(&g_int8_status, 0, 36);
     }
   } else {
     const int quad = warp & 3, chalf = (warp - 2) >> 2;
@@ -559,9 +560,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid
 // workspace or atomics are needed.  The weights' loads start before the quantisation has ended.
 constexpr int kPartThreads = 64 + 32 * kEpiWarps, kMaxSplit = 8;
 
-// Two CTAs of a part kernel share an SM: about 100 KB of ring each.
+// The ring takes what the SM has where one CTA comes to an SM, and half of it where two do: a part waits on load
+// latency, and more bytes in flight hide more of it.
 __host__ __device__ constexpr int part_stage_bytes(int tn) { return (BM + tn) * BKB; }
-__host__ __device__ constexpr int part_stages(int tn) { return 100 * 1024 / part_stage_bytes(tn); }
+__host__ __device__ constexpr int part_stages(int tn, bool alone) { return (alone ? 208 : 104) * 1024 / part_stage_bytes(tn); }
 
 struct PartOut {
   const int* tile;                     // [TN][128] sums of this CTA's part of K
@@ -622,13 +624,13 @@ __device__ __forceinline__ void reduce_parts(const Out& o, const PartOut& p) {
 template <typename T, int TN>
 __global__ void __launch_bounds__(kPartThreads, 2) int8_part_kernel(const __grid_constant__ CUtensorMap tmW,
                                                                    const __grid_constant__ CUtensorMap tmX, Out o,
-                                                                   int kb_all, int vec_out) {
-  constexpr int STAGE = part_stage_bytes(TN), NST = part_stages(TN);
+                                                                   int kb_all, int nst, int vec_out) {
+  constexpr int STAGE = part_stage_bytes(TN), MAXST = part_stages(TN, true);
   constexpr int TCOLS = TN < 32 ? 32 : TN;
   constexpr uint32_t IDESC = tc::idesc_i8(BM, TN);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ __align__(8) uint64_t full_bar[NST], empty_bar[NST], tfull_bar;
+  __shared__ __align__(8) uint64_t full_bar[MAXST], empty_bar[MAXST], tfull_bar;
   __shared__ uint32_t tmem_base_s;
   __shared__ volatile int abort_flag;
   __shared__ float sx_s[TN];
@@ -639,7 +641,7 @@ __global__ void __launch_bounds__(kPartThreads, 2) int8_part_kernel(const __grid
   const int kb0 = (int)((int64_t)kb_all * part / split), kb1 = (int)((int64_t)kb_all * (part + 1) / split);
   const int n0 = blockIdx.x * BM, m0 = blockIdx.y * TN;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < NST; ++s) {
+    for (int s = 0; s < nst; ++s) {
       tc::mbar_init(&full_bar[s], 1);
       tc::mbar_init(&empty_bar[s], 1);
     }
@@ -657,54 +659,67 @@ __global__ void __launch_bounds__(kPartThreads, 2) int8_part_kernel(const __grid
   tc::tc_fence_after();
   const uint32_t tmem_base = tmem_base_s;
 
+  const int nkb = kb1 - kb0;
   if (warp == 0) {
-    if (lane == 0) {
-      const int nkb = kb1 - kb0;
-      const int ahead = nkb < NST ? nkb : NST;
+    const int ahead = nkb < nst ? nkb : nst;
+    if (tc::elect_one())
       for (int s = 0; s < ahead; ++s) {
         tc::mbar_arrive_expect_tx(&full_bar[s], STAGE);
         tc::tma_load_2d(ring + s * STAGE, &tmW, (kb0 + s) * BKB, n0, &full_bar[s]);
       }
-      tc::wait_prerequisites();
+    __syncwarp();
+    tc::wait_prerequisites();
+    if (tc::elect_one())
       for (int s = 0; s < ahead; ++s)
         tc::tma_load_2d(ring + s * STAGE + BM * BKB, &tmX, (kb0 + s) * BKB, m0, &full_bar[s]);
-      int issued = ahead;
-      for (int i = ahead; i < nkb; ++i) {
-        const int s = i % NST;
-        if (!tc::mbar_wait(&empty_bar[s], (uint32_t)((i / NST) & 1) ^ 1u, &abort_flag, budget)) {
-          give_up(&abort_flag, 41);
-          break;
-        }
-        tc::mbar_arrive_expect_tx(&full_bar[s], STAGE);
-        tc::tma_load_2d(ring + s * STAGE, &tmW, (kb0 + i) * BKB, n0, &full_bar[s]);
-        tc::tma_load_2d(ring + s * STAGE + BM * BKB, &tmX, (kb0 + i) * BKB, m0, &full_bar[s]);
-        ++issued;
+    __syncwarp();
+    int issued = ahead, stage = 0;
+    uint32_t phase = 0;
+    for (int i = ahead; i < nkb; ++i) {
+      if (!tc::mbar_wait_warp(&empty_bar[stage], phase, &abort_flag, budget)) {
+        give_up(&abort_flag, 41);
+        break;
       }
-      for (int s = 0; s < NST && s < issued; ++s) {  // every load issued lands before the CTA may exit
-        const int last = s + (issued - 1 - s) / NST * NST;
-        if (!tc::mbar_wait(&full_bar[s], (uint32_t)((last / NST) & 1), nullptr, kWaitBudget))
-          atomicCAS(&g_int8_status, 0, 45);
+      if (tc::elect_one()) {
+        tc::mbar_arrive_expect_tx(&full_bar[stage], STAGE);
+        tc::tma_load_2d(ring + stage * STAGE, &tmW, (kb0 + i) * BKB, n0, &full_bar[stage]);
+        tc::tma_load_2d(ring + stage * STAGE + BM * BKB, &tmX, (kb0 + i) * BKB, m0, &full_bar[stage]);
       }
+      ++issued;
+      if (++stage == nst) {
+        stage = 0;
+        phase ^= 1u;
+      }
+    }
+    for (int s = 0; s < nst && s < issued; ++s) {  // every load issued lands before the CTA may exit
+      const int last = s + (issued - 1 - s) / nst * nst;
+      if (!tc::mbar_wait(&full_bar[s], (uint32_t)((last / nst) & 1), nullptr, kWaitBudget))
+        atomicCAS(&g_int8_status, 0, 45);
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      const int nkb = kb1 - kb0;
-      for (int i = 0; i < nkb; ++i) {
-        const int s = i % NST;
-        if (!tc::mbar_wait(&full_bar[s], (uint32_t)((i / NST) & 1), &abort_flag, budget)) {
-          give_up(&abort_flag, 43);
-          break;
-        }
-        tc::tc_fence_after();
-        const uint32_t sa = tc::smem_u32(ring + s * STAGE), sb = sa + BM * BKB;
+    const uint64_t desc = tc::smem_desc(tc::smem_u32(ring), 16u, 1024u, tc::kLayoutSW128);
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int i = 0; i < nkb; ++i) {
+      if (!tc::mbar_wait_warp(&full_bar[stage], phase, &abort_flag, budget)) {
+        give_up(&abort_flag, 43);
+        break;
+      }
+      tc::tc_fence_after();
+      const uint64_t da = desc + (uint64_t)(stage * (STAGE / 16)), db = da + BM * BKB / 16;
+      if (tc::elect_one()) {
 #pragma unroll
         for (int k = 0; k < BKB / 32; ++k)
-          tc::mma_i8(tmem_base, tc::smem_desc(sa + k * 32, 16u, 1024u, tc::kLayoutSW128),
-                     tc::smem_desc(sb + k * 32, 16u, 1024u, tc::kLayoutSW128), IDESC, (i > 0 || k > 0) ? 1u : 0u);
-        tc::mma_commit(&empty_bar[s]);
+          tc::mma_i8(tmem_base, da + k * 2, db + k * 2, IDESC, (i > 0 || k > 0) ? 1u : 0u);
+        tc::mma_commit(&empty_bar[stage]);
       }
-      tc::mma_commit(&tfull_bar);  // also after a wait that gave up: the MMAs issued complete before TMEM is freed
+      if (++stage == nst) {
+        stage = 0;
+        phase ^= 1u;
+      }
     }
+    // also after a wait that gave up: the MMAs issued complete before TMEM is freed
+    if (tc::elect_one()) tc::mma_commit(&tfull_bar);
   }
   __syncwarp();
   if (warp >= 2 && warp < 6) {
@@ -735,7 +750,8 @@ __global__ void __launch_bounds__(kPartThreads, 2) int8_part_kernel(const __grid
   else if (split == 4) reduce_parts<T, 4>(o, po);
   else reduce_parts<T, 8>(o, po);
   __syncwarp();
-  if (split > 1) tc::cluster_sync();  // no CTA leaves while another reads its tile
+  // No CTA leaves while another reads its tile: what a thread read, it has used in the stores before this.
+  if (split > 1) tc::cluster_sync_relaxed();
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
@@ -811,9 +827,10 @@ int parts(const int8_t* q, int64_t ldq, const int8_t* w, int64_t ldw, const Out&
   ATS_TRY(operand_map(&mw, w, K, o.N, ldw, BM));
   ATS_TRY(operand_map(&mx, q, K, o.M, ldq, TN));
   const dim3 grid((unsigned)((o.N + BM - 1) / BM), (unsigned)((o.M + TN - 1) / TN), (unsigned)split);
-  const int smem = 1024 + part_stages(TN) * part_stage_bytes(TN);
+  const int nst = part_stages(TN, (int64_t)grid.x * grid.y * grid.z <= num_sms());
+  const int smem = 1024 + nst * part_stage_bytes(TN);
   return launch_after(int8_part_kernel<T, TN>, grid, kPartThreads, smem, split, st, "int8_part", mw, mx, o,
-                      (K + BKB - 1) / BKB, o.N % 4 == 0 && aligned16(o.y) ? 1 : 0);
+                      (K + BKB - 1) / BKB, nst, o.N % 4 == 0 && aligned16(o.y) ? 1 : 0);
 }
 
 template <typename T>

@@ -268,6 +268,12 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
 
+// The same without ordering memory (a release waits for every global store of the CTA): for CTAs that only must not
+// leave before the others are here.
+__device__ __forceinline__ void cluster_sync_relaxed() {
+  asm volatile("barrier.cluster.arrive.relaxed;\n\tbarrier.cluster.wait;" ::: "memory");
+}
+
 // Address, in the cluster's shared window, of this CTA's shared object at `saddr` as it sits in CTA `rank`.
 __device__ __forceinline__ uint32_t cluster_addr(uint32_t saddr, uint32_t rank) {
   uint32_t r;
@@ -341,6 +347,19 @@ __host__ __device__ constexpr uint32_t idesc_bf16(int M, int N, bool a_mn, bool 
 // Instruction descriptor, kind::i8: D s32, A/B signed 8-bit, both K-major, N>>3, M>>4.
 __host__ __device__ constexpr uint32_t idesc_i8(int M, int N) {
   return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+
+// One lane of the (converged) warp.  A role that loops with its whole warp and elects the lane that issues keeps its
+// addresses and descriptors in uniform registers; under a divergent branch every tcgen05.mma costs over 100 cycles.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
+}
+
+// mbar_wait by a whole warp: true for every lane, or false for every lane when one gave up.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort, long long budget) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, budget));
 }
 
 // ------------------------------------------- programmatic dependent launch
