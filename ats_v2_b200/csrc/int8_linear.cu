@@ -333,10 +333,11 @@ __global__ void __launch_bounds__(kDotThreads, 4) int8_dot_kernel(const T* __res
 // ------------------------------------------------- tensor cores, many tokens
 // tcgen05.mma kind::i8 on 128 tokens x BN channels, K in blocks of 128 bytes: one persistent CTA per SM, a TMA
 // producer warp, an MMA warp with two accumulators in TMEM, eight epilogue warps (two per TMEM lane quadrant, half
-// of the columns each) that scale, round and store through swizzled boxes.
+// of the columns each) that scale, round and store whole 128-byte
+// pieces of rows through a swizzled box in shared memory (a TMA store of the box queues behind the loads).
 constexpr int BM = 128, BKB = 128;
 constexpr int kEpiWarps = 8, kTileThreads = 64 + 32 * kEpiWarps;
-constexpr int kBox = 32 * 64, kBoxesPerWarp = 2;  // a box: 32 rows of 64 bytes
+constexpr int kBox = 32 * 128;  // an epilogue warp's staging: 32 rows of 128 bytes
 constexpr int kBandM = 16;                        // M tiles per band of the tile order
 
 __host__ __device__ constexpr int tile_stage_bytes(int bn) { return (BM + bn) * BKB; }
@@ -346,7 +347,7 @@ struct TileArgs {
   Out o;
   int kb;       // K blocks
   int mt, nt;   // tiles
-  int tma_out;  // rows of y are 16-byte multiples: boxes leave by TMA
+  int vec_out;  // rows of y are 16-byte multiples
 };
 
 // Tile t: bands of kBandM M tiles, M fastest inside a band, so that the CTAs that run together share weights and
@@ -362,11 +363,10 @@ __device__ __forceinline__ void tile_of(const TileArgs& p, int t, int& m, int& n
 template <typename T, int BN>
 __global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid_constant__ CUtensorMap tmA,
                                                                    const __grid_constant__ CUtensorMap tmB,
-                                                                   const __grid_constant__ CUtensorMap tmO,
                                                                    TileArgs p) {
   constexpr int STAGE = tile_stage_bytes(BN), NST = tile_stages(BN);
   constexpr uint32_t IDESC = tc::idesc_i8(BM, BN);
-  constexpr int BOX_COLS = 64 / (int)sizeof(T);
+  constexpr int BOX_COLS = 128 / (int)sizeof(T);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* staging = ring + NST * STAGE;
@@ -475,8 +475,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid
     }
   } else {
     const int quad = warp & 3, chalf = (warp - 2) >> 2;
-    uint8_t* boxes = staging + (warp - 2) * kBoxesPerWarp * kBox;
-    int puts = 0, i = 0;
+    uint8_t* box = staging + (warp - 2) * kBox;
+    int i = 0;
     for (int t = blockIdx.x; t < total && !abort_flag; t += gridDim.x, ++i) {
       int m, n;
       tile_of(p, t, m, n);
@@ -490,7 +490,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid
         sw[j] = col < p.o.N ? p.o.sw[col] : 0.f;
         bw[j] = col < p.o.N ? bias_at(p.o, col) : 0.f;
       }
-      if (!tc::mbar_wait(&tfull_bar[acc], (uint32_t)(i >> 1) & 1u, &abort_flag, budget)) {
+      if (!tc::mbar_wait_warp(&tfull_bar[acc], (uint32_t)(i >> 1) & 1u, &abort_flag, budget)) {
         give_up(&abort_flag, 34);
         break;
       }
@@ -499,53 +499,60 @@ __global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid
 #pragma unroll
       for (int c = 0; c < BN / 2; c += BOX_COLS) {
         const int col0 = n * BN + chalf * (BN / 2) + c;
+        uint32_t r[BOX_COLS];
+#pragma unroll
+        for (int h = 0; h < BOX_COLS; h += 16) tc::tmem_ld16_async(t_row + c + h, r + h);
+        tc::tmem_ld_wait();
+        if (c + BOX_COLS == BN / 2) {  // the accumulator is read: the next tile's products may start
+          tc::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(&tempty_bar[acc]);
+        }
         float v[BOX_COLS];
 #pragma unroll
-        for (int h = 0; h < BOX_COLS; h += 16) {
-          uint32_t r[16];
-          tc::tmem_ld16(t_row + c + h, r);
+        for (int e = 0; e < BOX_COLS; ++e)
+          v[e] = (float)(int)r[e] * (sx * __shfl_sync(0xffffffffu, sw[(c + e) / 32], (c + e) % 32));
+        if (p.o.bias != nullptr)  // one branch: one for each element would serialise them
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            v[h + j] = (float)(int)r[j] * (sx * __shfl_sync(0xffffffffu, sw[(c + h) / 32], (c + h) % 32 + j));
-            if (p.o.bias != nullptr) v[h + j] += __shfl_sync(0xffffffffu, bw[(c + h) / 32], (c + h) % 32 + j);
-          }
-        }
-        uint8_t* box = boxes + (puts % kBoxesPerWarp) * kBox;
-        if (lane == 0) tc::bulk_wait_read<kBoxesPerWarp - 1>();
-        __syncwarp();
+          for (int e = 0; e < BOX_COLS; ++e) v[e] += __shfl_sync(0xffffffffu, bw[(c + e) / 32], (c + e) % 32);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {  // row `lane`, 16-byte piece q at its swizzled place (conflict-free)
+        for (int q = 0; q < 8; ++q) {  // row `lane`, 16-byte piece q at its swizzled place (conflict-free)
           float u[Chunk<T>::N];
 #pragma unroll
           for (int j = 0; j < Chunk<T>::N; ++j) u[j] = v[q * Chunk<T>::N + j];
           uint4 w;
           pack_chunk<T>(u, w);
-          *reinterpret_cast<uint4*>(box + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4)) = w;
+          *reinterpret_cast<uint4*>(box + lane * 128 + ((q ^ (lane & 7)) << 4)) = w;
         }
-        if (p.tma_out) {
-          tc::fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            if (col0 < p.o.N && row0 < p.o.M) tc::tma_store_2d(&tmO, box, col0, row0);
-            tc::bulk_commit();
+        __syncwarp();
+        if (p.vec_out) {  // 8 lanes write 128 bytes of a row
+          const int q = lane & 7, col = col0 + q * Chunk<T>::N;
+          uint4 w[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int rr = k * 4 + (lane >> 3);
+            w[k] = *reinterpret_cast<const uint4*>(box + rr * 128 + ((q ^ (rr & 7)) << 4));
+          }
+          if (col < p.o.N) {
+            T* y = static_cast<T*>(p.o.y) + (int64_t)(row0 + (lane >> 3)) * p.o.N + col;
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              if (row0 + k * 4 + (lane >> 3) < p.o.M) *reinterpret_cast<uint4*>(y + (int64_t)k * 4 * p.o.N) = w[k];
           }
         } else {  // rows of y that are not 16-byte multiples: element by element, along the rows
-          __syncwarp();
-          constexpr int ROWS = 32 / BOX_COLS;  // rows a warp writes at once
-          const int cc = lane % BOX_COLS, byte = cc * (int)sizeof(T);
-          for (int r = lane / BOX_COLS; r < 32; r += ROWS)
-            if (row0 + r < p.o.M && col0 + cc < p.o.N)
-              static_cast<T*>(p.o.y)[(int64_t)(row0 + r) * p.o.N + col0 + cc] = *reinterpret_cast<const T*>(
-                  box + r * 64 + (((byte >> 4) ^ ((r >> 1) & 3)) << 4) + (byte & 15));
-          __syncwarp();
+#pragma unroll 1
+          for (int rr = 0; rr < 32 && row0 + rr < p.o.M; ++rr)
+#pragma unroll
+            for (int cc = lane; cc < BOX_COLS; cc += 32) {
+              const int byte = cc * (int)sizeof(T);
+              if (col0 + cc < p.o.N)
+                static_cast<T*>(p.o.y)[(int64_t)(row0 + rr) * p.o.N + col0 + cc] =
+                    *reinterpret_cast<const T*>(box + rr * 128 + (((byte >> 4) ^ (rr & 7)) << 4) + (byte & 15));
+            }
         }
-        ++puts;
+        __syncwarp();
       }
-      tc::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) tc::mbar_arrive(&tempty_bar[acc]);
     }
-    if (lane == 0) tc::bulk_wait<0>();
   }
   tc::tc_fence_before();
   __syncthreads();
@@ -766,8 +773,8 @@ size_t q_bytes(int64_t M, int64_t K) { return align_up((size_t)(M * padded_k(K))
 PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
 std::once_flag g_encode_once;
 
-int encode(CUtensorMap* m, CUtensorMapDataType type, const void* base, uint64_t inner, uint64_t outer,
-           uint64_t row_bytes, uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle swz) {
+// Operand of int8 rows: boxes of 128 bytes x `box_rows`, 128-byte swizzle; bytes past K and rows past the end read as 0.
+int operand_map(CUtensorMap* m, const void* base, int64_t K, int64_t rows, int64_t ld, int box_rows) {
   std::call_once(g_encode_once, [] {
     void* fn = nullptr;
     cudaDriverEntryPointQueryResult q;
@@ -776,20 +783,15 @@ int encode(CUtensorMap* m, CUtensorMapDataType type, const void* base, uint64_t 
       g_encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
   });
   if (g_encode == nullptr) return fail(ATS_ECUDA, "int8_linear: cuTensorMapEncodeTiled unavailable");
-  cuuint64_t dims[2] = {inner, outer};
-  cuuint64_t strides[1] = {row_bytes};
-  cuuint32_t box[2] = {box_inner, box_outer};
+  cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)ld};
+  cuuint32_t box[2] = {BKB, (cuuint32_t)box_rows};
   cuuint32_t es[2] = {1, 1};
-  CUresult r = g_encode(m, type, 2, const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        swz, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  CUresult r = g_encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, es,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(ATS_ECUDA, "int8_linear: cuTensorMapEncodeTiled failed (%d)", (int)r);
   return ATS_OK;
-}
-
-// Operand of int8 rows: boxes of 128 bytes x `rows`, 128-byte swizzle; bytes past K and rows past the end read as 0.
-int operand_map(CUtensorMap* m, const void* base, int64_t K, int64_t rows, int64_t ld, int box_rows) {
-  return encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, (uint64_t)K, (uint64_t)rows, (uint64_t)ld, BKB,
-                (uint32_t)box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 template <typename T>
@@ -803,22 +805,16 @@ int dot(const void* x, const int8_t* w, int64_t ldw, const Out& o, int K, cudaSt
 
 template <typename T, int BN>
 int tiles(const int8_t* q, int64_t ldq, const int8_t* w, int64_t ldw, const Out& o, int K, cudaStream_t st) {
-  CUtensorMap ma, mb, mo;
+  CUtensorMap ma, mb;
   ATS_TRY(operand_map(&ma, q, K, o.M, ldq, BM));
   ATS_TRY(operand_map(&mb, w, K, o.N, ldw, BN));
-  TileArgs p{o, (K + BKB - 1) / BKB, (o.M + BM - 1) / BM, (o.N + BN - 1) / BN, 0};
-  const int64_t row_bytes = (int64_t)o.N * (int64_t)sizeof(T);
-  p.tma_out = row_bytes % 16 == 0 && aligned16(o.y);
-  if (p.tma_out)
-    ATS_TRY(encode(&mo, sizeof(T) == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, o.y,
-                   (uint64_t)o.N, (uint64_t)o.M, (uint64_t)row_bytes, 64 / sizeof(T), 32, CU_TENSOR_MAP_SWIZZLE_64B));
-  else
-    mo = ma;
+  const int vec = (int64_t)o.N * (int64_t)sizeof(T) % 16 == 0 && aligned16(o.y);
+  const TileArgs p{o, (K + BKB - 1) / BKB, (o.M + BM - 1) / BM, (o.N + BN - 1) / BN, vec};
   const int64_t total = (int64_t)p.mt * p.nt;
   if (total > 0x7fffffff - 4096) return fail(ATS_EUNSUPPORTED, "int8_linear: too many tiles");
   const int grid = total < gemm_ctas() ? (int)total : gemm_ctas();
-  const int smem = 1024 + tile_stages(BN) * tile_stage_bytes(BN) + kEpiWarps * kBoxesPerWarp * kBox;
-  return launch_after(int8_tile_kernel<T, BN>, dim3((unsigned)grid), kTileThreads, smem, 1, st, "int8_tile", ma, mb, mo, p);
+  const int smem = 1024 + tile_stages(BN) * tile_stage_bytes(BN) + kEpiWarps * kBox;
+  return launch_after(int8_tile_kernel<T, BN>, dim3((unsigned)grid), kTileThreads, smem, 1, st, "int8_tile", ma, mb, p);
 }
 
 template <typename T, int TN>
