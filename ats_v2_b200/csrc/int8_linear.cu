@@ -180,9 +180,9 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G) int8_quantize_kernel(const 
 }
 
 // Launch whose prologue may start before the stream's previous kernel has ended (every kernel here waits for it with
-// wait_prerequisites); cluster_z CTAs along z are one cluster.
+// wait_prerequisites), in clusters of CTAs.
 template <typename F, typename... A>
-int launch_after(F kernel, dim3 grid, int threads, int smem, int cluster_z, cudaStream_t st, const char* what,
+int launch_after(F kernel, dim3 grid, int threads, int smem, dim3 cluster, cudaStream_t st, const char* what,
                  A... args) {
   // All with one shared-memory split: an SM that has to change it between two kernels first drains.
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
@@ -195,15 +195,15 @@ int launch_after(F kernel, dim3 grid, int threads, int smem, int cluster_z, cuda
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = 1;
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = (unsigned)cluster_z;
+  attr[1].val.clusterDim.x = cluster.x;
+  attr[1].val.clusterDim.y = cluster.y;
+  attr[1].val.clusterDim.z = cluster.z;
   cfg.gridDim = grid;
   cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = st;
   cfg.attrs = attr;
-  cfg.numAttrs = cluster_z > 1 ? 2 : 1;
+  cfg.numAttrs = cluster.x * cluster.y * cluster.z > 1 ? 2 : 1;
   e = cudaLaunchKernelEx(&cfg, kernel, args...);
   if (e != cudaSuccess) return fail(ATS_ECUDA, "%s: %s", what, cudaGetErrorString(e));
   return check_launch(what);
@@ -216,7 +216,7 @@ int quantize_g(const T* x, int64_t ldx, int8_t* q, int64_t ldq, float* scale, in
   const int64_t per = THREADS / G;
   const unsigned grid = (unsigned)((rows + per - 1) / per);
   auto go = [&](auto kernel) {
-    return launch_after(kernel, dim3(grid), THREADS, 0, 1, st, "int8_quantize", x, ldx, q, ldq, scale, rows, K);
+    return launch_after(kernel, dim3(grid), THREADS, 0, dim3(1), st, "int8_quantize", x, ldx, q, ldq, scale, rows, K);
   };
   if (vec) return q16 ? go(int8_quantize_kernel<T, G, true, true>) : go(int8_quantize_kernel<T, G, true, false>);
   return q16 ? go(int8_quantize_kernel<T, G, false, true>) : go(int8_quantize_kernel<T, G, false, false>);
@@ -331,17 +331,21 @@ __global__ void __launch_bounds__(kDotThreads, 4) int8_dot_kernel(const T* __res
 }
 
 // ------------------------------------------------- tensor cores, many tokens
-// tcgen05.mma kind::i8 on 128 tokens x BN channels, K in blocks of 128 bytes: one persistent CTA per SM, a TMA
-// producer warp, an MMA warp with two accumulators in TMEM, eight epilogue warps (two per TMEM lane quadrant, half
-// of the columns each) that scale, round and store whole 128-byte
-// pieces of rows through a swizzled box in shared memory (a TMA store of the box queues behind the loads).
+// tcgen05.mma kind::i8, K in blocks of 128 bytes: one persistent CTA per SM, a TMA producer warp, an MMA warp with
+// two accumulators in TMEM, eight epilogue warps (two per TMEM lane quadrant, half of the columns each) that scale,
+// round and store whole 128-byte pieces of rows through a swizzled box in shared memory.
+//
+// PAIR: two CTAs of a cluster share a tile of 256 tokens x BN channels (cta_group::2).  Each loads its 128 tokens
+// and half of the channels, 32 KB a block instead of 48: single CTAs are held by what L2 delivers to the SMs, about
+// 15 TB/s.  All loads of a block count on CTA 0's full barrier; CTA 0 issues the MMAs and its commits reach the
+// empty and accumulator barriers of both; both epilogues release the accumulator on CTA 0.
 constexpr int BM = 128, BKB = 128;
 constexpr int kEpiWarps = 8, kTileThreads = 64 + 32 * kEpiWarps;
 constexpr int kBox = 32 * 128;  // an epilogue warp's staging: 32 rows of 128 bytes
 constexpr int kBandM = 16;                        // M tiles per band of the tile order
 
-__host__ __device__ constexpr int tile_stage_bytes(int bn) { return (BM + bn) * BKB; }
-__host__ __device__ constexpr int tile_stages(int bn) { return 4 * tile_stage_bytes(256) / tile_stage_bytes(bn); }
+__host__ __device__ constexpr int tile_stage_bytes(int bn, bool pair) { return (BM + (pair ? bn / 2 : bn)) * BKB; }
+__host__ __device__ constexpr int tile_stages(int bn, bool pair) { return 192 * 1024 / tile_stage_bytes(bn, pair); }
 
 struct TileArgs {
   Out o;
@@ -360,22 +364,30 @@ __device__ __forceinline__ void tile_of(const TileArgs& p, int t, int& m, int& n
   m = m0 + (r - n * gm);
 }
 
-template <typename T, int BN>
+template <typename T, int BN, bool PAIR>
 __global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid_constant__ CUtensorMap tmA,
                                                                    const __grid_constant__ CUtensorMap tmB,
                                                                    TileArgs p) {
-  constexpr int STAGE = tile_stage_bytes(BN), NST = tile_stages(BN);
-  constexpr uint32_t IDESC = tc::idesc_i8(BM, BN);
+  constexpr int TM = PAIR ? 2 * BM : BM, B_ROWS = PAIR ? BN / 2 : BN;
+  constexpr int STAGE = tile_stage_bytes(BN, PAIR), NST = tile_stages(BN, PAIR);
+  constexpr uint32_t IDESC = tc::idesc_i8(TM, BN);
   constexpr int BOX_COLS = 128 / (int)sizeof(T);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* staging = ring + NST * STAGE;
   __shared__ __align__(8) uint64_t full_bar[NST], empty_bar[NST], tfull_bar[2], tempty_bar[2], done_bar;
   __shared__ uint32_t tmem_base_s;
+  __shared__ int peer_issued_s;  // PAIR, CTA 0: blocks that CTA 1 loaded
   __shared__ volatile int abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long budget = g_int8_wait_budget;
   const int total = p.mt * p.nt;
+  const uint32_t cta = PAIR ? tc::cluster_ctarank() : 0u;
+  const int t_first = PAIR ? (int)blockIdx.x / 2 : (int)blockIdx.x, t_step = PAIR ? (int)gridDim.x / 2 : (int)gridDim.x;
+  auto stop = [&](int code) {  // a role that gives up stops the others, in both CTAs of a pair
+    give_up(&abort_flag, code);
+    if constexpr (PAIR) tc::st_cluster_u32(tc::cluster_addr(tc::smem_u32((const void*)&abort_flag), cta ^ 1u), 1u);
+  };
   if (threadIdx.x == 0) {
     for (int s = 0; s < NST; ++s) {
       tc::mbar_init(&full_bar[s], 1);
@@ -383,7 +395,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid
     }
     for (int a = 0; a < 2; ++a) {
       tc::mbar_init(&tfull_bar[a], 1);
-      tc::mbar_init(&tempty_bar[a], kEpiWarps);
+      tc::mbar_init(&tempty_bar[a], PAIR ? 2 * kEpiWarps : kEpiWarps);
     }
     tc::mbar_init(&done_bar, 1);
     tc::fence_barrier_init();
@@ -391,97 +403,129 @@ __global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid
     abort_flag = 0;
   }
   if (warp == 1) {
-    tc::tmem_alloc(&tmem_base_s, 2 * BN);
-    tc::tmem_relinquish();
+    if constexpr (PAIR) {
+      tc::tmem_alloc_pair(&tmem_base_s, 2 * BN);
+      tc::tmem_relinquish_pair();
+    } else {
+      tc::tmem_alloc(&tmem_base_s, 2 * BN);
+      tc::tmem_relinquish();
+    }
   }
   tc::tc_fence_before();
   __syncthreads();
+  if constexpr (PAIR) tc::cluster_sync();  // both CTAs' barriers exist before either signals the other's
   tc::tc_fence_after();
   const uint32_t tmem_base = tmem_base_s;
+  // every load issued lands before the CTA may exit: the last phase of each stage of the first `issued` blocks
+  auto drain = [&](int issued) {
+    for (int s = 0; s < NST && s < issued; ++s) {
+      const int last = s + (issued - 1 - s) / NST * NST;
+      if (!tc::mbar_wait(&full_bar[s], (uint32_t)((last / NST) & 1), nullptr, kWaitBudget))
+        atomicCAS(&g_int8_status, 0, 35);
+    }
+  };
+  int issued_blocks = 0;
   tc::wait_prerequisites();  // the quantised tokens and their scales
 
   if (warp == 0) {
-    int stage = 0, issued = 0;
+    int stage = 0;
     uint32_t phase = 0;
-    for (int t = blockIdx.x; t < total; t += gridDim.x) {
+    const uint32_t full0 = PAIR ? tc::cluster_addr(tc::smem_u32(&full_bar[0]), 0u) : 0u;
+    for (int t = t_first; t < total; t += t_step) {
       int m, n;
       tile_of(p, t, m, n);
+      const int row = m * TM + (int)cta * BM, col = n * BN + (int)cta * B_ROWS;
       bool ok = true;
       for (int kb = 0; kb < p.kb; ++kb) {
         ok = tc::mbar_wait_warp(&empty_bar[stage], phase ^ 1u, &abort_flag, budget);
         if (!ok) break;
         if (tc::elect_one()) {
           uint8_t* sa = ring + stage * STAGE;
-          tc::mbar_arrive_expect_tx(&full_bar[stage], STAGE);
-          tc::tma_load_2d(sa, &tmA, kb * BKB, m * BM, &full_bar[stage]);
-          tc::tma_load_2d(sa + BM * BKB, &tmB, kb * BKB, n * BN, &full_bar[stage]);
+          if constexpr (PAIR) {
+            if (cta == 0) tc::mbar_arrive_expect_tx(&full_bar[stage], 2 * STAGE);
+            tc::tma_load_2d_pair(sa, &tmA, kb * BKB, row, full0 + (uint32_t)stage * 8u);
+            tc::tma_load_2d_pair(sa + BM * BKB, &tmB, kb * BKB, col, full0 + (uint32_t)stage * 8u);
+          } else {
+            tc::mbar_arrive_expect_tx(&full_bar[stage], STAGE);
+            tc::tma_load_2d(sa, &tmA, kb * BKB, row, &full_bar[stage]);
+            tc::tma_load_2d(sa + BM * BKB, &tmB, kb * BKB, col, &full_bar[stage]);
+          }
         }
-        ++issued;
+        ++issued_blocks;
         if (++stage == NST) {
           stage = 0;
           phase ^= 1u;
         }
       }
       if (!ok) {
-        give_up(&abort_flag, 31);
+        stop(31);
         break;
       }
     }
-    // every load issued lands before the CTA may exit
-    for (int s = 0; s < NST && s < issued; ++s) {
-      const int last = s + (issued - 1 - s) / NST * NST;
-      if (!tc::mbar_wait(&full_bar[s], (uint32_t)((last / NST) & 1), nullptr, kWaitBudget))
-        atomicCAS(&g_int8_status, 0, 35);
+    if constexpr (PAIR) {  // CTA 0 drains the loads of both after the first cluster barrier
+      if (cta != 0 && lane == 0)
+        tc::st_cluster_u32(tc::cluster_addr(tc::smem_u32(&peer_issued_s), 0u), (uint32_t)issued_blocks);
+    } else {
+      drain(issued_blocks);
     }
   } else if (warp == 1) {
-    const uint64_t desc = tc::smem_desc(tc::smem_u32(ring), 16u, 1024u, tc::kLayoutSW128);
-    int stage = 0, i = 0;
-    uint32_t phase = 0;
-    bool issued = false, ok = true;
-    for (int t = blockIdx.x; t < total && ok; t += gridDim.x, ++i) {
-      const int acc = i & 1;
-      ok = tc::mbar_wait_warp(&tempty_bar[acc], ((uint32_t)(i >> 1) & 1u) ^ 1u, &abort_flag, budget);
-      if (!ok) {
-        give_up(&abort_flag, 32);
-        break;
-      }
-      tc::tc_fence_after();
-      for (int kb = 0; kb < p.kb; ++kb) {
-        ok = tc::mbar_wait_warp(&full_bar[stage], phase, &abort_flag, budget);
+    if (cta == 0) {
+      const uint64_t desc = tc::smem_desc(tc::smem_u32(ring), 16u, 1024u, tc::kLayoutSW128);
+      auto commit = [&](uint64_t* bar) {
+        if constexpr (PAIR) tc::mma_commit_both(bar);
+        else tc::mma_commit(bar);
+      };
+      int stage = 0, i = 0;
+      uint32_t phase = 0;
+      bool issued = false, ok = true;
+      for (int t = t_first; t < total && ok; t += t_step, ++i) {
+        const int acc = i & 1;
+        ok = tc::mbar_wait_warp(&tempty_bar[acc], ((uint32_t)(i >> 1) & 1u) ^ 1u, &abort_flag, budget);
         if (!ok) {
-          give_up(&abort_flag, 33);
+          stop(32);
           break;
         }
         tc::tc_fence_after();
-        // the start address of a descriptor is in units of 16 bytes; the ring ends below 2^18
-        const uint64_t da = desc + (uint64_t)(stage * (STAGE / 16)), db = da + BM * BKB / 16;
-        if (tc::elect_one()) {
+        for (int kb = 0; kb < p.kb; ++kb) {
+          ok = tc::mbar_wait_warp(&full_bar[stage], phase, &abort_flag, budget);
+          if (!ok) {
+            stop(33);
+            break;
+          }
+          tc::tc_fence_after();
+          // the start address of a descriptor is in units of 16 bytes; the ring ends below 2^18
+          const uint64_t da = desc + (uint64_t)(stage * (STAGE / 16)), db = da + BM * BKB / 16;
+          if (tc::elect_one()) {
 #pragma unroll
-          for (int k = 0; k < BKB / 32; ++k)
-            tc::mma_i8(tmem_base + (uint32_t)(acc * BN), da + k * 2, db + k * 2, IDESC, (kb > 0 || k > 0) ? 1u : 0u);
-          tc::mma_commit(&empty_bar[stage]);
-          if (kb == p.kb - 1) tc::mma_commit(&tfull_bar[acc]);
-        }
-        issued = true;
-        if (++stage == NST) {
-          stage = 0;
-          phase ^= 1u;
+            for (int k = 0; k < BKB / 32; ++k) {
+              const uint32_t d = tmem_base + (uint32_t)(acc * BN), more = (kb > 0 || k > 0) ? 1u : 0u;
+              if constexpr (PAIR) tc::mma_i8_pair(d, da + k * 2, db + k * 2, IDESC, more);
+              else tc::mma_i8(d, da + k * 2, db + k * 2, IDESC, more);
+            }
+            commit(&empty_bar[stage]);
+            if (kb == p.kb - 1) commit(&tfull_bar[acc]);
+          }
+          issued = true;
+          if (++stage == NST) {
+            stage = 0;
+            phase ^= 1u;
+          }
         }
       }
-    }
-    if (issued) {  // all MMAs complete before TMEM is freed
-      if (tc::elect_one()) tc::mma_commit(&done_bar);
-      if (!tc::mbar_wait(&done_bar, 0u, nullptr, kWaitBudget)) atomicCAS(&g_int8_status, 0, 36);
+      if (issued) {  // all MMAs complete before TMEM is freed
+        if (tc::elect_one()) commit(&done_bar);
+        if (!tc::mbar_wait(&done_bar, 0u, nullptr, kWaitBudget)) atomicCAS(&g_int8_status, 0, 36);
+      }
     }
   } else {
     const int quad = warp & 3, chalf = (warp - 2) >> 2;
     uint8_t* box = staging + (warp - 2) * kBox;
     int i = 0;
-    for (int t = blockIdx.x; t < total && !abort_flag; t += gridDim.x, ++i) {
+    for (int t = t_first; t < total && !abort_flag; t += t_step, ++i) {
       int m, n;
       tile_of(p, t, m, n);
       const int acc = i & 1;
-      const int row0 = m * BM + quad * 32, row = row0 + lane;
+      const int row0 = m * TM + (int)cta * BM + quad * 32, row = row0 + lane;
       const float sx = row < p.o.M ? p.o.sx[row] : 0.f;
       float sw[BN / 64], bw[BN / 64];  // of column lane + 32 j of the warp's half, in flight during the wait
 #pragma unroll
@@ -491,7 +535,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid
         bw[j] = col < p.o.N ? bias_at(p.o, col) : 0.f;
       }
       if (!tc::mbar_wait_warp(&tfull_bar[acc], (uint32_t)(i >> 1) & 1u, &abort_flag, budget)) {
-        give_up(&abort_flag, 34);
+        stop(34);
         break;
       }
       tc::tc_fence_after();
@@ -506,7 +550,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid
         if (c + BOX_COLS == BN / 2) {  // the accumulator is read: the next tile's products may start
           tc::tc_fence_before();
           __syncwarp();
-          if (lane == 0) tc::mbar_arrive(&tempty_bar[acc]);
+          if (lane == 0) {
+            if (PAIR && cta != 0) tc::mbar_arrive_cluster(tc::cluster_addr(tc::smem_u32(&tempty_bar[acc]), 0u));
+            else tc::mbar_arrive(&tempty_bar[acc]);
+          }
         }
         float v[BOX_COLS];
 #pragma unroll
@@ -556,8 +603,33 @@ __global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid
   }
   tc::tc_fence_before();
   __syncthreads();
-  tc::tc_fence_after();
-  if (warp == 1) tc::tmem_dealloc(tmem_base, 2 * BN);
+  if constexpr (PAIR) {
+    // CTA 0's MMAs read CTA 1's ring and write its TMEM, and CTA 1's loads and epilogue signal CTA 0's barriers.
+    // After the first barrier CTA 0 knows how many blocks each loaded.  Where only one of them loaded a block (the
+    // other gave up) it settles that block's count -- the half that never came counted as done, the half on its way
+    // expected -- and waits for every phase, so no load is in flight when the second barrier lets both exit.
+    tc::cluster_sync();
+    if (cta == 0 && warp == 0 && lane == 0) {
+      const int own = issued_blocks, peer = peer_issued_s;
+      const int lo = own < peer ? own : peer, hi = own < peer ? peer : own;
+      if (hi - lo > NST) {  // cannot happen: a stage is loaded again only after both halves of its last load
+        atomicCAS(&g_int8_status, 0, 37);
+      } else {
+        for (int k = lo; k < hi; ++k) {
+          if (k < own) tc::mbar_complete_tx(&full_bar[k % NST], STAGE);
+          else tc::mbar_arrive_expect_tx(&full_bar[k % NST], STAGE);
+        }
+        drain(hi);
+      }
+    }
+    __syncwarp();
+    tc::cluster_sync_relaxed();
+  }
+  if (warp == 1) {
+    tc::tc_fence_after();
+    if constexpr (PAIR) tc::tmem_dealloc_pair(tmem_base, 2 * BN);
+    else tc::tmem_dealloc(tmem_base, 2 * BN);
+  }
 }
 
 // -------------------------------------------------- tensor cores, few tokens
@@ -799,22 +871,59 @@ int dot(const void* x, const int8_t* w, int64_t ldw, const Out& o, int K, cudaSt
   const int warps = kDotThreads / 32;
   const int64_t want = (o.N + warps - 1) / warps, cap = (int64_t)num_sms() * 4;
   const unsigned grid = (unsigned)(want < cap ? want : cap);
-  return launch_after(int8_dot_kernel<T>, dim3(grid), kDotThreads, (int)padded_k(K), 1, st, "int8_dot",
+  return launch_after(int8_dot_kernel<T>, dim3(grid), kDotThreads, (int)padded_k(K), dim3(1), st, "int8_dot",
                       static_cast<const T*>(x), w, ldw, o, K, aligned16(x) ? 1 : 0);
 }
 
-template <typename T, int BN>
+// Pairs of CTAs that are resident at once on the current device.
+template <typename F>
+int pairs_that_fit(F kernel, int smem, int* out) {
+  static thread_local int fit[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return fail(ATS_ECUDA, "int8_tile: no current device");
+  if (fit[dev] == 0) {
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(num_sms() / 2 * 2));
+    cfg.blockDim = dim3(kTileThreads);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    int n = 0;
+    if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
+    if (e != cudaSuccess || n < 1) return fail(ATS_ECUDA, "int8_tile: no pair fits (%s)", cudaGetErrorString(e));
+    fit[dev] = n;
+  }
+  *out = fit[dev];
+  return ATS_OK;
+}
+
+template <typename T, int BN, bool PAIR>
 int tiles(const int8_t* q, int64_t ldq, const int8_t* w, int64_t ldw, const Out& o, int K, cudaStream_t st) {
+  constexpr int TM = PAIR ? 2 * BM : BM;
+  auto kernel = int8_tile_kernel<T, BN, PAIR>;
   CUtensorMap ma, mb;
   ATS_TRY(operand_map(&ma, q, K, o.M, ldq, BM));
-  ATS_TRY(operand_map(&mb, w, K, o.N, ldw, BN));
+  ATS_TRY(operand_map(&mb, w, K, o.N, ldw, PAIR ? BN / 2 : BN));
   const int vec = (int64_t)o.N * (int64_t)sizeof(T) % 16 == 0 && aligned16(o.y);
-  const TileArgs p{o, (K + BKB - 1) / BKB, (o.M + BM - 1) / BM, (o.N + BN - 1) / BN, vec};
+  const TileArgs p{o, (K + BKB - 1) / BKB, (o.M + TM - 1) / TM, (o.N + BN - 1) / BN, vec};
   const int64_t total = (int64_t)p.mt * p.nt;
   if (total > 0x7fffffff - 4096) return fail(ATS_EUNSUPPORTED, "int8_linear: too many tiles");
-  const int grid = total < gemm_ctas() ? (int)total : gemm_ctas();
-  const int smem = 1024 + tile_stages(BN) * tile_stage_bytes(BN) + kEpiWarps * kBox;
-  return launch_after(int8_tile_kernel<T, BN>, dim3((unsigned)grid), kTileThreads, smem, 1, st, "int8_tile", ma, mb, p);
+  const int smem = 1024 + tile_stages(BN, PAIR) * tile_stage_bytes(BN, PAIR) + kEpiWarps * kBox;
+  int64_t at_once = gemm_ctas();
+  if (PAIR) {
+    int fit = 0;
+    ATS_TRY(pairs_that_fit(kernel, smem, &fit));
+    at_once = at_once / 2 < fit ? at_once / 2 : fit;
+    if (at_once < 1) at_once = 1;
+  }
+  const unsigned grid = (unsigned)(total < at_once ? total : at_once) * (PAIR ? 2 : 1);
+  return launch_after(kernel, dim3(grid), kTileThreads, smem, dim3(PAIR ? 2 : 1), st, "int8_tile", ma, mb, p);
 }
 
 template <typename T, int TN>
@@ -825,7 +934,7 @@ int parts(const int8_t* q, int64_t ldq, const int8_t* w, int64_t ldw, const Out&
   const dim3 grid((unsigned)((o.N + BM - 1) / BM), (unsigned)((o.M + TN - 1) / TN), (unsigned)split);
   const int nst = part_stages(TN, (int64_t)grid.x * grid.y * grid.z <= num_sms());
   const int smem = 1024 + nst * part_stage_bytes(TN);
-  return launch_after(int8_part_kernel<T, TN>, grid, kPartThreads, smem, split, st, "int8_part", mw, mx, o,
+  return launch_after(int8_part_kernel<T, TN>, grid, kPartThreads, smem, dim3(1, 1, (unsigned)split), st, "int8_part", mw, mx, o,
                       (K + BKB - 1) / BKB, nst, o.N % 4 == 0 && aligned16(o.y) ? 1 : 0);
 }
 
@@ -852,9 +961,9 @@ int linear(const void* x, int64_t ldx, const int8_t* w, int64_t ldw, Out o, int6
     }
   }
   // 256 columns read fewer bytes per product; 128 where they leave fewer SMs idle.
-  const int64_t mt = (o.M + BM - 1) / BM;
-  return mt * ((o.N + 255) / 256) > num_sms() * 3 / 4 ? tiles<T, 256>(q, ldq, w, ldw, o, (int)K, st)
-                                                      : tiles<T, 128>(q, ldq, w, ldw, o, (int)K, st);
+  const int64_t mt = (o.M + BM - 1) / BM, nt256 = (o.N + 255) / 256;
+  if (mt * nt256 <= num_sms() * 3 / 4) return tiles<T, 128, false>(q, ldq, w, ldw, o, (int)K, st);
+  return tiles<T, 256, true>(q, ldq, w, ldw, o, (int)K, st);
 }
 
 }  // namespace

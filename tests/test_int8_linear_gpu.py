@@ -86,7 +86,8 @@ def test_feature_counts(M, N, K, dt):
     check(M, N, K, dt, bias=True, seed=N + K)
 
 
-@pytest.mark.parametrize("M,N,K", [(2048, 1024, 2048), (1111, 2056, 1000), (4100, 520, 272), (700, 11264, 512)])
+@pytest.mark.parametrize("M,N,K", [(2048, 1024, 2048), (1111, 2056, 1000), (4100, 520, 272), (700, 11264, 512), (5001, 1003, 260),
+                                   (2000, 3001, 500), (4500, 4500, 64), (2304, 4096, 16), (1400, 2500, 130)])
 @pytest.mark.parametrize("dt", ["bf16", "f32"])
 def test_larger_products(M, N, K, dt):
     check(M, N, K, dt, bias=True)
