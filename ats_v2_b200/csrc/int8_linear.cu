@@ -244,6 +244,10 @@ struct Out {
   int M, N;
 };
 
+// The scaled sum, and the bias added: rounded apart in every kernel here (never fused), so that a token's result does
+// not depend on how many come with it.
+__device__ __forceinline__ float scaled(int sum, float sx, float sw) { return __fmul_rn((float)sum, __fmul_rn(sx, sw)); }
+
 __device__ __forceinline__ float bias_at(const Out& o, int n) {
   if (o.bias == nullptr) return 0.f;
   return o.bias_bf16 ? __bfloat162float(static_cast<const bf16*>(o.bias)[n]) : static_cast<const float*>(o.bias)[n];
@@ -254,7 +258,7 @@ __device__ __forceinline__ float bias_at(const Out& o, int n) {
 // its warps already in flight, then a warp takes an output channel at a time: 16 weights per lane and step against
 // the token's integers.  The weights are read once; they bound it.
 constexpr int kDotThreads = 256, kDotStep = 8;
-constexpr int kDotSmem = 48 * 1024;  // longest token, in bytes
+constexpr int kDotLongest = 16384;  // a warp walks its channels 4 KB at a time: longer rows are split over SMs instead
 
 template <typename T>
 __global__ void __launch_bounds__(kDotThreads, 4) int8_dot_kernel(const T* __restrict__ x,
@@ -323,29 +327,29 @@ __global__ void __launch_bounds__(kDotThreads, 4) int8_dot_kernel(const T* __res
     if (lane < 16 && k < K) acc += (int)w[n * ldw + k] * (int)qs[k];
     acc = warp_sum_i(acc);
     if (lane == 0) {
-      float v = (float)acc * (sx * o.sw[n]);
-      if (o.bias != nullptr) v += bias_at(o, (int)n);
+      float v = scaled(acc, sx, o.sw[n]);
+      if (o.bias != nullptr) v = __fadd_rn(v, bias_at(o, (int)n));
       static_cast<T*>(o.y)[n] = Cvt<T>::from_f(v);
     }
   }
 }
 
 // ------------------------------------------------- tensor cores, many tokens
-// tcgen05.mma kind::i8, K in blocks of 128 bytes: one persistent CTA per SM, a TMA producer warp, an MMA warp with
-// two accumulators in TMEM, eight epilogue warps (two per TMEM lane quadrant, half of the columns each) that scale,
-// round and store whole 128-byte pieces of rows through a swizzled box in shared memory.
-//
-// PAIR: two CTAs of a cluster share a tile of 256 tokens x BN channels (cta_group::2).  Each loads its 128 tokens
-// and half of the channels, 32 KB a block instead of 48: single CTAs are held by what L2 delivers to the SMs, about
-// 15 TB/s.  All loads of a block count on CTA 0's full barrier; CTA 0 issues the MMAs and its commits reach the
-// empty and accumulator barriers of both; both epilogues release the accumulator on CTA 0.
+// tcgen05.mma kind::i8, K in blocks of 128 bytes, 256 tokens x 256 channels on a cluster of two CTAs (cta_group::2):
+// persistent, each CTA with a TMA producer warp and eight epilogue warps (two per TMEM lane quadrant, half of the
+// columns each) that scale, round and store whole 128-byte pieces of rows through a swizzled box in shared memory;
+// CTA 0's MMA warp issues for both, into two accumulators.  Each CTA loads its 128 tokens and half of the channels,
+// 32 KB a block where a single CTA of 128 x 256 loads 48: single CTAs were held by what L2 delivers to the SMs, about
+// 15 TB/s (8192^3: 440 us, 386 us in pairs).  All loads of a block count on CTA 0's full barrier; its commits reach
+// the empty and accumulator barriers of both; both epilogues release the accumulator on CTA 0.  A block takes 509 to
+// 544 SM cycles against the 512 of its MMAs, so the clock under the power limit bounds it.
 constexpr int BM = 128, BKB = 128;
 constexpr int kEpiWarps = 8, kTileThreads = 64 + 32 * kEpiWarps;
 constexpr int kBox = 32 * 128;  // an epilogue warp's staging: 32 rows of 128 bytes
 constexpr int kBandM = 16;                        // M tiles per band of the tile order
 
-__host__ __device__ constexpr int tile_stage_bytes(int bn, bool pair) { return (BM + (pair ? bn / 2 : bn)) * BKB; }
-__host__ __device__ constexpr int tile_stages(int bn, bool pair) { return 192 * 1024 / tile_stage_bytes(bn, pair); }
+constexpr int TM = 2 * BM, BN = 256, B_ROWS = BN / 2;  // a pair's tile, and the channels one CTA loads
+constexpr int kTileStage = (BM + B_ROWS) * BKB, kTileStages = 192 * 1024 / kTileStage;
 
 struct TileArgs {
   Out o;
@@ -364,12 +368,11 @@ __device__ __forceinline__ void tile_of(const TileArgs& p, int t, int& m, int& n
   m = m0 + (r - n * gm);
 }
 
-template <typename T, int BN, bool PAIR>
+template <typename T>
 __global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid_constant__ CUtensorMap tmA,
                                                                    const __grid_constant__ CUtensorMap tmB,
                                                                    TileArgs p) {
-  constexpr int TM = PAIR ? 2 * BM : BM, B_ROWS = PAIR ? BN / 2 : BN;
-  constexpr int STAGE = tile_stage_bytes(BN, PAIR), NST = tile_stages(BN, PAIR);
+  constexpr int STAGE = kTileStage, NST = kTileStages;
   constexpr uint32_t IDESC = tc::idesc_i8(TM, BN);
   constexpr int BOX_COLS = 128 / (int)sizeof(T);
   extern __shared__ uint8_t smem_raw[];
@@ -377,16 +380,16 @@ __global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid
   uint8_t* staging = ring + NST * STAGE;
   __shared__ __align__(8) uint64_t full_bar[NST], empty_bar[NST], tfull_bar[2], tempty_bar[2], done_bar;
   __shared__ uint32_t tmem_base_s;
-  __shared__ int peer_issued_s;  // PAIR, CTA 0: blocks that CTA 1 loaded
+  __shared__ int peer_issued_s;  // CTA 0: blocks that CTA 1 loaded
   __shared__ volatile int abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long budget = g_int8_wait_budget;
   const int total = p.mt * p.nt;
-  const uint32_t cta = PAIR ? tc::cluster_ctarank() : 0u;
-  const int t_first = PAIR ? (int)blockIdx.x / 2 : (int)blockIdx.x, t_step = PAIR ? (int)gridDim.x / 2 : (int)gridDim.x;
+  const uint32_t cta = tc::cluster_ctarank();
+  const int t_first = (int)blockIdx.x / 2, t_step = (int)gridDim.x / 2;
   auto stop = [&](int code) {  // a role that gives up stops the others, in both CTAs of a pair
     give_up(&abort_flag, code);
-    if constexpr (PAIR) tc::st_cluster_u32(tc::cluster_addr(tc::smem_u32((const void*)&abort_flag), cta ^ 1u), 1u);
+    tc::st_cluster_u32(tc::cluster_addr(tc::smem_u32((const void*)&abort_flag), cta ^ 1u), 1u);
   };
   if (threadIdx.x == 0) {
     for (int s = 0; s < NST; ++s) {
@@ -395,7 +398,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid
     }
     for (int a = 0; a < 2; ++a) {
       tc::mbar_init(&tfull_bar[a], 1);
-      tc::mbar_init(&tempty_bar[a], PAIR ? 2 * kEpiWarps : kEpiWarps);
+      tc::mbar_init(&tempty_bar[a], 2 * kEpiWarps);
     }
     tc::mbar_init(&done_bar, 1);
     tc::fence_barrier_init();
@@ -403,17 +406,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid
     abort_flag = 0;
   }
   if (warp == 1) {
-    if constexpr (PAIR) {
-      tc::tmem_alloc_pair(&tmem_base_s, 2 * BN);
-      tc::tmem_relinquish_pair();
-    } else {
-      tc::tmem_alloc(&tmem_base_s, 2 * BN);
-      tc::tmem_relinquish();
-    }
+    tc::tmem_alloc_pair(&tmem_base_s, 2 * BN);
+    tc::tmem_relinquish_pair();
   }
   tc::tc_fence_before();
   __syncthreads();
-  if constexpr (PAIR) tc::cluster_sync();  // both CTAs' barriers exist before either signals the other's
+  tc::cluster_sync();  // both CTAs' barriers exist before either signals the other's
   tc::tc_fence_after();
   const uint32_t tmem_base = tmem_base_s;
   // every load issued lands before the CTA may exit: the last phase of each stage of the first `issued` blocks
@@ -430,7 +428,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid
   if (warp == 0) {
     int stage = 0;
     uint32_t phase = 0;
-    const uint32_t full0 = PAIR ? tc::cluster_addr(tc::smem_u32(&full_bar[0]), 0u) : 0u;
+    const uint32_t full0 = tc::cluster_addr(tc::smem_u32(&full_bar[0]), 0u);
     for (int t = t_first; t < total; t += t_step) {
       int m, n;
       tile_of(p, t, m, n);
@@ -441,15 +439,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid
         if (!ok) break;
         if (tc::elect_one()) {
           uint8_t* sa = ring + stage * STAGE;
-          if constexpr (PAIR) {
-            if (cta == 0) tc::mbar_arrive_expect_tx(&full_bar[stage], 2 * STAGE);
-            tc::tma_load_2d_pair(sa, &tmA, kb * BKB, row, full0 + (uint32_t)stage * 8u);
-            tc::tma_load_2d_pair(sa + BM * BKB, &tmB, kb * BKB, col, full0 + (uint32_t)stage * 8u);
-          } else {
-            tc::mbar_arrive_expect_tx(&full_bar[stage], STAGE);
-            tc::tma_load_2d(sa, &tmA, kb * BKB, row, &full_bar[stage]);
-            tc::tma_load_2d(sa + BM * BKB, &tmB, kb * BKB, col, &full_bar[stage]);
-          }
+          if (cta == 0) tc::mbar_arrive_expect_tx(&full_bar[stage], 2 * STAGE);
+          tc::tma_load_2d_pair(sa, &tmA, kb * BKB, row, full0 + (uint32_t)stage * 8u);
+          tc::tma_load_2d_pair(sa + BM * BKB, &tmB, kb * BKB, col, full0 + (uint32_t)stage * 8u);
         }
         ++issued_blocks;
         if (++stage == NST) {
@@ -462,19 +454,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid
         break;
       }
     }
-    if constexpr (PAIR) {  // CTA 0 drains the loads of both after the first cluster barrier
-      if (cta != 0 && lane == 0)
-        tc::st_cluster_u32(tc::cluster_addr(tc::smem_u32(&peer_issued_s), 0u), (uint32_t)issued_blocks);
-    } else {
-      drain(issued_blocks);
-    }
+    if (cta != 0 && lane == 0)  // CTA 0 drains the loads of both after the first cluster barrier
+      tc::st_cluster_u32(tc::cluster_addr(tc::smem_u32(&peer_issued_s), 0u), (uint32_t)issued_blocks);
   } else if (warp == 1) {
     if (cta == 0) {
       const uint64_t desc = tc::smem_desc(tc::smem_u32(ring), 16u, 1024u, tc::kLayoutSW128);
-      auto commit = [&](uint64_t* bar) {
-        if constexpr (PAIR) tc::mma_commit_both(bar);
-        else tc::mma_commit(bar);
-      };
       int stage = 0, i = 0;
       uint32_t phase = 0;
       bool issued = false, ok = true;
@@ -497,13 +481,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid
           const uint64_t da = desc + (uint64_t)(stage * (STAGE / 16)), db = da + BM * BKB / 16;
           if (tc::elect_one()) {
 #pragma unroll
-            for (int k = 0; k < BKB / 32; ++k) {
-              const uint32_t d = tmem_base + (uint32_t)(acc * BN), more = (kb > 0 || k > 0) ? 1u : 0u;
-              if constexpr (PAIR) tc::mma_i8_pair(d, da + k * 2, db + k * 2, IDESC, more);
-              else tc::mma_i8(d, da + k * 2, db + k * 2, IDESC, more);
-            }
-            commit(&empty_bar[stage]);
-            if (kb == p.kb - 1) commit(&tfull_bar[acc]);
+            for (int k = 0; k < BKB / 32; ++k)
+              tc::mma_i8_pair(tmem_base + (uint32_t)(acc * BN), da + k * 2, db + k * 2, IDESC,
+                              (kb > 0 || k > 0) ? 1u : 0u);
+            tc::mma_commit_both(&empty_bar[stage]);
+            if (kb == p.kb - 1) tc::mma_commit_both(&tfull_bar[acc]);
           }
           issued = true;
           if (++stage == NST) {
@@ -513,7 +495,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid
         }
       }
       if (issued) {  // all MMAs complete before TMEM is freed
-        if (tc::elect_one()) commit(&done_bar);
+        if (tc::elect_one()) tc::mma_commit_both(&done_bar);
         if (!tc::mbar_wait(&done_bar, 0u, nullptr, kWaitBudget)) atomicCAS(&g_int8_status, 0, 36);
       }
     }
@@ -551,17 +533,18 @@ __global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid
           tc::tc_fence_before();
           __syncwarp();
           if (lane == 0) {
-            if (PAIR && cta != 0) tc::mbar_arrive_cluster(tc::cluster_addr(tc::smem_u32(&tempty_bar[acc]), 0u));
+            if (cta != 0) tc::mbar_arrive_cluster(tc::cluster_addr(tc::smem_u32(&tempty_bar[acc]), 0u));
             else tc::mbar_arrive(&tempty_bar[acc]);
           }
         }
         float v[BOX_COLS];
 #pragma unroll
         for (int e = 0; e < BOX_COLS; ++e)
-          v[e] = (float)(int)r[e] * (sx * __shfl_sync(0xffffffffu, sw[(c + e) / 32], (c + e) % 32));
+          v[e] = scaled((int)r[e], sx, __shfl_sync(0xffffffffu, sw[(c + e) / 32], (c + e) % 32));
         if (p.o.bias != nullptr)  // one branch: one for each element would serialise them
 #pragma unroll
-          for (int e = 0; e < BOX_COLS; ++e) v[e] += __shfl_sync(0xffffffffu, bw[(c + e) / 32], (c + e) % 32);
+          for (int e = 0; e < BOX_COLS; ++e)
+            v[e] = __fadd_rn(v[e], __shfl_sync(0xffffffffu, bw[(c + e) / 32], (c + e) % 32));
 #pragma unroll
         for (int q = 0; q < 8; ++q) {  // row `lane`, 16-byte piece q at its swizzled place (conflict-free)
           float u[Chunk<T>::N];
@@ -603,32 +586,29 @@ __global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid
   }
   tc::tc_fence_before();
   __syncthreads();
-  if constexpr (PAIR) {
-    // CTA 0's MMAs read CTA 1's ring and write its TMEM, and CTA 1's loads and epilogue signal CTA 0's barriers.
-    // After the first barrier CTA 0 knows how many blocks each loaded.  Where only one of them loaded a block (the
-    // other gave up) it settles that block's count -- the half that never came counted as done, the half on its way
-    // expected -- and waits for every phase, so no load is in flight when the second barrier lets both exit.
-    tc::cluster_sync();
-    if (cta == 0 && warp == 0 && lane == 0) {
-      const int own = issued_blocks, peer = peer_issued_s;
-      const int lo = own < peer ? own : peer, hi = own < peer ? peer : own;
-      if (hi - lo > NST) {  // cannot happen: a stage is loaded again only after both halves of its last load
-        atomicCAS(&g_int8_status, 0, 37);
-      } else {
-        for (int k = lo; k < hi; ++k) {
-          if (k < own) tc::mbar_complete_tx(&full_bar[k % NST], STAGE);
-          else tc::mbar_arrive_expect_tx(&full_bar[k % NST], STAGE);
-        }
-        drain(hi);
+  // CTA 0's MMAs read CTA 1's ring and write its TMEM, and CTA 1's loads and epilogue signal CTA 0's barriers.  After
+  // the first barrier CTA 0 knows how many blocks each loaded.  Where only one of them loaded a block (the other gave
+  // up) it settles that block's count -- the half that never came counted as done, the half on its way expected -- and
+  // waits for every phase, so no load is in flight when the second barrier lets both exit.
+  tc::cluster_sync();
+  if (cta == 0 && warp == 0 && lane == 0) {
+    const int own = issued_blocks, peer = peer_issued_s;
+    const int lo = own < peer ? own : peer, hi = own < peer ? peer : own;
+    if (hi - lo > NST) {  // cannot happen: a stage is loaded again only after both halves of its last load
+      atomicCAS(&g_int8_status, 0, 37);
+    } else {
+      for (int k = lo; k < hi; ++k) {
+        if (k < own) tc::mbar_complete_tx(&full_bar[k % NST], STAGE);
+        else tc::mbar_arrive_expect_tx(&full_bar[k % NST], STAGE);
       }
+      drain(hi);
     }
-    __syncwarp();
-    tc::cluster_sync_relaxed();
   }
+  __syncwarp();
+  tc::cluster_sync_relaxed();
   if (warp == 1) {
     tc::tc_fence_after();
-    if constexpr (PAIR) tc::tmem_dealloc_pair(tmem_base, 2 * BN);
-    else tc::tmem_dealloc(tmem_base, 2 * BN);
+    tc::tmem_dealloc_pair(tmem_base, 2 * BN);
   }
 }
 
@@ -639,10 +619,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid
 // workspace or atomics are needed.  The weights' loads start before the quantisation has ended.
 constexpr int kPartThreads = 64 + 32 * kEpiWarps, kMaxSplit = 8;
 
-// The ring takes what the SM has where one CTA comes to an SM, and half of it where two do: a part waits on load
-// latency, and more bytes in flight hide more of it.
+// Two CTAs share an SM, with half of its shared memory each.
 __host__ __device__ constexpr int part_stage_bytes(int tn) { return (BM + tn) * BKB; }
-__host__ __device__ constexpr int part_stages(int tn, bool alone) { return (alone ? 208 : 104) * 1024 / part_stage_bytes(tn); }
+__host__ __device__ constexpr int part_stages(int tn) { return 104 * 1024 / part_stage_bytes(tn); }
 
 struct PartOut {
   const int* tile;                     // [TN][128] sums of this CTA's part of K
@@ -683,9 +662,11 @@ __device__ __forceinline__ void reduce_parts(const Out& o, const PartOut& p) {
 #pragma unroll
       for (int z = 1; z < S; ++z) a.x += b[u][z].x, a.y += b[u][z].y, a.z += b[u][z].z, a.w += b[u][z].w;
       const float sx = i < share ? p.sx_s[p.first + i] : 0.f;
-      float v[4] = {(float)a.x * (sx * sw.x), (float)a.y * (sx * sw.y), (float)a.z * (sx * sw.z),
-                    (float)a.w * (sx * sw.w)};
-      if (o.bias != nullptr) v[0] += bw.x, v[1] += bw.y, v[2] += bw.z, v[3] += bw.w;
+      float v[4] = {scaled(a.x, sx, sw.x), scaled(a.y, sx, sw.y), scaled(a.z, sx, sw.z), scaled(a.w, sx, sw.w)};
+      if (o.bias != nullptr) {
+        v[0] = __fadd_rn(v[0], bw.x), v[1] = __fadd_rn(v[1], bw.y);
+        v[2] = __fadd_rn(v[2], bw.z), v[3] = __fadd_rn(v[3], bw.w);
+      }
       T* y = static_cast<T*>(o.y) + (int64_t)(p.m0 + p.first + i) * o.N + n;
       if (whole && i < share) {
         T e[4] = {Cvt<T>::from_f(v[0]), Cvt<T>::from_f(v[1]), Cvt<T>::from_f(v[2]), Cvt<T>::from_f(v[3])};
@@ -703,13 +684,13 @@ __device__ __forceinline__ void reduce_parts(const Out& o, const PartOut& p) {
 template <typename T, int TN>
 __global__ void __launch_bounds__(kPartThreads, 2) int8_part_kernel(const __grid_constant__ CUtensorMap tmW,
                                                                    const __grid_constant__ CUtensorMap tmX, Out o,
-                                                                   int kb_all, int nst, int vec_out) {
-  constexpr int STAGE = part_stage_bytes(TN), MAXST = part_stages(TN, true);
+                                                                   int kb_all, int vec_out) {
+  constexpr int STAGE = part_stage_bytes(TN), NST = part_stages(TN);
   constexpr int TCOLS = TN < 32 ? 32 : TN;
   constexpr uint32_t IDESC = tc::idesc_i8(BM, TN);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ __align__(8) uint64_t full_bar[MAXST], empty_bar[MAXST], tfull_bar;
+  __shared__ __align__(8) uint64_t full_bar[NST], empty_bar[NST], tfull_bar;
   __shared__ uint32_t tmem_base_s;
   __shared__ volatile int abort_flag;
   __shared__ float sx_s[TN];
@@ -720,7 +701,7 @@ __global__ void __launch_bounds__(kPartThreads, 2) int8_part_kernel(const __grid
   const int kb0 = (int)((int64_t)kb_all * part / split), kb1 = (int)((int64_t)kb_all * (part + 1) / split);
   const int n0 = blockIdx.x * BM, m0 = blockIdx.y * TN;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < nst; ++s) {
+    for (int s = 0; s < NST; ++s) {
       tc::mbar_init(&full_bar[s], 1);
       tc::mbar_init(&empty_bar[s], 1);
     }
@@ -740,7 +721,7 @@ __global__ void __launch_bounds__(kPartThreads, 2) int8_part_kernel(const __grid
 
   const int nkb = kb1 - kb0;
   if (warp == 0) {
-    const int ahead = nkb < nst ? nkb : nst;
+    const int ahead = nkb < NST ? nkb : NST;
     if (tc::elect_one())
       for (int s = 0; s < ahead; ++s) {
         tc::mbar_arrive_expect_tx(&full_bar[s], STAGE);
@@ -765,14 +746,14 @@ __global__ void __launch_bounds__(kPartThreads, 2) int8_part_kernel(const __grid
         tc::tma_load_2d(ring + stage * STAGE + BM * BKB, &tmX, (kb0 + i) * BKB, m0, &full_bar[stage]);
       }
       ++issued;
-      if (++stage == nst) {
+      if (++stage == NST) {
         stage = 0;
         phase ^= 1u;
       }
     }
-    for (int s = 0; s < nst && s < issued; ++s) {  // every load issued lands before the CTA may exit
-      const int last = s + (issued - 1 - s) / nst * nst;
-      if (!tc::mbar_wait(&full_bar[s], (uint32_t)((last / nst) & 1), nullptr, kWaitBudget))
+    for (int s = 0; s < NST && s < issued; ++s) {  // every load issued lands before the CTA may exit
+      const int last = s + (issued - 1 - s) / NST * NST;
+      if (!tc::mbar_wait(&full_bar[s], (uint32_t)((last / NST) & 1), nullptr, kWaitBudget))
         atomicCAS(&g_int8_status, 0, 45);
     }
   } else if (warp == 1) {
@@ -792,7 +773,7 @@ __global__ void __launch_bounds__(kPartThreads, 2) int8_part_kernel(const __grid
           tc::mma_i8(tmem_base, da + k * 2, db + k * 2, IDESC, (i > 0 || k > 0) ? 1u : 0u);
         tc::mma_commit(&empty_bar[stage]);
       }
-      if (++stage == nst) {
+      if (++stage == NST) {
         stage = 0;
         phase ^= 1u;
       }
@@ -903,27 +884,23 @@ int pairs_that_fit(F kernel, int smem, int* out) {
   return ATS_OK;
 }
 
-template <typename T, int BN, bool PAIR>
+template <typename T>
 int tiles(const int8_t* q, int64_t ldq, const int8_t* w, int64_t ldw, const Out& o, int K, cudaStream_t st) {
-  constexpr int TM = PAIR ? 2 * BM : BM;
-  auto kernel = int8_tile_kernel<T, BN, PAIR>;
+  auto kernel = int8_tile_kernel<T>;
   CUtensorMap ma, mb;
   ATS_TRY(operand_map(&ma, q, K, o.M, ldq, BM));
-  ATS_TRY(operand_map(&mb, w, K, o.N, ldw, PAIR ? BN / 2 : BN));
+  ATS_TRY(operand_map(&mb, w, K, o.N, ldw, B_ROWS));
   const int vec = (int64_t)o.N * (int64_t)sizeof(T) % 16 == 0 && aligned16(o.y);
   const TileArgs p{o, (K + BKB - 1) / BKB, (o.M + TM - 1) / TM, (o.N + BN - 1) / BN, vec};
   const int64_t total = (int64_t)p.mt * p.nt;
   if (total > 0x7fffffff - 4096) return fail(ATS_EUNSUPPORTED, "int8_linear: too many tiles");
-  const int smem = 1024 + tile_stages(BN, PAIR) * tile_stage_bytes(BN, PAIR) + kEpiWarps * kBox;
-  int64_t at_once = gemm_ctas();
-  if (PAIR) {
-    int fit = 0;
-    ATS_TRY(pairs_that_fit(kernel, smem, &fit));
-    at_once = at_once / 2 < fit ? at_once / 2 : fit;
-    if (at_once < 1) at_once = 1;
-  }
-  const unsigned grid = (unsigned)(total < at_once ? total : at_once) * (PAIR ? 2 : 1);
-  return launch_after(kernel, dim3(grid), kTileThreads, smem, dim3(PAIR ? 2 : 1), st, "int8_tile", ma, mb, p);
+  const int smem = 1024 + kTileStages * kTileStage + kEpiWarps * kBox;
+  int pairs = 0;
+  ATS_TRY(pairs_that_fit(kernel, smem, &pairs));
+  if (pairs > gemm_ctas() / 2) pairs = gemm_ctas() / 2;
+  if (pairs > total) pairs = (int)total;
+  if (pairs < 1) pairs = 1;
+  return launch_after(kernel, dim3(2 * (unsigned)pairs), kTileThreads, smem, dim3(2), st, "int8_tile", ma, mb, p);
 }
 
 template <typename T, int TN>
@@ -932,38 +909,37 @@ int parts(const int8_t* q, int64_t ldq, const int8_t* w, int64_t ldw, const Out&
   ATS_TRY(operand_map(&mw, w, K, o.N, ldw, BM));
   ATS_TRY(operand_map(&mx, q, K, o.M, ldq, TN));
   const dim3 grid((unsigned)((o.N + BM - 1) / BM), (unsigned)((o.M + TN - 1) / TN), (unsigned)split);
-  const int nst = part_stages(TN, (int64_t)grid.x * grid.y * grid.z <= num_sms());
-  const int smem = 1024 + nst * part_stage_bytes(TN);
+  const int smem = 1024 + part_stages(TN) * part_stage_bytes(TN);
   return launch_after(int8_part_kernel<T, TN>, grid, kPartThreads, smem, dim3(1, 1, (unsigned)split), st, "int8_part", mw, mx, o,
-                      (K + BKB - 1) / BKB, nst, o.N % 4 == 0 && aligned16(o.y) ? 1 : 0);
+                      (K + BKB - 1) / BKB, o.N % 4 == 0 && aligned16(o.y) ? 1 : 0);
 }
 
 template <typename T>
 int linear(const void* x, int64_t ldx, const int8_t* w, int64_t ldw, Out o, int64_t K, int8_t* q, float* sx,
            cudaStream_t st) {
-  if (o.M == 1 && padded_k(K) <= kDotSmem - 1024) return dot<T>(x, w, ldw, o, (int)K, st);
+  if (o.M == 1 && K <= kDotLongest) return dot<T>(x, w, ldw, o, (int)K, st);
   const int64_t ldq = padded_k(K);
   ATS_TRY(quantize_t<T>(x, ldx, q, ldq, sx, o.M, K, st));
   o.sx = sx;
-  const int64_t nt = (o.N + BM - 1) / BM;
+  // Few tiles of 128 channels: as many token columns as hold the tokens, at most 64, or 128 where 64 would make more
+  // than two CTAs per SM.  K is split while that gives idle SMs work (2 blocks of K to a part) or an SM a second CTA
+  // (8 blocks), and while the parts to be summed stay within 256 columns: 48 tokens 4096x11008, in us: 25.7 whole,
+  // 16.6 in 2, 12.6 in 4, 16.2 in 8; 1024^3: 7.8 whole, 8.8 in 2; 4 tokens 4096x4096: 11.8 whole, 7.4 in 4.
+  const int64_t nt = (o.N + BM - 1) / BM, two = 2 * (int64_t)num_sms();
   const int kb = (int)((K + BKB - 1) / BKB);
-  // Few tokens: as many columns as hold them, and K split until two CTAs share each SM (a part keeps 2 blocks).
-  const int tn = o.M <= 16 ? 16 : o.M <= 32 ? 32 : o.M <= 64 ? 64 : 128;
-  const int64_t part_tiles = nt * ((o.M + tn - 1) / tn);
-  if (part_tiles <= 2 * num_sms() && (o.M + tn - 1) / tn <= 65535) {
-    int split = 1;
-    while (split < kMaxSplit && part_tiles * split * 2 <= 2 * num_sms() && kb >= split * 4) split *= 2;
-    switch (tn) {
-      case 16: return parts<T, 16>(q, ldq, w, ldw, o, (int)K, split, st);
-      case 32: return parts<T, 32>(q, ldq, w, ldw, o, (int)K, split, st);
-      case 64: return parts<T, 64>(q, ldq, w, ldw, o, (int)K, split, st);
-      default: return parts<T, 128>(q, ldq, w, ldw, o, (int)K, split, st);
-    }
+  const int tn = o.M <= 16 ? 16 : o.M <= 32 ? 32 : nt * ((o.M + 63) / 64) <= two ? 64 : 128;
+  const int64_t mt = (o.M + tn - 1) / tn, ctas = nt * mt;
+  if (ctas > two || mt > 65535) return tiles<T>(q, ldq, w, ldw, o, (int)K, st);
+  int split = 1;
+  while (split < kMaxSplit && 2 * split * tn <= 256 && 2 * split * ctas <= two &&
+         kb >= 2 * split * (2 * split * ctas <= num_sms() ? 2 : 8))
+    split *= 2;
+  switch (tn) {
+    case 16: return parts<T, 16>(q, ldq, w, ldw, o, (int)K, split, st);
+    case 32: return parts<T, 32>(q, ldq, w, ldw, o, (int)K, split, st);
+    case 64: return parts<T, 64>(q, ldq, w, ldw, o, (int)K, split, st);
+    default: return parts<T, 128>(q, ldq, w, ldw, o, (int)K, split, st);
   }
-  // 256 columns read fewer bytes per product; 128 where they leave fewer SMs idle.
-  const int64_t mt = (o.M + BM - 1) / BM, nt256 = (o.N + 255) / 256;
-  if (mt * nt256 <= num_sms() * 3 / 4) return tiles<T, 128, false>(q, ldq, w, ldw, o, (int)K, st);
-  return tiles<T, 256, true>(q, ldq, w, ldw, o, (int)K, st);
 }
 
 }  // namespace
