@@ -17,6 +17,8 @@
 // All arithmetic is float32, each result rounded once.  HBM bounds it: the
 // forward reads two rows and writes two, the backward reads four and writes
 // two.
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace ats {
@@ -61,8 +63,357 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
   return t;
 }
 
+// ------------------------------------------------------------ rows in registers
+// One block walks a run of consecutive rows; a thread owns NV vectors of VB bytes of every row, so its weights, gate
+// (per span) and sums over rows stay in its registers.  Each thread copies its own pieces of the rows ahead into its
+// own slots of shared memory (cp.async), STAGES rows deep: no thread reads another's, so the only barriers are the two
+// row sums.  Measured at 16384 x 4096 bf16 against the loads issued straight into registers: see the entry points.
+template <int BYTES> struct Raw;
+template <> struct Raw<16> { using type = uint4; };
+template <> struct Raw<8> { using type = uint2; };
+template <> struct Raw<4> { using type = uint32_t; };
+template <> struct Raw<2> { using type = uint16_t; };
+
+template <int BYTES>
+__device__ __forceinline__ void copy_ahead(void* dst, const void* src) {
+  if constexpr (BYTES == 2) {  // cp.async moves 4, 8 or 16 bytes
+    *static_cast<uint16_t*>(dst) = *static_cast<const uint16_t*>(src);
+  } else if constexpr (BYTES == 32) {
+    copy_ahead<16>(dst, src);
+    copy_ahead<16>(static_cast<char*>(dst) + 16, static_cast<const char*>(src) + 16);
+  } else {
+    const uint32_t d = static_cast<uint32_t>(__cvta_generic_to_shared(dst));
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(src) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(d), "l"(src), "n"(BYTES) : "memory");
+  }
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+constexpr int kRowThreads = 512;  // most threads of a row block
+__host__ __device__ constexpr int stages_of(int bytes) { return bytes >= 64 ? 1 : bytes >= 32 ? 2 : bytes >= 16 ? 4 : 8; }
+
+// One thread's view of its vectors: column of vector j, and whether the row has it.
+template <typename T, int VB, int NV>
+struct Mine {
+  static constexpr int VEC = VB / (int)sizeof(T), EPT = NV * VEC, STAGES = stages_of(NV * VB);
+  using R = typename Raw<VB>::type;
+  int nthr, tid, nvec;
+  __device__ __forceinline__ Mine(int H) : nthr((int)blockDim.x), tid((int)threadIdx.x), nvec(H / VEC) {}
+  __device__ __forceinline__ bool has(int j) const { return tid + j * nthr < nvec; }
+  __device__ __forceinline__ int col(int j) const { return (tid + j * nthr) * VEC; }
+  // slot of vector j of tensor t in stage st, of NT tensors
+  __device__ __forceinline__ char* slot(char* ring, int st, int t, int nt, int j) const {
+    return ring + ((size_t)((st * nt + t) * NV + j) * nthr + tid) * VB;
+  }
+  __device__ __forceinline__ void ahead(char* ring, int st, int t, int nt, const void* base, int64_t row, int H) const {
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+      if (has(j)) copy_ahead<VB>(slot(ring, st, t, nt, j), static_cast<const T*>(base) + row * H + col(j));
+  }
+  __device__ __forceinline__ void take(char* ring, int st, int t, int nt, float (&v)[EPT]) const {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      R raw{};
+      if (has(j)) raw = *reinterpret_cast<const R*>(slot(ring, st, t, nt, j));
+      const T* e = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[j * VEC + i] = Cvt<T>::to_f(e[i]);
+    }
+  }
+  // EPT values of a row of `p` (bf16 or float32, 16-byte aligned) from its first element `at`; 0 where the row has no
+  // such column
+  __device__ __forceinline__ void fetch(const void* p, int64_t at, int is_bf16, float (&v)[EPT]) const {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      float t[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) t[i] = 0.f;
+      if (has(j)) {
+        if (is_bf16) load_vec<bf16>(static_cast<const bf16*>(p) + at + col(j), t);
+        else load_vec<float>(static_cast<const float*>(p) + at + col(j), t);
+      }
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[j * VEC + i] = t[i];
+    }
+  }
+  template <typename U>
+  __device__ __forceinline__ static void load_vec(const U* p, float (&t)[VEC]) {
+    constexpr int BYTES = VEC * (int)sizeof(U), PIECE = BYTES > 16 ? 16 : BYTES, N = PIECE / (int)sizeof(U);
+#pragma unroll
+    for (int q = 0; q < BYTES / PIECE; ++q) {
+      const typename Raw<PIECE>::type raw = reinterpret_cast<const typename Raw<PIECE>::type*>(p)[q];
+      const U* e = reinterpret_cast<const U*>(&raw);
+#pragma unroll
+      for (int i = 0; i < N; ++i) t[q * N + i] = Cvt<U>::to_f(e[i]);
+    }
+  }
+  __device__ __forceinline__ void put(void* base, int64_t row, int H, const float (&v)[EPT]) const {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      R raw;
+      T* e = reinterpret_cast<T*>(&raw);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) e[i] = Cvt<T>::from_f(v[j * VEC + i]);
+      if (has(j)) *reinterpret_cast<R*>(static_cast<T*>(base) + row * H + col(j)) = raw;
+    }
+  }
+  // the same into a bf16 or float32 row that is 16-byte aligned
+  __device__ __forceinline__ void put_as(void* base, int64_t at, int is_bf16, const float (&v)[EPT]) const {
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+      if (has(j)) {
+        if (is_bf16) store_vec<bf16>(static_cast<bf16*>(base) + at + col(j), v + j * VEC);
+        else store_vec<float>(static_cast<float*>(base) + at + col(j), v + j * VEC);
+      }
+  }
+  template <typename U>
+  __device__ __forceinline__ static void store_vec(U* p, const float* v) {
+    constexpr int BYTES = VEC * (int)sizeof(U), PIECE = BYTES > 16 ? 16 : BYTES, N = PIECE / (int)sizeof(U);
+#pragma unroll
+    for (int q = 0; q < BYTES / PIECE; ++q) {
+      typename Raw<PIECE>::type raw;
+      U* e = reinterpret_cast<U*>(&raw);
+#pragma unroll
+      for (int i = 0; i < N; ++i) e[i] = Cvt<U>::from_f(v[q * N + i]);
+      reinterpret_cast<typename Raw<PIECE>::type*>(p)[q] = raw;
+    }
+  }
+};
+
+// Sum over the block by up to 16 warps.
+__device__ __forceinline__ float row_sum(float v, float4* red) {
+  v = warp_sum(v);
+  if (blockDim.x == 32) return v;
+  if ((threadIdx.x & 31) == 0) reinterpret_cast<float*>(red)[threadIdx.x >> 5] = v;
+  __syncthreads();
+  float t = 0.f;
+#pragma unroll
+  for (int i = 0; i < kRowThreads / 128; ++i) {
+    const float4 q = red[i];  // warps that are not there hold 0
+    t += (q.x + q.y) + (q.z + q.w);
+  }
+  return t;
+}
+
+// A thread's columns of the two weights and the gate: in registers, or, from 16 columns a thread on, in its own places
+// of shared memory (with 16 the backward's registers would spill).
+enum { W_POST = 0, W_PRE = 1, W_GATE = 2 };
+template <int EPT>
+struct Columns {
+  static constexpr bool SHARED = EPT >= 16;
+  float r[SHARED ? 1 : 3][SHARED ? 1 : EPT];
+  float* mem;
+  int nthr;
+  __device__ __forceinline__ void set(int k, const float (&v)[EPT]) {
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) {
+      if constexpr (SHARED) mem[(k * EPT + i) * nthr] = v[i];
+      else r[k][i] = v[i];
+    }
+  }
+  __device__ __forceinline__ float at(int k, int i) const {
+    if constexpr (SHARED) return mem[(k * EPT + i) * nthr];
+    else return r[k][i];
+  }
+  static __host__ __device__ constexpr int bytes(int threads) { return SHARED ? 3 * EPT * 4 * threads : 0; }
+};
+
+template <typename T, int VB, int NV, int GATE>
+__global__ void __launch_bounds__(kRowThreads) sandwich_fwd_kernel(const __grid_constant__ NormArgs p) {
+  using M = Mine<T, VB, NV>;
+  constexpr int EPT = M::EPT, ST = M::STAGES;
+  extern __shared__ __align__(16) char ring[];
+  __shared__ float4 red[2][kRowThreads / 128];
+  const M me(p.H);
+  const int64_t r0 = p.rows * blockIdx.x / gridDim.x, r1 = p.rows * (blockIdx.x + 1) / gridDim.x;
+  auto ahead = [&](int64_t row) {
+    if (row < r1) {
+      const int st = (int)((row - r0) % ST);
+      me.ahead(ring, st, 0, 2, p.x, row, p.H);
+      me.ahead(ring, st, 1, 2, p.res, row, p.H);
+    }
+    copies_commit();
+  };
+  for (int i = 0; i < ST; ++i) ahead(r0 + i);
+  if (threadIdx.x < 2 * kRowThreads / 128) (&red[0][0])[threadIdx.x] = make_float4(0.f, 0.f, 0.f, 0.f);
+  Columns<EPT> w;
+  w.mem = reinterpret_cast<float*>(ring + ST * 2 * NV * VB * me.nthr) + me.tid;
+  w.nthr = me.nthr;
+  auto fetch = [&](int k, const void* base, int64_t at, int is_bf16) {
+    float v[EPT];
+    me.fetch(base, at, is_bf16, v);
+    w.set(k, v);
+  };
+  fetch(W_POST, p.w_post, 0, p.w_bf16);
+  fetch(W_PRE, p.w_pre, 0, p.w_bf16);
+  int64_t gate_end = r0;  // first row that needs another gate row
+  __syncthreads();
+  const float inv_h = 1.0f / (float)p.H;
+  for (int64_t row = r0; row < r1; ++row) {
+    if (GATE == GATE_SPAN && row == gate_end) {
+      const int64_t i = row / p.span;
+      fetch(W_GATE, p.gate, i * p.H, p.gate_bf16);
+      gate_end = (i + 1) * p.span;
+    }
+    if (GATE == GATE_ROW) fetch(W_GATE, p.gate, row * p.H, p.gate_bf16);
+    copies_wait<ST - 1>();
+    float x[EPT], s[EPT];
+    const int st = (int)((row - r0) % ST);
+    me.take(ring, st, 0, 2, x);
+    me.take(ring, st, 1, 2, s);
+    ahead(row + ST);
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) ss = fmaf(x[i], x[i], ss);
+    const float rx = 1.0f / sqrtf(row_sum(ss, red[0]) * inv_h + p.eps);
+    ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) {
+      const float pn = x[i] * rx * w.at(W_POST, i);
+      s[i] = fmaf(p.scale, s[i], GATE == GATE_NONE ? pn : w.at(W_GATE, i) * pn);
+      ss = fmaf(s[i], s[i], ss);
+    }
+    me.put(p.s, row, p.H, s);
+    const float rs = 1.0f / sqrtf(row_sum(ss, red[1]) * inv_h + p.eps);
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) s[i] = s[i] * rs * w.at(W_PRE, i);
+    me.put(p.h, row, p.H, s);
+    if (threadIdx.x == 0 && p.rx != nullptr) {
+      p.rx[row] = rx;
+      p.rs[row] = rs;
+    }
+  }
+}
+
+template <typename T, int VB, int NV, int GATE>
+__global__ void __launch_bounds__(kRowThreads) sandwich_bwd_kernel(const __grid_constant__ NormArgs p) {
+  using M = Mine<T, VB, NV>;
+  constexpr int EPT = M::EPT, ST = M::STAGES;
+  extern __shared__ __align__(16) char ring[];
+  __shared__ float4 red[2][kRowThreads / 128];
+  const M me(p.H);
+  // consecutive units (row ranges inside one span): their rows are consecutive too
+  const int64_t u0 = p.units * blockIdx.x / gridDim.x, u1 = p.units * (blockIdx.x + 1) / gridDim.x;
+  auto first_row = [&](int64_t u) {
+    const int64_t i = u / p.units_per_span, k = u - i * p.units_per_span;
+    return i * p.span + p.span * k / p.units_per_span;
+  };
+  const int64_t r0 = first_row(u0), r1 = first_row(u1);
+  auto ahead = [&](int64_t row) {
+    if (row < r1) {
+      const int st = (int)((row - r0) % ST);
+      me.ahead(ring, st, 0, 4, p.x, row, p.H);
+      me.ahead(ring, st, 1, 4, p.res, row, p.H);
+      if (p.dh != nullptr) me.ahead(ring, st, 2, 4, p.dh, row, p.H);
+      if (p.ds != nullptr) me.ahead(ring, st, 3, 4, p.ds, row, p.H);
+    }
+    copies_commit();
+  };
+  for (int i = 0; i < ST; ++i) ahead(r0 + i);
+  if (threadIdx.x < 2 * kRowThreads / 128) (&red[0][0])[threadIdx.x] = make_float4(0.f, 0.f, 0.f, 0.f);
+  Columns<EPT> w;
+  w.mem = reinterpret_cast<float*>(ring + ST * 4 * NV * VB * me.nthr) + me.tid;
+  w.nthr = me.nthr;
+  auto fetch = [&](int k, const void* base, int64_t at, int is_bf16) {
+    float v[EPT];
+    me.fetch(base, at, is_bf16, v);
+    w.set(k, v);
+  };
+  fetch(W_POST, p.w_post, 0, p.w_bf16);
+  fetch(W_PRE, p.w_pre, 0, p.w_bf16);
+  float A[EPT], Bp[EPT];
+#pragma unroll
+  for (int i = 0; i < EPT; ++i) A[i] = Bp[i] = 0.f;
+  int64_t u = u0, unit_end = first_row(u0 + 1);
+  if (GATE == GATE_SPAN) fetch(W_GATE, p.gate, u / p.units_per_span * p.H, p.gate_bf16);
+  __syncthreads();
+  const float inv_h = 1.0f / (float)p.H;
+  float rx = p.rx[r0], rs = p.rs[r0];
+  for (int64_t row = r0; row < r1; ++row) {
+    if (GATE == GATE_ROW) fetch(W_GATE, p.gate, row * p.H, p.gate_bf16);
+    const int64_t next = row + 1 < r1 ? row + 1 : row;
+    const float rx_next = p.rx[next], rs_next = p.rs[next];
+    copies_wait<ST - 1>();
+    float x[EPT], S[EPT];
+    const int st = (int)((row - r0) % ST);
+    me.take(ring, st, 0, 4, x);
+    me.take(ring, st, 1, 4, S);
+    float c = 0.f;
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) {  // s
+      const float pn = x[i] * rx * w.at(W_POST, i);
+      S[i] = fmaf(p.scale, S[i], GATE == GATE_NONE ? pn : w.at(W_GATE, i) * pn);
+    }
+    if (p.dh != nullptr) {
+      float dh[EPT];
+      me.take(ring, st, 2, 4, dh);
+#pragma unroll
+      for (int i = 0; i < EPT; ++i) {
+        c = fmaf(dh[i] * w.at(W_PRE, i), S[i], c);
+        Bp[i] = fmaf(dh[i], S[i] * rs, Bp[i]);
+      }
+      const float k = row_sum(c, red[0]) * inv_h * rs * rs * rs;
+      // read again rather than held: with 16 columns a thread the registers would spill
+      if (EPT >= 16) me.take(ring, st, 2, 4, dh);
+#pragma unroll
+      for (int i = 0; i < EPT; ++i) S[i] = rs * (dh[i] * w.at(W_PRE, i)) - S[i] * k;
+    } else {
+#pragma unroll
+      for (int i = 0; i < EPT; ++i) S[i] = 0.f;
+      __syncthreads();  // the sums of two rows use red[1]
+    }
+    if (p.ds != nullptr) {
+      float ds[EPT];
+      me.take(ring, st, 3, 4, ds);
+#pragma unroll
+      for (int i = 0; i < EPT; ++i) S[i] += ds[i];
+    }
+    ahead(row + ST);
+    c = 0.f;
+    float out[EPT];
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) {
+      const float a = S[i] * (x[i] * rx);
+      if (GATE == GATE_ROW) {
+        A[i] = fmaf(w.at(W_GATE, i), a, A[i]);
+        out[i] = w.at(W_POST, i) * a;
+      } else {
+        A[i] += a;
+      }
+      const float v = GATE == GATE_NONE ? S[i] * w.at(W_POST, i) : S[i] * w.at(W_GATE, i) * w.at(W_POST, i);
+      c = fmaf(v, x[i], c);
+    }
+    if (GATE == GATE_ROW) me.put_as(p.dgate, row * p.H, p.gate_bf16, out);
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) out[i] = p.scale * S[i];
+    me.put(p.dres, row, p.H, out);
+    const float k = row_sum(c, red[1]) * inv_h * rx * rx * rx;
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) {
+      const float v = GATE == GATE_NONE ? S[i] * w.at(W_POST, i) : S[i] * w.at(W_GATE, i) * w.at(W_POST, i);
+      out[i] = fmaf(rx, v, -x[i] * k);
+    }
+    me.put(p.dx, row, p.H, out);
+    rx = rx_next, rs = rs_next;
+    if (row + 1 == unit_end) {
+      me.put_as(p.part_a, u * p.H, 0, A);
+      if (++u < u1) {
+        unit_end = first_row(u + 1);
+        if (GATE == GATE_SPAN) fetch(W_GATE, p.gate, u / p.units_per_span * p.H, p.gate_bf16);
+#pragma unroll
+        for (int i = 0; i < EPT; ++i) A[i] = 0.f;
+      }
+    }
+  }
+  me.put_as(p.part_b, (int64_t)blockIdx.x * p.H, 0, Bp);
+}
+
+// ------------------------------------------------- rows too long for that
+
 template <typename T>
-__global__ void __launch_bounds__(kMaxThreads) sandwich_fwd_kernel(NormArgs p, int gate) {
+__global__ void __launch_bounds__(kMaxThreads) sandwich_fwd_long_kernel(NormArgs p, int gate) {
   __shared__ float red[2][32];
   const T* xp = static_cast<const T*>(p.x);
   const T* rp = static_cast<const T*>(p.res);
@@ -96,7 +447,7 @@ __global__ void __launch_bounds__(kMaxThreads) sandwich_fwd_kernel(NormArgs p, i
 
 // Each block takes whole units (row ranges inside one span) and keeps its sums in its rows of the partial arrays.
 template <typename T>
-__global__ void __launch_bounds__(kMaxThreads) sandwich_bwd_kernel(NormArgs p, int gate) {
+__global__ void __launch_bounds__(kMaxThreads) sandwich_bwd_long_kernel(NormArgs p, int gate) {
   __shared__ float red[2][32];
   const T* xp = static_cast<const T*>(p.x);
   const T* rp = static_cast<const T*>(p.res);
@@ -209,12 +560,14 @@ struct BwdPlan {
   int units_per_span;
 };
 
-// Row ranges of the backward: about two blocks per SM, none across a span.
-BwdPlan bwd_plan(int64_t rows, int64_t span, int gate) {
+// Row ranges of the backward, none across a span.  A block of 4096 columns fills an SM; the partial rows of smaller
+// ones cost as much less.
+BwdPlan bwd_plan(int64_t rows, int64_t span, int64_t H, int gate) {
   BwdPlan b;
+  const int64_t blocks_per_sm = H >= 4096 ? 1 : H <= 256 ? 16 : 4096 / H;
   if (gate != GATE_SPAN) span = rows;
   b.spans = rows / span;
-  const int64_t want = (int64_t)num_sms() * 2;
+  const int64_t want = (int64_t)num_sms() * blocks_per_sm;
   int64_t per = b.spans >= want ? 1 : want / b.spans;
   if (per > span) per = span;
   b.units_per_span = (int)per;
@@ -246,6 +599,86 @@ int threads_for(int64_t H) {
   return t;
 }
 
+// Calls go(integral constants VB, NV) with the widest vectors that the width and every pointer allow, and as few of
+// them per thread as give at most kRowThreads threads; false where a row has too many for 16 elements a thread.
+template <typename T, typename F>
+bool pick_vectors(int64_t H, uintptr_t addr, F go) {
+  const int64_t es = sizeof(T);
+  if (addr % (uintptr_t)es != 0) return false;
+  int vb = 16;
+  while (vb > (int)es && (H * es % vb != 0 || addr % (uintptr_t)vb != 0)) vb >>= 1;
+  const int64_t per = (H * es / vb + kRowThreads - 1) / kRowThreads;  // vectors a thread needs
+#define ATS_PICK(VB_, NV_)                                                                   \
+  if (vb == VB_ && per <= NV_) {                                                              \
+    go(std::integral_constant<int, VB_>{}, std::integral_constant<int, NV_>{});               \
+    return true;                                                                             \
+  }
+  if constexpr (sizeof(T) == 2) {
+    ATS_PICK(16, 1) ATS_PICK(16, 2) ATS_PICK(8, 1) ATS_PICK(8, 2) ATS_PICK(8, 4) ATS_PICK(4, 2) ATS_PICK(4, 8)
+    ATS_PICK(2, 4) ATS_PICK(2, 16)
+  } else {
+    ATS_PICK(16, 1) ATS_PICK(16, 2) ATS_PICK(16, 4) ATS_PICK(8, 2) ATS_PICK(8, 8) ATS_PICK(4, 4) ATS_PICK(4, 16)
+  }
+#undef ATS_PICK
+  return false;
+}
+
+uintptr_t bits(const void* p) { return reinterpret_cast<uintptr_t>(p); }
+
+// Low bits of the rows' addresses.  The weights, the gate and its gradient are read and written in pieces of up to 16
+// bytes whatever the rows' vectors are: 1 (no vectors at all) where one of them is not aligned to that.
+uintptr_t row_bits(const NormArgs& p) {
+  const uintptr_t other = bits(p.w_post) | bits(p.w_pre) | bits(p.gate) | bits(p.dgate);
+  return bits(p.x) | bits(p.res) | (other % 16 != 0 ? 1 : 0);
+}
+
+template <typename F>
+int launch_rows(F kernel, const NormArgs& p, int64_t blocks, int threads, int smem, cudaStream_t st, const char* what) {
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return fail(ATS_ECUDA, "%s: %s", what, cudaGetErrorString(e));
+  kernel<<<(unsigned)blocks, threads, smem, st>>>(p);
+  return check_launch(what);
+}
+
+template <typename T>
+int fwd_t(const NormArgs& p, int gate, cudaStream_t st) {
+  int rc = ATS_OK;
+  const bool ok = pick_vectors<T>(p.H, row_bits(p) | bits(p.s) | bits(p.h), [&](auto vb, auto nv) {
+    using M = Mine<T, vb.value, nv.value>;
+    const int threads = (p.H / M::VEC + nv.value - 1) / nv.value;
+    const int t = (threads + 31) / 32 * 32;
+    const int smem = M::STAGES * 2 * nv.value * vb.value * t + Columns<M::EPT>::bytes(t);
+    // enough blocks to fill the SMs, each with a run of rows
+    const int64_t cap = (int64_t)num_sms() * (t >= 512 ? 2 : t >= 32 * 3 ? 1024 / t : 16);
+    const int64_t blocks = p.rows < cap ? p.rows : cap;
+    rc = gate == GATE_NONE   ? launch_rows(sandwich_fwd_kernel<T, vb.value, nv.value, GATE_NONE>, p, blocks, t, smem, st, "sandwich_norm_fwd")
+         : gate == GATE_SPAN ? launch_rows(sandwich_fwd_kernel<T, vb.value, nv.value, GATE_SPAN>, p, blocks, t, smem, st, "sandwich_norm_fwd")
+                             : launch_rows(sandwich_fwd_kernel<T, vb.value, nv.value, GATE_ROW>, p, blocks, t, smem, st, "sandwich_norm_fwd");
+  });
+  if (ok) return rc;
+  const int64_t cap = (int64_t)num_sms() * 16;
+  sandwich_fwd_long_kernel<T><<<(unsigned)(p.rows < cap ? p.rows : cap), threads_for(p.H), 0, st>>>(p, gate);
+  return check_launch("sandwich_norm_fwd");
+}
+
+template <typename T>
+int bwd_t(const NormArgs& p, int gate, int64_t blocks, cudaStream_t st) {
+  int rc = ATS_OK;
+  const uintptr_t addr = row_bits(p) | bits(p.dh) | bits(p.ds) | bits(p.dx) | bits(p.dres);
+  const bool ok = pick_vectors<T>(p.H, addr, [&](auto vb, auto nv) {
+    using M = Mine<T, vb.value, nv.value>;
+    const int threads = (p.H / M::VEC + nv.value - 1) / nv.value;
+    const int t = (threads + 31) / 32 * 32;
+    const int smem = M::STAGES * 4 * nv.value * vb.value * t + Columns<M::EPT>::bytes(t);
+    rc = gate == GATE_NONE   ? launch_rows(sandwich_bwd_kernel<T, vb.value, nv.value, GATE_NONE>, p, blocks, t, smem, st, "sandwich_norm_bwd")
+         : gate == GATE_SPAN ? launch_rows(sandwich_bwd_kernel<T, vb.value, nv.value, GATE_SPAN>, p, blocks, t, smem, st, "sandwich_norm_bwd")
+                             : launch_rows(sandwich_bwd_kernel<T, vb.value, nv.value, GATE_ROW>, p, blocks, t, smem, st, "sandwich_norm_bwd");
+  });
+  if (ok) return rc;
+  sandwich_bwd_long_kernel<T><<<(unsigned)blocks, threads_for(p.H), 0, st>>>(p, gate);
+  return check_launch("sandwich_norm_bwd");
+}
+
 }  // namespace
 }  // namespace ats
 
@@ -268,17 +701,14 @@ int ats_sandwich_norm_fwd(const void* x, const void* residual, ats_dtype dtype, 
   p.rx = rstd_x, p.rs = rstd_sum;
   p.rows = rows, p.span = rows_per_gate, p.H = (int)hidden, p.scale = residual_scale, p.eps = eps;
   const int g = gate_kind(gate, rows_per_gate);
-  const int64_t cap = (int64_t)num_sms() * 16;
-  const unsigned grid = (unsigned)(rows < cap ? rows : cap);
   cudaStream_t st = (cudaStream_t)stream;
-  if (dtype == ATS_BF16) sandwich_fwd_kernel<bf16><<<grid, threads_for(hidden), 0, st>>>(p, g);
-  else sandwich_fwd_kernel<float><<<grid, threads_for(hidden), 0, st>>>(p, g);
-  return check_launch("sandwich_norm_fwd");
+  return dtype == ATS_BF16 ? fwd_t<bf16>(p, g, st) : fwd_t<float>(p, g, st);
 }
 
 size_t ats_sandwich_norm_bwd_workspace_bytes(int64_t rows, int64_t hidden, int64_t rows_per_gate) {
   if (rows <= 0 || hidden <= 0 || rows_per_gate < 0 || (rows_per_gate > 0 && rows % rows_per_gate != 0)) return 0;
-  const BwdPlan b = bwd_plan(rows, rows_per_gate > 1 ? rows_per_gate : rows, rows_per_gate > 1 ? GATE_SPAN : GATE_NONE);
+  const BwdPlan b = bwd_plan(rows, rows_per_gate > 1 ? rows_per_gate : rows, hidden,
+                             rows_per_gate > 1 ? GATE_SPAN : GATE_NONE);
   return (size_t)(b.units + b.blocks + (rows_per_gate > 1 ? b.spans : 0)) * (size_t)hidden * sizeof(float);
 }
 
@@ -294,10 +724,10 @@ int ats_sandwich_norm_bwd(const void* dh, const void* dsum, const void* x, const
       dw_pre == nullptr || (gate != nullptr && dgate == nullptr))
     return fail(ATS_EBADARG, "sandwich_norm_bwd: null pointer");
   const int g = gate_kind(gate, rows_per_gate);
-  if (workspace == nullptr ||
+  if (workspace == nullptr || !aligned16(workspace) ||
       workspace_bytes < ats_sandwich_norm_bwd_workspace_bytes(rows, hidden, gate != nullptr ? rows_per_gate : 0))
     return fail(ATS_EBADARG, "sandwich_norm_bwd: workspace too small");
-  const BwdPlan b = bwd_plan(rows, rows_per_gate, g);
+  const BwdPlan b = bwd_plan(rows, rows_per_gate, hidden, g);
   NormArgs p{};
   p.x = x, p.res = residual, p.dh = dh, p.ds = dsum, p.dx = dx, p.dres = dresidual;
   p.w_post = w_post, p.w_pre = w_pre, p.gate = gate, p.dgate = dgate;
@@ -310,9 +740,7 @@ int ats_sandwich_norm_bwd(const void* dh, const void* dsum, const void* x, const
   p.part_b = p.part_a + b.units * hidden;
   float* gate_a = p.part_b + b.blocks * hidden;
   cudaStream_t st = (cudaStream_t)stream;
-  if (dtype == ATS_BF16) sandwich_bwd_kernel<bf16><<<(unsigned)b.blocks, threads_for(hidden), 0, st>>>(p, g);
-  else sandwich_bwd_kernel<float><<<(unsigned)b.blocks, threads_for(hidden), 0, st>>>(p, g);
-  ATS_TRY(check_launch("sandwich_norm_bwd"));
+  ATS_TRY(dtype == ATS_BF16 ? bwd_t<bf16>(p, g, b.blocks, st) : bwd_t<float>(p, g, b.blocks, st));
   const unsigned cols = (unsigned)((hidden + kReduceCols - 1) / kReduceCols);
   const float* a = p.part_a;
   int64_t na = b.units;
