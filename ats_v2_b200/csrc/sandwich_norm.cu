@@ -64,27 +64,35 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
 }
 
 // ------------------------------------------------------------ rows in registers
-// One block walks a run of consecutive rows; a thread owns NV vectors of VB bytes of every row, so its weights, gate
-// (per span) and sums over rows stay in its registers.  Each thread copies its own pieces of the rows ahead into its
-// own slots of shared memory (cp.async), STAGES rows deep: no thread reads another's, so the only barriers are the two
-// row sums.  Measured at 16384 x 4096 bf16 against the loads issued straight into registers: see the entry points.
+// One block walks a run of consecutive rows; a thread owns NV vectors of VB bytes of every row, so its sums over rows
+// stay in its registers, and its columns of the weights (and of the gate, per span) in its own places of shared
+// memory.  Each thread copies its own pieces of the rows ahead into its own slots of shared memory (cp.async), STAGES
+// rows deep: no thread reads another's, so the only barriers are the two row sums.  Two blocks share an SM where their
+// registers allow it, so that one's barrier waits pass under the other's arithmetic.
+//
+// Per column, with xr = x rx, t = s rs, and gw = gate w_post:
+//   s = a res + gw xr;  u = dh w_pre;  S = ds + rs u - t rs m(u t);  dx = rx (gw S - xr m(gw S xr))
 template <int BYTES> struct Raw;
 template <> struct Raw<16> { using type = uint4; };
 template <> struct Raw<8> { using type = uint2; };
 template <> struct Raw<4> { using type = uint32_t; };
 template <> struct Raw<2> { using type = uint16_t; };
 
+// Copy BYTES, or zeros where `there` is false, without a branch (one for every vector would serialise a row).
 template <int BYTES>
-__device__ __forceinline__ void copy_ahead(void* dst, const void* src) {
+__device__ __forceinline__ void copy_ahead(void* dst, const void* src, bool there) {
   if constexpr (BYTES == 2) {  // cp.async moves 4, 8 or 16 bytes
-    *static_cast<uint16_t*>(dst) = *static_cast<const uint16_t*>(src);
+    const uint16_t v = *static_cast<const uint16_t*>(src);
+    *static_cast<uint16_t*>(dst) = there ? v : (uint16_t)0;
   } else if constexpr (BYTES == 32) {
-    copy_ahead<16>(dst, src);
-    copy_ahead<16>(static_cast<char*>(dst) + 16, static_cast<const char*>(src) + 16);
+    copy_ahead<16>(dst, src, there);
+    copy_ahead<16>(static_cast<char*>(dst) + 16, static_cast<const char*>(src) + 16, there);
   } else {
-    const uint32_t d = static_cast<uint32_t>(__cvta_generic_to_shared(dst));
-    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(src) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(d), "l"(src), "n"(BYTES) : "memory");
+    const uint32_t d = static_cast<uint32_t>(__cvta_generic_to_shared(dst)), n = there ? BYTES : 0;
+    if constexpr (BYTES == 16)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(src), "r"(n) : "memory");
+    else
+      asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(d), "l"(src), "n"(BYTES), "r"(n) : "memory");
   }
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -92,51 +100,100 @@ template <int N>
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 constexpr int kRowThreads = 512;  // most threads of a row block
-__host__ __device__ constexpr int stages_of(int bytes) { return bytes >= 64 ? 1 : bytes >= 32 ? 2 : bytes >= 16 ? 4 : 8; }
 
-// One thread's view of its vectors: column of vector j, and whether the row has it.
-template <typename T, int VB, int NV>
+// One thread's part of the rows.
+template <typename T, int VB, int NV, int GATE>
 struct Mine {
-  static constexpr int VEC = VB / (int)sizeof(T), EPT = NV * VEC, STAGES = stages_of(NV * VB);
+  static constexpr int VEC = VB / (int)sizeof(T), EPT = NV * VEC;
+  static_assert(EPT % 4 == 0, "whole float4s of columns");
+  static constexpr int ROW = NV * VB;  // bytes of a row of T
+  // a gate row streams beside the others, in room for float32, where a thread has few enough columns
+  static constexpr bool STREAM_GATE = GATE == 2 && EPT <= 8;
+  static constexpr int BLOCKS = ROW <= 16 && GATE != 2 ? 2 : 1;  // on an SM
+  static constexpr int COLS = GATE == 2 && !STREAM_GATE ? 3 : 2;  // sets of columns kept
   using R = typename Raw<VB>::type;
   int nthr, tid, nvec;
-  __device__ __forceinline__ Mine(int H) : nthr((int)blockDim.x), tid((int)threadIdx.x), nvec(H / VEC) {}
+  char* ring;
+  float4* cols;
+  int stage_bytes;
+  __device__ __forceinline__ Mine(int H, char* smem, int tensors, int stages)
+      : nthr((int)blockDim.x), tid((int)threadIdx.x), nvec(H / VEC), ring(smem) {
+    stage_bytes = nthr * (tensors * ROW + (STREAM_GATE ? EPT * 4 : 0));
+    cols = reinterpret_cast<float4*>(smem + stages * stage_bytes) + tid;
+  }
+  static __host__ constexpr int smem(int threads, int tensors, int stages) {
+    return threads * (stages * (tensors * ROW + (STREAM_GATE ? EPT * 4 : 0)) + COLS * EPT * 4);
+  }
   __device__ __forceinline__ bool has(int j) const { return tid + j * nthr < nvec; }
   __device__ __forceinline__ int col(int j) const { return (tid + j * nthr) * VEC; }
-  // slot of vector j of tensor t in stage st, of NT tensors
-  __device__ __forceinline__ char* slot(char* ring, int st, int t, int nt, int j) const {
-    return ring + ((size_t)((st * nt + t) * NV + j) * nthr + tid) * VB;
+  // a column that exists, for addresses
+  __device__ __forceinline__ int safe(int j) const { return has(j) ? col(j) : 0; }
+  __device__ __forceinline__ char* slot(int st, int t, int j) const {
+    return ring + st * stage_bytes + ((t * NV + j) * nthr + tid) * VB;
   }
-  __device__ __forceinline__ void ahead(char* ring, int st, int t, int nt, const void* base, int64_t row, int H) const {
+  __device__ __forceinline__ void ahead(int st, int t, const void* base, int64_t at) const {
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
-      if (has(j)) copy_ahead<VB>(slot(ring, st, t, nt, j), static_cast<const T*>(base) + row * H + col(j));
+    for (int j = 0; j < NV; ++j) copy_ahead<VB>(slot(st, t, j), static_cast<const T*>(base) + at + safe(j), has(j));
   }
-  __device__ __forceinline__ void take(char* ring, int st, int t, int nt, float (&v)[EPT]) const {
+  __device__ __forceinline__ void take(int st, int t, float (&v)[EPT]) const {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      R raw{};
-      if (has(j)) raw = *reinterpret_cast<const R*>(slot(ring, st, t, nt, j));
+      const R raw = *reinterpret_cast<const R*>(slot(st, t, j));
       const T* e = reinterpret_cast<const T*>(&raw);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) v[j * VEC + i] = Cvt<T>::to_f(e[i]);
     }
   }
-  // EPT values of a row of `p` (bf16 or float32, 16-byte aligned) from its first element `at`; 0 where the row has no
-  // such column
+  // the streamed gate: behind the `tensors` row tensors of a stage
+  __device__ __forceinline__ char* gate_slot(int st, int tensors, int j) const {
+    return ring + st * stage_bytes + tensors * ROW * nthr + (j * nthr + tid) * VEC * 4;
+  }
+  __device__ __forceinline__ void gate_ahead(int st, int tensors, const void* base, int64_t at, int is_bf16) const {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      if (is_bf16) copy_ahead<VEC * 2>(gate_slot(st, tensors, j), static_cast<const bf16*>(base) + at + safe(j), has(j));
+      else copy_ahead<VEC * 4>(gate_slot(st, tensors, j), static_cast<const float*>(base) + at + safe(j), has(j));
+    }
+  }
+  __device__ __forceinline__ void gate_take(int st, int tensors, int is_bf16, float (&v)[EPT]) const {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      float t[VEC];
+      if (is_bf16) load_vec<bf16>(reinterpret_cast<const bf16*>(gate_slot(st, tensors, j)), t);
+      else load_vec<float>(reinterpret_cast<const float*>(gate_slot(st, tensors, j)), t);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[j * VEC + i] = t[i];
+    }
+  }
+  // EPT values of a row of `p` (bf16 or float32, 16-byte aligned) from element `at`; 0 where the row has no column
   __device__ __forceinline__ void fetch(const void* p, int64_t at, int is_bf16, float (&v)[EPT]) const {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       float t[VEC];
+      if (is_bf16) load_vec<bf16>(static_cast<const bf16*>(p) + at + safe(j), t);
+      else load_vec<float>(static_cast<const float*>(p) + at + safe(j), t);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) t[i] = 0.f;
-      if (has(j)) {
-        if (is_bf16) load_vec<bf16>(static_cast<const bf16*>(p) + at + col(j), t);
-        else load_vec<float>(static_cast<const float*>(p) + at + col(j), t);
-      }
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) v[j * VEC + i] = t[i];
+      for (int i = 0; i < VEC; ++i) v[j * VEC + i] = has(j) ? t[i] : 0.f;
     }
+  }
+  __device__ __forceinline__ void put(void* base, int64_t at, const float (&v)[EPT]) const {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      R raw;
+      T* e = reinterpret_cast<T*>(&raw);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) e[i] = Cvt<T>::from_f(v[j * VEC + i]);
+      if (has(j)) *reinterpret_cast<R*>(static_cast<T*>(base) + at + col(j)) = raw;
+    }
+  }
+  // the same into a bf16 or float32 row that is 16-byte aligned
+  __device__ __forceinline__ void put_as(void* base, int64_t at, int is_bf16, const float (&v)[EPT]) const {
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+      if (has(j)) {
+        if (is_bf16) store_vec<bf16>(static_cast<bf16*>(base) + at + col(j), v + j * VEC);
+        else store_vec<float>(static_cast<float*>(base) + at + col(j), v + j * VEC);
+      }
   }
   template <typename U>
   __device__ __forceinline__ static void load_vec(const U* p, float (&t)[VEC]) {
@@ -148,25 +205,6 @@ struct Mine {
 #pragma unroll
       for (int i = 0; i < N; ++i) t[q * N + i] = Cvt<U>::to_f(e[i]);
     }
-  }
-  __device__ __forceinline__ void put(void* base, int64_t row, int H, const float (&v)[EPT]) const {
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      R raw;
-      T* e = reinterpret_cast<T*>(&raw);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) e[i] = Cvt<T>::from_f(v[j * VEC + i]);
-      if (has(j)) *reinterpret_cast<R*>(static_cast<T*>(base) + row * H + col(j)) = raw;
-    }
-  }
-  // the same into a bf16 or float32 row that is 16-byte aligned
-  __device__ __forceinline__ void put_as(void* base, int64_t at, int is_bf16, const float (&v)[EPT]) const {
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-      if (has(j)) {
-        if (is_bf16) store_vec<bf16>(static_cast<bf16*>(base) + at + col(j), v + j * VEC);
-        else store_vec<float>(static_cast<float*>(base) + at + col(j), v + j * VEC);
-      }
   }
   template <typename U>
   __device__ __forceinline__ static void store_vec(U* p, const float* v) {
@@ -180,7 +218,30 @@ struct Mine {
       reinterpret_cast<typename Raw<PIECE>::type*>(p)[q] = raw;
     }
   }
+  // set k of this thread's columns, four at a time
+  __device__ __forceinline__ void keep(int k, const float (&v)[EPT]) const {
+#pragma unroll
+    for (int q = 0; q < EPT / 4; ++q)
+      cols[(k * (EPT / 4) + q) * nthr] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+  }
+  __device__ __forceinline__ void kept(int k, float (&v)[EPT]) const {
+#pragma unroll
+    for (int q = 0; q < EPT / 4; ++q) {
+      const float4 t = cols[(k * (EPT / 4) + q) * nthr];
+      v[4 * q] = t.x, v[4 * q + 1] = t.y, v[4 * q + 2] = t.z, v[4 * q + 3] = t.w;
+    }
+  }
 };
+
+// Rows in flight: as many as half the SM (a whole one for a block alone) holds beside the columns, at most 8.
+template <typename M>
+__host__ __device__ constexpr int stages_of(int tensors) {
+  const int room = (M::BLOCKS == 2 ? 108 : 216) * 1024 / kRowThreads - M::COLS * M::EPT * 4;
+  const int n = room / (tensors * M::ROW + (M::STREAM_GATE ? M::EPT * 4 : 0));
+  return n >= 8 ? 8 : n >= 4 ? 4 : n >= 2 ? 2 : 1;
+}
+
+enum { COL_GATE_POST = 0, COL_PRE = 1, COL_GATE = 2 };
 
 // Sum over the block by up to 16 warps.
 __device__ __forceinline__ float row_sum(float v, float4* red) {
@@ -197,89 +258,85 @@ __device__ __forceinline__ float row_sum(float v, float4* red) {
   return t;
 }
 
-// A thread's columns of the two weights and the gate: in registers, or, from 16 columns a thread on, in its own places
-// of shared memory (with 16 the backward's registers would spill).
-enum { W_POST = 0, W_PRE = 1, W_GATE = 2 };
-template <int EPT>
-struct Columns {
-  static constexpr bool SHARED = EPT >= 16;
-  float r[SHARED ? 1 : 3][SHARED ? 1 : EPT];
-  float* mem;
-  int nthr;
-  __device__ __forceinline__ void set(int k, const float (&v)[EPT]) {
+// gate (where there is one per span) times w_post into set COL_GATE_POST.
+template <typename M>
+__device__ __forceinline__ void keep_gate_post(const M& me, const NormArgs& p, bool gated, int64_t gate_row) {
+  float w[M::EPT];
+  me.fetch(p.w_post, 0, p.w_bf16, w);
+  if (gated) {
+    float g[M::EPT];
+    me.fetch(p.gate, gate_row * p.H, p.gate_bf16, g);
 #pragma unroll
-    for (int i = 0; i < EPT; ++i) {
-      if constexpr (SHARED) mem[(k * EPT + i) * nthr] = v[i];
-      else r[k][i] = v[i];
-    }
+    for (int i = 0; i < M::EPT; ++i) w[i] *= g[i];
   }
-  __device__ __forceinline__ float at(int k, int i) const {
-    if constexpr (SHARED) return mem[(k * EPT + i) * nthr];
-    else return r[k][i];
-  }
-  static __host__ __device__ constexpr int bytes(int threads) { return SHARED ? 3 * EPT * 4 * threads : 0; }
-};
+  me.keep(COL_GATE_POST, w);
+}
 
 template <typename T, int VB, int NV, int GATE>
-__global__ void __launch_bounds__(kRowThreads) sandwich_fwd_kernel(const __grid_constant__ NormArgs p) {
-  using M = Mine<T, VB, NV>;
-  constexpr int EPT = M::EPT, ST = M::STAGES;
-  extern __shared__ __align__(16) char ring[];
+__global__ void __launch_bounds__(kRowThreads, Mine<T, VB, NV, GATE>::BLOCKS)
+    sandwich_fwd_kernel(const __grid_constant__ NormArgs p) {
+  using M = Mine<T, VB, NV, GATE>;
+  constexpr int EPT = M::EPT, ST = stages_of<M>(2);
+  extern __shared__ __align__(16) char smem[];
   __shared__ float4 red[2][kRowThreads / 128];
-  const M me(p.H);
+  const M me(p.H, smem, 2, ST);
   const int64_t r0 = p.rows * blockIdx.x / gridDim.x, r1 = p.rows * (blockIdx.x + 1) / gridDim.x;
-  auto ahead = [&](int64_t row) {
+  auto ahead = [&](int64_t row, int st) {
     if (row < r1) {
-      const int st = (int)((row - r0) % ST);
-      me.ahead(ring, st, 0, 2, p.x, row, p.H);
-      me.ahead(ring, st, 1, 2, p.res, row, p.H);
+      me.ahead(st, 0, p.x, row * p.H);
+      me.ahead(st, 1, p.res, row * p.H);
+      if constexpr (M::STREAM_GATE) me.gate_ahead(st, 2, p.gate, row * p.H, p.gate_bf16);
     }
     copies_commit();
   };
-  for (int i = 0; i < ST; ++i) ahead(r0 + i);
+  for (int i = 0; i < ST; ++i) ahead(r0 + i, i);
   if (threadIdx.x < 2 * kRowThreads / 128) (&red[0][0])[threadIdx.x] = make_float4(0.f, 0.f, 0.f, 0.f);
-  Columns<EPT> w;
-  w.mem = reinterpret_cast<float*>(ring + ST * 2 * NV * VB * me.nthr) + me.tid;
-  w.nthr = me.nthr;
-  auto fetch = [&](int k, const void* base, int64_t at, int is_bf16) {
-    float v[EPT];
-    me.fetch(base, at, is_bf16, v);
-    w.set(k, v);
-  };
-  fetch(W_POST, p.w_post, 0, p.w_bf16);
-  fetch(W_PRE, p.w_pre, 0, p.w_bf16);
-  int64_t gate_end = r0;  // first row that needs another gate row
+  {
+    float w[EPT];
+    me.fetch(p.w_pre, 0, p.w_bf16, w);
+    me.keep(COL_PRE, w);
+  }
+  keep_gate_post(me, p, GATE == GATE_SPAN, GATE == GATE_SPAN ? r0 / p.span : 0);
+  int64_t gate_end = GATE == GATE_SPAN ? (r0 / p.span + 1) * p.span : 0;  // first row that needs another gate row
   __syncthreads();
   const float inv_h = 1.0f / (float)p.H;
+  int st = 0;
   for (int64_t row = r0; row < r1; ++row) {
     if (GATE == GATE_SPAN && row == gate_end) {
-      const int64_t i = row / p.span;
-      fetch(W_GATE, p.gate, i * p.H, p.gate_bf16);
-      gate_end = (i + 1) * p.span;
+      keep_gate_post(me, p, true, row / p.span);
+      gate_end += p.span;
     }
-    if (GATE == GATE_ROW) fetch(W_GATE, p.gate, row * p.H, p.gate_bf16);
+    float g[GATE == GATE_ROW ? EPT : 1];
+    if constexpr (GATE == GATE_ROW && !M::STREAM_GATE) me.fetch(p.gate, row * p.H, p.gate_bf16, g);
     copies_wait<ST - 1>();
     float x[EPT], s[EPT];
-    const int st = (int)((row - r0) % ST);
-    me.take(ring, st, 0, 2, x);
-    me.take(ring, st, 1, 2, s);
-    ahead(row + ST);
+    me.take(st, 0, x);
+    me.take(st, 1, s);
+    if constexpr (M::STREAM_GATE) me.gate_take(st, 2, p.gate_bf16, g);
+    ahead(row + ST, st);
+    if (++st == ST) st = 0;
     float ss = 0.f;
 #pragma unroll
     for (int i = 0; i < EPT; ++i) ss = fmaf(x[i], x[i], ss);
     const float rx = 1.0f / sqrtf(row_sum(ss, red[0]) * inv_h + p.eps);
     ss = 0.f;
+    {
+      float w[EPT];
+      me.kept(COL_GATE_POST, w);
 #pragma unroll
-    for (int i = 0; i < EPT; ++i) {
-      const float pn = x[i] * rx * w.at(W_POST, i);
-      s[i] = fmaf(p.scale, s[i], GATE == GATE_NONE ? pn : w.at(W_GATE, i) * pn);
-      ss = fmaf(s[i], s[i], ss);
+      for (int i = 0; i < EPT; ++i) {
+        const float gw = GATE == GATE_ROW ? g[GATE == GATE_ROW ? i : 0] * w[i] : w[i];
+        s[i] = fmaf(gw, x[i] * rx, p.scale * s[i]);
+        ss = fmaf(s[i], s[i], ss);
+      }
     }
-    me.put(p.s, row, p.H, s);
+    me.put(p.s, row * p.H, s);
     const float rs = 1.0f / sqrtf(row_sum(ss, red[1]) * inv_h + p.eps);
+    float w[EPT];
+    me.kept(COL_PRE, w);
 #pragma unroll
-    for (int i = 0; i < EPT; ++i) s[i] = s[i] * rs * w.at(W_PRE, i);
-    me.put(p.h, row, p.H, s);
+    for (int i = 0; i < EPT; ++i) s[i] = s[i] * rs * w[i];
+    me.put(p.h, row * p.H, s);
     if (threadIdx.x == 0 && p.rx != nullptr) {
       p.rx[row] = rx;
       p.rs[row] = rs;
@@ -288,12 +345,13 @@ __global__ void __launch_bounds__(kRowThreads) sandwich_fwd_kernel(const __grid_
 }
 
 template <typename T, int VB, int NV, int GATE>
-__global__ void __launch_bounds__(kRowThreads) sandwich_bwd_kernel(const __grid_constant__ NormArgs p) {
-  using M = Mine<T, VB, NV>;
-  constexpr int EPT = M::EPT, ST = M::STAGES;
-  extern __shared__ __align__(16) char ring[];
+__global__ void __launch_bounds__(kRowThreads, Mine<T, VB, NV, GATE>::BLOCKS)
+    sandwich_bwd_kernel(const __grid_constant__ NormArgs p) {
+  using M = Mine<T, VB, NV, GATE>;
+  constexpr int EPT = M::EPT, ST = stages_of<M>(4);
+  extern __shared__ __align__(16) char smem[];
   __shared__ float4 red[2][kRowThreads / 128];
-  const M me(p.H);
+  const M me(p.H, smem, 4, ST);
   // consecutive units (row ranges inside one span): their rows are consecutive too
   const int64_t u0 = p.units * blockIdx.x / gridDim.x, u1 = p.units * (blockIdx.x + 1) / gridDim.x;
   auto first_row = [&](int64_t u) {
@@ -301,107 +359,125 @@ __global__ void __launch_bounds__(kRowThreads) sandwich_bwd_kernel(const __grid_
     return i * p.span + p.span * k / p.units_per_span;
   };
   const int64_t r0 = first_row(u0), r1 = first_row(u1);
-  auto ahead = [&](int64_t row) {
+  const bool has_dh = p.dh != nullptr, has_ds = p.ds != nullptr;
+  auto ahead = [&](int64_t row, int st) {
     if (row < r1) {
-      const int st = (int)((row - r0) % ST);
-      me.ahead(ring, st, 0, 4, p.x, row, p.H);
-      me.ahead(ring, st, 1, 4, p.res, row, p.H);
-      if (p.dh != nullptr) me.ahead(ring, st, 2, 4, p.dh, row, p.H);
-      if (p.ds != nullptr) me.ahead(ring, st, 3, 4, p.ds, row, p.H);
+      me.ahead(st, 0, p.x, row * p.H);
+      me.ahead(st, 1, p.res, row * p.H);
+      if (has_dh) me.ahead(st, 2, p.dh, row * p.H);
+      if (has_ds) me.ahead(st, 3, p.ds, row * p.H);
+      if constexpr (M::STREAM_GATE) me.gate_ahead(st, 4, p.gate, row * p.H, p.gate_bf16);
     }
     copies_commit();
   };
-  for (int i = 0; i < ST; ++i) ahead(r0 + i);
+  for (int i = 0; i < ST; ++i) ahead(r0 + i, i);
   if (threadIdx.x < 2 * kRowThreads / 128) (&red[0][0])[threadIdx.x] = make_float4(0.f, 0.f, 0.f, 0.f);
-  Columns<EPT> w;
-  w.mem = reinterpret_cast<float*>(ring + ST * 4 * NV * VB * me.nthr) + me.tid;
-  w.nthr = me.nthr;
-  auto fetch = [&](int k, const void* base, int64_t at, int is_bf16) {
-    float v[EPT];
-    me.fetch(base, at, is_bf16, v);
-    w.set(k, v);
-  };
-  fetch(W_POST, p.w_post, 0, p.w_bf16);
-  fetch(W_PRE, p.w_pre, 0, p.w_bf16);
+  {
+    float w[EPT];
+    me.fetch(p.w_pre, 0, p.w_bf16, w);
+    me.keep(COL_PRE, w);
+  }
   float A[EPT], Bp[EPT];
 #pragma unroll
   for (int i = 0; i < EPT; ++i) A[i] = Bp[i] = 0.f;
   int64_t u = u0, unit_end = first_row(u0 + 1);
-  if (GATE == GATE_SPAN) fetch(W_GATE, p.gate, u / p.units_per_span * p.H, p.gate_bf16);
+  keep_gate_post(me, p, GATE == GATE_SPAN, u / p.units_per_span);
   __syncthreads();
   const float inv_h = 1.0f / (float)p.H;
   float rx = p.rx[r0], rs = p.rs[r0];
+  int st = 0;
   for (int64_t row = r0; row < r1; ++row) {
-    if (GATE == GATE_ROW) fetch(W_GATE, p.gate, row * p.H, p.gate_bf16);
+    const int64_t at = row * p.H;
     const int64_t next = row + 1 < r1 ? row + 1 : row;
     const float rx_next = p.rx[next], rs_next = p.rs[next];
-    copies_wait<ST - 1>();
-    float x[EPT], S[EPT];
-    const int st = (int)((row - r0) % ST);
-    me.take(ring, st, 0, 4, x);
-    me.take(ring, st, 1, 4, S);
-    float c = 0.f;
-#pragma unroll
-    for (int i = 0; i < EPT; ++i) {  // s
-      const float pn = x[i] * rx * w.at(W_POST, i);
-      S[i] = fmaf(p.scale, S[i], GATE == GATE_NONE ? pn : w.at(W_GATE, i) * pn);
+    if constexpr (GATE == GATE_ROW && !M::STREAM_GATE) {
+      float g[EPT];
+      me.fetch(p.gate, at, p.gate_bf16, g);
+      me.keep(COL_GATE, g);
     }
-    if (p.dh != nullptr) {
-      float dh[EPT];
-      me.take(ring, st, 2, 4, dh);
+    copies_wait<ST - 1>();
+    // gate w_post of this row: kept, or formed from the streamed gate
+    auto gate_post = [&](float (&w)[EPT]) {
+      me.kept(COL_GATE_POST, w);
+      if constexpr (GATE == GATE_ROW) {
+        float g[EPT];
+        if constexpr (M::STREAM_GATE) me.gate_take(st, 4, p.gate_bf16, g);
+        else me.kept(COL_GATE, g);
+#pragma unroll
+        for (int i = 0; i < EPT; ++i) w[i] *= g[i];
+      }
+    };
+    float xr[EPT], S[EPT];
+    me.take(st, 0, xr);
+    me.take(st, 1, S);
+    {
+      float w[EPT];
+      gate_post(w);
 #pragma unroll
       for (int i = 0; i < EPT; ++i) {
-        c = fmaf(dh[i] * w.at(W_PRE, i), S[i], c);
-        Bp[i] = fmaf(dh[i], S[i] * rs, Bp[i]);
+        xr[i] *= rx;
+        S[i] = fmaf(w[i], xr[i], p.scale * S[i]) * rs;  // t
       }
-      const float k = row_sum(c, red[0]) * inv_h * rs * rs * rs;
-      // read again rather than held: with 16 columns a thread the registers would spill
-      if (EPT >= 16) me.take(ring, st, 2, 4, dh);
+    }
+    float c = 0.f;
+    if (has_dh) {
+      float dh[EPT], w[EPT];
+      me.take(st, 2, dh);
+      me.kept(COL_PRE, w);
 #pragma unroll
-      for (int i = 0; i < EPT; ++i) S[i] = rs * (dh[i] * w.at(W_PRE, i)) - S[i] * k;
+      for (int i = 0; i < EPT; ++i) {
+        Bp[i] = fmaf(dh[i], S[i], Bp[i]);
+        dh[i] *= w[i];  // u
+        c = fmaf(dh[i], S[i], c);
+      }
+      const float k = row_sum(c, red[0]) * inv_h * rs;
+#pragma unroll
+      for (int i = 0; i < EPT; ++i) S[i] = fmaf(rs, dh[i], -S[i] * k);
     } else {
 #pragma unroll
       for (int i = 0; i < EPT; ++i) S[i] = 0.f;
-      __syncthreads();  // the sums of two rows use red[1]
+      __syncthreads();  // the second sums of two rows use the same place
     }
-    if (p.ds != nullptr) {
+    if (has_ds) {
       float ds[EPT];
-      me.take(ring, st, 3, 4, ds);
+      me.take(st, 3, ds);
 #pragma unroll
       for (int i = 0; i < EPT; ++i) S[i] += ds[i];
     }
-    ahead(row + ST);
+    float v[EPT];  // gate w_post, then gate w_post S
+    gate_post(v);
     c = 0.f;
-    float out[EPT];
+    if constexpr (GATE == GATE_ROW) {
+      float w[EPT], out[EPT];
+      me.kept(COL_GATE_POST, w);
+#pragma unroll
+      for (int i = 0; i < EPT; ++i) out[i] = w[i] * (S[i] * xr[i]);
+      me.put_as(p.dgate, at, p.gate_bf16, out);
+      if constexpr (M::STREAM_GATE) me.gate_take(st, 4, p.gate_bf16, w);
+      else me.kept(COL_GATE, w);
+#pragma unroll
+      for (int i = 0; i < EPT; ++i) A[i] = fmaf(w[i], S[i] * xr[i], A[i]);
+    }
+    ahead(row + ST, st);
+    if (++st == ST) st = 0;
 #pragma unroll
     for (int i = 0; i < EPT; ++i) {
-      const float a = S[i] * (x[i] * rx);
-      if (GATE == GATE_ROW) {
-        A[i] = fmaf(w.at(W_GATE, i), a, A[i]);
-        out[i] = w.at(W_POST, i) * a;
-      } else {
-        A[i] += a;
-      }
-      const float v = GATE == GATE_NONE ? S[i] * w.at(W_POST, i) : S[i] * w.at(W_GATE, i) * w.at(W_POST, i);
-      c = fmaf(v, x[i], c);
+      if (GATE != GATE_ROW) A[i] = fmaf(S[i], xr[i], A[i]);
+      v[i] *= S[i];
+      c = fmaf(v[i], xr[i], c);
+      S[i] *= p.scale;
     }
-    if (GATE == GATE_ROW) me.put_as(p.dgate, row * p.H, p.gate_bf16, out);
+    me.put(p.dres, at, S);
+    const float k = row_sum(c, red[1]) * inv_h;
 #pragma unroll
-    for (int i = 0; i < EPT; ++i) out[i] = p.scale * S[i];
-    me.put(p.dres, row, p.H, out);
-    const float k = row_sum(c, red[1]) * inv_h * rx * rx * rx;
-#pragma unroll
-    for (int i = 0; i < EPT; ++i) {
-      const float v = GATE == GATE_NONE ? S[i] * w.at(W_POST, i) : S[i] * w.at(W_GATE, i) * w.at(W_POST, i);
-      out[i] = fmaf(rx, v, -x[i] * k);
-    }
-    me.put(p.dx, row, p.H, out);
+    for (int i = 0; i < EPT; ++i) v[i] = rx * fmaf(-xr[i], k, v[i]);
+    me.put(p.dx, at, v);
     rx = rx_next, rs = rs_next;
     if (row + 1 == unit_end) {
       me.put_as(p.part_a, u * p.H, 0, A);
       if (++u < u1) {
         unit_end = first_row(u + 1);
-        if (GATE == GATE_SPAN) fetch(W_GATE, p.gate, u / p.units_per_span * p.H, p.gate_bf16);
+        if (GATE == GATE_SPAN) keep_gate_post(me, p, true, u / p.units_per_span);
 #pragma unroll
         for (int i = 0; i < EPT; ++i) A[i] = 0.f;
       }
@@ -560,11 +636,11 @@ struct BwdPlan {
   int units_per_span;
 };
 
-// Row ranges of the backward, none across a span.  A block of 4096 columns fills an SM; the partial rows of smaller
+// Row ranges of the backward, none across a span.  Two blocks of 4096 columns fill an SM; the partial rows of smaller
 // ones cost as much less.
 BwdPlan bwd_plan(int64_t rows, int64_t span, int64_t H, int gate) {
   BwdPlan b;
-  const int64_t blocks_per_sm = H >= 4096 ? 1 : H <= 256 ? 16 : 4096 / H;
+  const int64_t blocks_per_sm = H >= 4096 ? 2 : H <= 512 ? 16 : 8192 / H;
   if (gate != GATE_SPAN) span = rows;
   b.spans = rows / span;
   const int64_t want = (int64_t)num_sms() * blocks_per_sm;
@@ -623,6 +699,9 @@ bool pick_vectors(int64_t H, uintptr_t addr, F go) {
   return false;
 }
 
+// Threads of a row: whole warps with nv vectors each.
+int row_threads(int H, int vec, int nv) { return ((H / vec + nv - 1) / nv + 31) / 32 * 32; }
+
 uintptr_t bits(const void* p) { return reinterpret_cast<uintptr_t>(p); }
 
 // Low bits of the rows' addresses.  The weights, the gate and its gradient are read and written in pieces of up to 16
@@ -640,20 +719,27 @@ int launch_rows(F kernel, const NormArgs& p, int64_t blocks, int threads, int sm
   return check_launch(what);
 }
 
+// go(GATE constant) for the gate of this call.
+template <typename F>
+int by_gate(int gate, F go) {
+  if (gate == GATE_NONE) return go(std::integral_constant<int, GATE_NONE>{});
+  if (gate == GATE_SPAN) return go(std::integral_constant<int, GATE_SPAN>{});
+  return go(std::integral_constant<int, GATE_ROW>{});
+}
+
 template <typename T>
 int fwd_t(const NormArgs& p, int gate, cudaStream_t st) {
   int rc = ATS_OK;
   const bool ok = pick_vectors<T>(p.H, row_bits(p) | bits(p.s) | bits(p.h), [&](auto vb, auto nv) {
-    using M = Mine<T, vb.value, nv.value>;
-    const int threads = (p.H / M::VEC + nv.value - 1) / nv.value;
-    const int t = (threads + 31) / 32 * 32;
-    const int smem = M::STAGES * 2 * nv.value * vb.value * t + Columns<M::EPT>::bytes(t);
-    // enough blocks to fill the SMs, each with a run of rows
-    const int64_t cap = (int64_t)num_sms() * (t >= 512 ? 2 : t >= 32 * 3 ? 1024 / t : 16);
-    const int64_t blocks = p.rows < cap ? p.rows : cap;
-    rc = gate == GATE_NONE   ? launch_rows(sandwich_fwd_kernel<T, vb.value, nv.value, GATE_NONE>, p, blocks, t, smem, st, "sandwich_norm_fwd")
-         : gate == GATE_SPAN ? launch_rows(sandwich_fwd_kernel<T, vb.value, nv.value, GATE_SPAN>, p, blocks, t, smem, st, "sandwich_norm_fwd")
-                             : launch_rows(sandwich_fwd_kernel<T, vb.value, nv.value, GATE_ROW>, p, blocks, t, smem, st, "sandwich_norm_fwd");
+    rc = by_gate(gate, [&](auto g) {
+      using M = Mine<T, vb.value, nv.value, g.value>;
+      const int t = row_threads(p.H, M::VEC, M::ROW / vb.value);
+      // enough blocks to fill the SMs, each with a run of rows
+      const int64_t per_sm = t * M::BLOCKS >= 1024 ? 2 : M::BLOCKS * kRowThreads / t;
+      const int64_t cap = (int64_t)num_sms() * (per_sm < 16 ? per_sm : 16);
+      return launch_rows(sandwich_fwd_kernel<T, vb.value, nv.value, g.value>, p, p.rows < cap ? p.rows : cap, t,
+                         M::smem(t, 2, stages_of<M>(2)), st, "sandwich_norm_fwd");
+    });
   });
   if (ok) return rc;
   const int64_t cap = (int64_t)num_sms() * 16;
@@ -666,13 +752,12 @@ int bwd_t(const NormArgs& p, int gate, int64_t blocks, cudaStream_t st) {
   int rc = ATS_OK;
   const uintptr_t addr = row_bits(p) | bits(p.dh) | bits(p.ds) | bits(p.dx) | bits(p.dres);
   const bool ok = pick_vectors<T>(p.H, addr, [&](auto vb, auto nv) {
-    using M = Mine<T, vb.value, nv.value>;
-    const int threads = (p.H / M::VEC + nv.value - 1) / nv.value;
-    const int t = (threads + 31) / 32 * 32;
-    const int smem = M::STAGES * 4 * nv.value * vb.value * t + Columns<M::EPT>::bytes(t);
-    rc = gate == GATE_NONE   ? launch_rows(sandwich_bwd_kernel<T, vb.value, nv.value, GATE_NONE>, p, blocks, t, smem, st, "sandwich_norm_bwd")
-         : gate == GATE_SPAN ? launch_rows(sandwich_bwd_kernel<T, vb.value, nv.value, GATE_SPAN>, p, blocks, t, smem, st, "sandwich_norm_bwd")
-                             : launch_rows(sandwich_bwd_kernel<T, vb.value, nv.value, GATE_ROW>, p, blocks, t, smem, st, "sandwich_norm_bwd");
+    rc = by_gate(gate, [&](auto g) {
+      using M = Mine<T, vb.value, nv.value, g.value>;
+      const int t = row_threads(p.H, M::VEC, M::ROW / vb.value);
+      return launch_rows(sandwich_bwd_kernel<T, vb.value, nv.value, g.value>, p, blocks, t,
+                         M::smem(t, 4, stages_of<M>(4)), st, "sandwich_norm_bwd");
+    });
   });
   if (ok) return rc;
   sandwich_bwd_long_kernel<T><<<(unsigned)blocks, threads_for(p.H), 0, st>>>(p, gate);
