@@ -20,12 +20,12 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "tc_ptx.cuh"
 
 namespace ats {
 namespace {
 
 constexpr int kMaxThreads = 1024;
-constexpr int kReduceCols = 32, kReduceLanes = 32;
 
 enum Gate { GATE_NONE = 0, GATE_SPAN = 1, GATE_ROW = 2 };  // a gate row per span of rows, or per row
 
@@ -233,12 +233,11 @@ struct Mine {
   }
 };
 
-// Rows in flight: as many as half the SM (a whole one for a block alone) holds beside the columns, at most 8.
+// Rows in flight: 64 KB of them for 512 threads where two such blocks share an SM, 128 KB for one alone, at most 4.
 template <typename M>
 __host__ __device__ constexpr int stages_of(int tensors) {
-  const int room = (M::BLOCKS == 2 ? 108 : 216) * 1024 / kRowThreads - M::COLS * M::EPT * 4;
-  const int n = room / (tensors * M::ROW + (M::STREAM_GATE ? M::EPT * 4 : 0));
-  return n >= 8 ? 8 : n >= 4 ? 4 : n >= 2 ? 2 : 1;
+  const int n = (M::BLOCKS == 2 ? 64 : 128) * 1024 / kRowThreads / (tensors * M::ROW + (M::STREAM_GATE ? M::EPT * 4 : 0));
+  return n >= 4 ? 4 : n >= 2 ? 2 : 1;
 }
 
 enum { COL_GATE_POST = 0, COL_PRE = 1, COL_GATE = 2 };
@@ -352,6 +351,7 @@ __global__ void __launch_bounds__(kRowThreads, Mine<T, VB, NV, GATE>::BLOCKS)
   extern __shared__ __align__(16) char smem[];
   __shared__ float4 red[2][kRowThreads / 128];
   const M me(p.H, smem, 4, ST);
+  tc::launch_dependents();  // the sums' kernel may be brought up; it waits for this one
   // consecutive units (row ranges inside one span): their rows are consecutive too
   const int64_t u0 = p.units * blockIdx.x / gridDim.x, u1 = p.units * (blockIdx.x + 1) / gridDim.x;
   auto first_row = [&](int64_t u) {
@@ -581,54 +581,67 @@ __global__ void __launch_bounds__(kMaxThreads) sandwich_bwd_long_kernel(NormArgs
   }
 }
 
-// Column sums of n rows of `part` for 32 columns, by 32 lanes of rows and then the lanes in order; valid in lane 0.
-__device__ __forceinline__ float column_sum(const float* part, int64_t n, int H, int col, int rl,
-                                            float (*red)[kReduceCols + 1]) {
-  const int cl = threadIdx.x % kReduceCols;
-  float t = 0.f;
-  if (col < H)
-    for (int64_t q = rl; q < n; q += kReduceLanes) t += part[q * H + col];
-  __syncthreads();
-  red[rl][cl] = t;
-  __syncthreads();
-  float u = 0.f;
-  if (rl == 0)
-    for (int q = 0; q < kReduceLanes; ++q) u += red[q][cl];
-  return u;
-}
-
 __device__ __forceinline__ void store_as(void* p, int64_t i, int is_bf16, float v) {
   if (is_bf16) static_cast<bf16*>(p)[i] = __float2bfloat16_rn(v);
   else static_cast<float*>(p)[i] = v;
 }
 
-// One span: dgate = w_post A, and gate A into row `span` of part_a's first rows' place for the sum over spans.
-__global__ void __launch_bounds__(kReduceCols* kReduceLanes) sandwich_gate_kernel(NormArgs p, float* gate_a) {
-  __shared__ float red[kReduceLanes][kReduceCols + 1];
-  const int cl = threadIdx.x % kReduceCols, rl = threadIdx.x / kReduceCols;
-  const int col = blockIdx.x * kReduceCols + cl;
-  const int64_t spans = p.rows / p.span;
-  for (int64_t i = blockIdx.y; i < spans; i += gridDim.y) {
-    const float A = column_sum(p.part_a + i * p.units_per_span * p.H, p.units_per_span, p.H, col, rl, red);
-    if (rl == 0 && col < p.H) {
-      store_as(p.dgate, i * p.H + col, p.gate_bf16, load_as(p.w_post, col, p.w_bf16) * A);
-      gate_a[i * p.H + col] = load_as(p.gate, i * p.H + col, p.gate_bf16) * A;
-    }
-  }
+// Sums of the partial rows, 16 columns and 64 lanes of rows to a block, in a fixed order.  The lanes are dealt to the
+// spans (64 / spans each, or a span at a time each where there are more): dgate = w_post A of the span, and the
+// spans' gate A add up to dw_post.
+constexpr int kSumCols = 16, kSumLanes = 64;
+
+// n values of a column in four running sums
+__device__ __forceinline__ float lane_sum(const float (*v)[kSumCols + 1], int first, int n, int cl) {
+  float u[4] = {0.f, 0.f, 0.f, 0.f};
+  int q = 0;
+  for (; q + 4 <= n; q += 4)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u[i] += v[first + q + i][cl];
+  for (; q < n; ++q) u[0] += v[first + q][cl];
+  return (u[0] + u[1]) + (u[2] + u[3]);
 }
 
-__global__ void __launch_bounds__(kReduceCols* kReduceLanes) sandwich_dw_kernel(NormArgs p, const float* a, int64_t na,
-                                                                               int64_t nb, void* dw_post,
-                                                                               void* dw_pre) {
-  __shared__ float red[kReduceLanes][kReduceCols + 1];
-  const int cl = threadIdx.x % kReduceCols, rl = threadIdx.x / kReduceCols;
-  const int col = blockIdx.x * kReduceCols + cl;
-  const float A = column_sum(a, na, p.H, col, rl, red);
-  const float Bp = column_sum(p.part_b, nb, p.H, col, rl, red);
-  if (rl == 0 && col < p.H) {
-    store_as(dw_post, col, p.w_bf16, A);
-    store_as(dw_pre, col, p.w_bf16, Bp);
+__global__ void __launch_bounds__(kSumCols* kSumLanes) sandwich_sums_kernel(NormArgs p, int gate, int64_t spans,
+                                                                           int64_t blocks, void* dw_post,
+                                                                           void* dw_pre) {
+  __shared__ float red[3][kSumLanes][kSumCols + 1];
+  const int cl = threadIdx.x % kSumCols, rl = threadIdx.x / kSumCols;
+  const int col = blockIdx.x * kSumCols + cl;
+  const bool in = col < p.H;
+  const int64_t ups = p.units_per_span;
+  int groups = 1;  // spans at a time
+  while (groups < spans && groups < kSumLanes) groups <<= 1;
+  const int per = kSumLanes / groups;
+  const float wp = in ? load_as(p.w_post, col, p.w_bf16) : 0.f;
+  tc::wait_prerequisites();
+  float post = 0.f, a = 0.f, pre = 0.f;
+  for (int64_t i = rl / per; i < spans; i += groups) {  // once where a span has several lanes
+    a = 0.f;
+    if (in) {
+#pragma unroll 4
+      for (int64_t k = rl % per; k < ups; k += per) a += p.part_a[(i * ups + k) * p.H + col];
+      if (gate == GATE_SPAN) {
+        post = fmaf(a, load_as(p.gate, i * p.H + col, p.gate_bf16), post);
+        if (per == 1) store_as(p.dgate, i * p.H + col, p.gate_bf16, wp * a);
+      } else {
+        post += a;
+      }
+    }
   }
+  if (in) {
+#pragma unroll 4
+    for (int64_t q = rl; q < blocks; q += kSumLanes) pre += p.part_b[q * p.H + col];
+  }
+  red[0][rl][cl] = post;
+  red[1][rl][cl] = pre;
+  red[2][rl][cl] = a;
+  __syncthreads();
+  if (!in) return;
+  if (rl == 0) store_as(dw_post, col, p.w_bf16, lane_sum(red[0], 0, kSumLanes, cl));
+  if (rl == 2) store_as(dw_pre, col, p.w_bf16, lane_sum(red[1], 0, kSumLanes, cl));  // another warp
+  if (gate == GATE_SPAN && per > 1 && rl % per == per - 1 && rl / per < spans)
+    store_as(p.dgate, rl / per * (int64_t)p.H + col, p.gate_bf16, wp * lane_sum(red[2], rl / per * per, per, cl));
 }
 
 struct BwdPlan {
@@ -636,14 +649,17 @@ struct BwdPlan {
   int units_per_span;
 };
 
-// Row ranges of the backward, none across a span.  Two blocks of 4096 columns fill an SM; the partial rows of smaller
-// ones cost as much less.
-BwdPlan bwd_plan(int64_t rows, int64_t span, int64_t H, int gate) {
+// Blocks of a backward on an SM, at most: those of fewer columns are smaller, and their partial rows cost less.
+int64_t most_per_sm(int64_t H) { return H >= 4096 ? 2 : H <= 512 ? 16 : 8192 / H; }
+
+// Row ranges (units) of the backward, none across a span, for `per_sm` blocks on each SM, but 8 rows to a block before
+// a second one on an SM: a partial row is as many bytes as a row or more.
+BwdPlan bwd_plan(int64_t rows, int64_t span, int64_t per_sm) {
   BwdPlan b;
-  const int64_t blocks_per_sm = H >= 4096 ? 2 : H <= 512 ? 16 : 8192 / H;
-  if (gate != GATE_SPAN) span = rows;
+  const int64_t sms = num_sms();
+  int64_t want = rows / 8 < sms ? sms : rows / 8;
+  if (want > sms * per_sm) want = sms * per_sm;
   b.spans = rows / span;
-  const int64_t want = (int64_t)num_sms() * blocks_per_sm;
   int64_t per = b.spans >= want ? 1 : want / b.spans;
   if (per > span) per = span;
   b.units_per_span = (int)per;
@@ -712,11 +728,25 @@ uintptr_t row_bits(const NormArgs& p) {
 }
 
 template <typename F>
-int launch_rows(F kernel, const NormArgs& p, int64_t blocks, int threads, int smem, cudaStream_t st, const char* what) {
+int set_smem(F kernel, int smem, const char* what) {
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return fail(ATS_ECUDA, "%s: %s", what, cudaGetErrorString(e));
-  kernel<<<(unsigned)blocks, threads, smem, st>>>(p);
-  return check_launch(what);
+  return e == cudaSuccess ? ATS_OK : fail(ATS_ECUDA, "%s: %s", what, cudaGetErrorString(e));
+}
+
+// Blocks of `threads` threads and `smem` bytes that an SM holds, 1 to 16: `regs` registers a thread.
+int64_t resident(int regs, int threads, int smem) {
+  const int64_t by_regs = 65536 / ((int64_t)(regs + 7) / 8 * 8 * threads), by_smem = 227 * 1024 / (smem + 1536);
+  const int64_t n = by_regs < by_smem ? by_regs : by_smem;
+  return n < 1 ? 1 : n > 16 ? 16 : n;
+}
+
+template <auto KERNEL>
+int regs_of() {
+  static const int regs = [] {
+    cudaFuncAttributes a;
+    return cudaFuncGetAttributes(&a, KERNEL) == cudaSuccess ? a.numRegs : 128;
+  }();
+  return regs;
 }
 
 // go(GATE constant) for the gate of this call.
@@ -733,12 +763,12 @@ int fwd_t(const NormArgs& p, int gate, cudaStream_t st) {
   const bool ok = pick_vectors<T>(p.H, row_bits(p) | bits(p.s) | bits(p.h), [&](auto vb, auto nv) {
     rc = by_gate(gate, [&](auto g) {
       using M = Mine<T, vb.value, nv.value, g.value>;
-      const int t = row_threads(p.H, M::VEC, M::ROW / vb.value);
-      // enough blocks to fill the SMs, each with a run of rows
-      const int64_t per_sm = t * M::BLOCKS >= 1024 ? 2 : M::BLOCKS * kRowThreads / t;
-      const int64_t cap = (int64_t)num_sms() * (per_sm < 16 ? per_sm : 16);
-      return launch_rows(sandwich_fwd_kernel<T, vb.value, nv.value, g.value>, p, p.rows < cap ? p.rows : cap, t,
-                         M::smem(t, 2, stages_of<M>(2)), st, "sandwich_norm_fwd");
+      constexpr auto kernel = sandwich_fwd_kernel<T, vb.value, nv.value, g.value>;
+      const int t = row_threads(p.H, M::VEC, nv.value), smem = M::smem(t, 2, stages_of<M>(2));
+      ATS_TRY(set_smem(kernel, smem, "sandwich_norm_fwd"));
+      const int64_t cap = num_sms() * resident(regs_of<kernel>(), t, smem);
+      kernel<<<(unsigned)(p.rows < cap ? p.rows : cap), t, smem, st>>>(p);
+      return check_launch("sandwich_norm_fwd");
     });
   });
   if (ok) return rc;
@@ -748,20 +778,46 @@ int fwd_t(const NormArgs& p, int gate, cudaStream_t st) {
 }
 
 template <typename T>
-int bwd_t(const NormArgs& p, int gate, int64_t blocks, cudaStream_t st) {
+int bwd_t(NormArgs p, int gate, float* workspace, void* dw_post, void* dw_pre, cudaStream_t st) {
+  BwdPlan b;
+  auto plan = [&](int64_t per_sm) {
+    const int64_t most = most_per_sm(p.H);
+    b = bwd_plan(p.rows, p.span, per_sm < most ? per_sm : most);
+    p.units_per_span = b.units_per_span, p.units = b.units;
+    p.part_a = workspace;
+    p.part_b = workspace + b.units * p.H;
+  };
   int rc = ATS_OK;
   const uintptr_t addr = row_bits(p) | bits(p.dh) | bits(p.ds) | bits(p.dx) | bits(p.dres);
   const bool ok = pick_vectors<T>(p.H, addr, [&](auto vb, auto nv) {
     rc = by_gate(gate, [&](auto g) {
       using M = Mine<T, vb.value, nv.value, g.value>;
-      const int t = row_threads(p.H, M::VEC, M::ROW / vb.value);
-      return launch_rows(sandwich_bwd_kernel<T, vb.value, nv.value, g.value>, p, blocks, t,
-                         M::smem(t, 4, stages_of<M>(4)), st, "sandwich_norm_bwd");
+      constexpr auto kernel = sandwich_bwd_kernel<T, vb.value, nv.value, g.value>;
+      const int t = row_threads(p.H, M::VEC, nv.value), smem = M::smem(t, 4, stages_of<M>(4));
+      ATS_TRY(set_smem(kernel, smem, "sandwich_norm_bwd"));
+      plan(resident(regs_of<kernel>(), t, smem));
+      kernel<<<(unsigned)b.blocks, t, smem, st>>>(p);
+      return check_launch("sandwich_norm_bwd");
     });
   });
-  if (ok) return rc;
-  sandwich_bwd_long_kernel<T><<<(unsigned)blocks, threads_for(p.H), 0, st>>>(p, gate);
-  return check_launch("sandwich_norm_bwd");
+  if (!ok) {
+    plan(2);
+    sandwich_bwd_long_kernel<T><<<(unsigned)b.blocks, threads_for(p.H), 0, st>>>(p, gate);
+    rc = check_launch("sandwich_norm_bwd");
+  }
+  ATS_TRY(rc);
+  cudaLaunchAttribute attr[1];  // brought up while the rows are still worked on
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((p.H + kSumCols - 1) / kSumCols));
+  cfg.blockDim = dim3(kSumCols * kSumLanes);
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, sandwich_sums_kernel, p, gate, b.spans, b.blocks, dw_post, dw_pre);
+  if (e != cudaSuccess) return fail(ATS_ECUDA, "sandwich_sums: %s", cudaGetErrorString(e));
+  return check_launch("sandwich_sums");
 }
 
 }  // namespace
@@ -792,9 +848,8 @@ int ats_sandwich_norm_fwd(const void* x, const void* residual, ats_dtype dtype, 
 
 size_t ats_sandwich_norm_bwd_workspace_bytes(int64_t rows, int64_t hidden, int64_t rows_per_gate) {
   if (rows <= 0 || hidden <= 0 || rows_per_gate < 0 || (rows_per_gate > 0 && rows % rows_per_gate != 0)) return 0;
-  const BwdPlan b = bwd_plan(rows, rows_per_gate > 1 ? rows_per_gate : rows, hidden,
-                             rows_per_gate > 1 ? GATE_SPAN : GATE_NONE);
-  return (size_t)(b.units + b.blocks + (rows_per_gate > 1 ? b.spans : 0)) * (size_t)hidden * sizeof(float);
+  const int64_t blocks = num_sms() * most_per_sm(hidden), spans = rows_per_gate > 1 ? rows / rows_per_gate : 1;
+  return (size_t)((spans > blocks ? spans : blocks) + blocks) * (size_t)hidden * sizeof(float);
 }
 
 int ats_sandwich_norm_bwd(const void* dh, const void* dsum, const void* x, const void* residual, ats_dtype dtype,
@@ -812,7 +867,6 @@ int ats_sandwich_norm_bwd(const void* dh, const void* dsum, const void* x, const
   if (workspace == nullptr || !aligned16(workspace) ||
       workspace_bytes < ats_sandwich_norm_bwd_workspace_bytes(rows, hidden, gate != nullptr ? rows_per_gate : 0))
     return fail(ATS_EBADARG, "sandwich_norm_bwd: workspace too small");
-  const BwdPlan b = bwd_plan(rows, rows_per_gate, hidden, g);
   NormArgs p{};
   p.x = x, p.res = residual, p.dh = dh, p.ds = dsum, p.dx = dx, p.dres = dresidual;
   p.w_post = w_post, p.w_pre = w_pre, p.gate = gate, p.dgate = dgate;
@@ -820,23 +874,9 @@ int ats_sandwich_norm_bwd(const void* dh, const void* dsum, const void* x, const
   p.rx = const_cast<float*>(rstd_x), p.rs = const_cast<float*>(rstd_sum);
   p.rows = rows, p.span = g == GATE_SPAN ? rows_per_gate : rows;
   p.H = (int)hidden, p.scale = residual_scale;
-  p.units_per_span = b.units_per_span, p.units = b.units;
-  p.part_a = static_cast<float*>(workspace);
-  p.part_b = p.part_a + b.units * hidden;
-  float* gate_a = p.part_b + b.blocks * hidden;
   cudaStream_t st = (cudaStream_t)stream;
-  ATS_TRY(dtype == ATS_BF16 ? bwd_t<bf16>(p, g, b.blocks, st) : bwd_t<float>(p, g, b.blocks, st));
-  const unsigned cols = (unsigned)((hidden + kReduceCols - 1) / kReduceCols);
-  const float* a = p.part_a;
-  int64_t na = b.units;
-  if (g == GATE_SPAN) {
-    sandwich_gate_kernel<<<dim3(cols, (unsigned)(b.spans < 1024 ? b.spans : 1024)), kReduceCols * kReduceLanes, 0, st>>>(
-        p, gate_a);
-    ATS_TRY(check_launch("sandwich_gate"));
-    a = gate_a, na = b.spans;
-  }
-  sandwich_dw_kernel<<<cols, kReduceCols * kReduceLanes, 0, st>>>(p, a, na, b.blocks, dw_post, dw_pre);
-  return check_launch("sandwich_dw");
+  float* ws = static_cast<float*>(workspace);
+  return dtype == ATS_BF16 ? bwd_t<bf16>(p, g, ws, dw_post, dw_pre, st) : bwd_t<float>(p, g, ws, dw_post, dw_pre, st);
 }
 
 }  // extern "C"

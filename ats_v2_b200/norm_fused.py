@@ -168,27 +168,37 @@ def fused_add_rmsnorm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Ten
     return _AddRMSNormFn.apply(x, residual, weight, eps)
 
 
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """t contiguous from a multiple of 16 bytes (a view may start anywhere): the kernels read weights and gates so."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _sandwich_forward(x2, r2, wp, wn, g, rows_per_gate, residual_scale, eps, train):
+    """The forward kernel on [rows, hidden] tensors: (h, s, rstd), rstd [2, rows] kept for the backward."""
+    rows, H = x2.shape
+    s, h = torch.empty_like(x2), torch.empty_like(x2)
+    rstd = torch.empty((2, rows), dtype=torch.float32, device=x2.device) if train else None
+    p = rstd.data_ptr() if train else 0
+    with _lib.device_of(x2):
+        _lib.call("ats_sandwich_norm_fwd", x2.data_ptr(), r2.data_ptr(), _lib.dtype_code(x2.dtype), wp.data_ptr(),
+                  wn.data_ptr(), _lib.dtype_code(wp.dtype), g.data_ptr() if g is not None else None,
+                  _lib.dtype_code(g.dtype) if g is not None else 0, rows_per_gate, residual_scale, eps, s.data_ptr(),
+                  h.data_ptr(), p or None, p + 4 * rows if p else None, rows, H, _lib.stream_of(x2))
+    return h, s, rstd
+
+
 class _SandwichNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, post_weight, pre_weight, gate, rows_per_gate, residual_scale, eps):
         ctx.set_materialize_grads(False)  # an unused result's gradient arrives as None and is not read
         H = x.shape[-1]
         x2, r2 = x.reshape(-1, H).contiguous(), residual.reshape(-1, H).contiguous()
-        wp, wn = post_weight.contiguous(), pre_weight.contiguous()
-        g = gate.contiguous() if gate is not None else None
-        rows = x2.shape[0]
-        s, h = torch.empty_like(x2), torch.empty_like(x2)
-        train = any(ctx.needs_input_grad)
-        rstd = torch.empty((2, rows), dtype=torch.float32, device=x.device) if train else None
-        with _lib.device_of(x):
-            _lib.call("ats_sandwich_norm_fwd", x2.data_ptr(), r2.data_ptr(), _lib.dtype_code(x2.dtype), wp.data_ptr(),
-                      wn.data_ptr(), _lib.dtype_code(wp.dtype), _lib.ptr(g),
-                      _lib.dtype_code(g.dtype) if g is not None else 0, rows_per_gate, residual_scale, eps,
-                      s.data_ptr(), h.data_ptr(), rstd[0].data_ptr() if train else None,
-                      rstd[1].data_ptr() if train else None, rows, H, _lib.stream_of(x))
-        if train:
-            ctx.save_for_backward(x2, r2, wp, wn, g, rstd)
-            ctx.meta = rows_per_gate, residual_scale, x.shape, gate.shape if gate is not None else None
+        wp, wn = _aligned(post_weight), _aligned(pre_weight)
+        g = _aligned(gate) if gate is not None else None
+        h, s, rstd = _sandwich_forward(x2, r2, wp, wn, g, rows_per_gate, residual_scale, eps, True)
+        ctx.save_for_backward(x2, r2, wp, wn, g, rstd)
+        ctx.meta = rows_per_gate, residual_scale, x.shape, gate.shape if gate is not None else None
         return h.view(x.shape), s.view(x.shape)
 
     @staticmethod
@@ -214,7 +224,7 @@ class _SandwichNormFn(torch.autograd.Function):
             _lib.call("ats_sandwich_norm_bwd", _lib.ptr(dh), _lib.ptr(ds), x.data_ptr(), r.data_ptr(),
                       _lib.dtype_code(x.dtype), wp.data_ptr(), wn.data_ptr(), _lib.dtype_code(wp.dtype), _lib.ptr(g),
                       _lib.dtype_code(g.dtype) if g is not None else 0, rows_per_gate, residual_scale,
-                      rstd[0].data_ptr(), rstd[1].data_ptr(), dx.data_ptr(), dr.data_ptr(), dwp.data_ptr(),
+                      rstd.data_ptr(), rstd.data_ptr() + 4 * rows, dx.data_ptr(), dr.data_ptr(), dwp.data_ptr(),
                       dwn.data_ptr(), _lib.ptr(dg), ws.data_ptr(), wsb, rows, H, _lib.stream_of(x))
         return (dx.view(shape), dr.view(shape), dwp, dwn, dg.view(gate_shape) if dg is not None else None,
                 None, None, None)
@@ -278,4 +288,11 @@ def fused_sandwich_norm(x: torch.Tensor, residual: torch.Tensor, post_weight: to
     residual_scale, eps = float(residual_scale), float(eps)
     if _lib.on_cpu("fused_sandwich_norm", x, residual, post_weight, pre_weight, gate):
         return _torch_sandwich_norm(x, residual, post_weight, pre_weight, gate, residual_scale, eps)
-    return _SandwichNormFn.apply(x, residual, post_weight, pre_weight, gate, rows_per_gate, residual_scale, eps)
+    tensors = (x, residual, post_weight, pre_weight, gate)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return _SandwichNormFn.apply(*tensors, rows_per_gate, residual_scale, eps)
+    H = x.shape[-1]
+    h, s, _ = _sandwich_forward(x.reshape(-1, H).contiguous(), residual.reshape(-1, H).contiguous(),
+                                _aligned(post_weight), _aligned(pre_weight),
+                                _aligned(gate) if gate is not None else None, rows_per_gate, residual_scale, eps, False)
+    return h.view(x.shape), s.view(x.shape)

@@ -194,23 +194,21 @@ def axis_of_pairs(sections: tuple[int, ...], interleaved: bool = False) -> bytes
     return bytes(a for _, a in (sorted(pairs) if interleaved else pairs))
 
 
-def _strides(t: torch.Tensor):
-    return _lib.strides3(t.stride(0), t.stride(1), t.stride(2))
-
-
 def _launch_axes(q, q_out, k, k_out, positions, inv_freq, axes: bytes, n_axes: int, backward: bool) -> None:
-    t = q if q is not None else k
-    B, _, S, D = t.shape
-    ps = (positions.stride(0), positions.stride(1) if positions.dim() == 3 else 0, positions.stride(-1))
     if q is None:
         q, q_out, k, k_out = k, k_out, None, None
-    with _lib.device_of(t):
-        _lib.call("ats_rope_axes_apply", q.data_ptr(), q_out.data_ptr(), q.shape[1], _strides(q), _strides(q_out),
-                  _lib.ptr(k), _lib.ptr(k_out), k.shape[1] if k is not None else 0,
-                  _strides(k) if k is not None else None, _strides(k_out) if k is not None else None,
-                  positions.data_ptr(), _lib.ATS_POS_TYPES[positions.dtype], _lib.strides3(*ps), n_axes,
-                  inv_freq.data_ptr(), axes, len(axes), B, S, D, _lib.dtype_code(t.dtype), 1 if backward else 0,
-                  _lib.stream_of(t))
+    B, H, S, D = q.shape
+    s3 = _lib.strides3
+    pos = positions.stride()
+    if k is not None:
+        kargs = (k.data_ptr(), k_out.data_ptr(), k.shape[1], s3(*k.stride()[:3]), s3(*k_out.stride()[:3]))
+    else:
+        kargs = (None, None, 0, None, None)
+    with _lib.device_of(q):
+        _lib.call("ats_rope_axes_apply", q.data_ptr(), q_out.data_ptr(), H, s3(*q.stride()[:3]),
+                  s3(*q_out.stride()[:3]), *kargs, positions.data_ptr(), _lib.ATS_POS_TYPES[positions.dtype],
+                  s3(pos[0], pos[1] if len(pos) == 3 else 0, pos[-1]), n_axes, inv_freq.data_ptr(), axes, len(axes),
+                  B, S, D, _lib.dtype_code(q.dtype), 1 if backward else 0, _lib.stream_of(q))
 
 
 class _MultiAxisRotaryFn(torch.autograd.Function):
@@ -284,7 +282,12 @@ def apply_multi_axis_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: 
                 _torch_multi_axis(k, positions, inv_freq, axes) if k is not None else None)
     q = _last_dim_contig(q)
     k = _last_dim_contig(k) if k is not None else None
-    return _MultiAxisRotaryFn.apply(q, k, positions, inv_freq.contiguous(), axes, n_axes)
+    inv_freq = inv_freq.contiguous()
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        return _MultiAxisRotaryFn.apply(q, k, positions, inv_freq, axes, n_axes)
+    q_out, k_out = torch.empty_like(q), torch.empty_like(k) if k is not None else None
+    _launch_axes(q, q_out, k, k_out, positions, inv_freq, axes, n_axes, False)
+    return q_out, k_out
 
 
 class MultiAxisRotaryEmbedding(nn.Module):
