@@ -272,7 +272,7 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 
 def stream_of(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(t.device.index)  # current_stream(t.device).cuda_stream without the object
 
 
 _SAME_DEVICE = contextlib.nullcontext()
@@ -297,6 +297,9 @@ def on_cpu(name: str, *tensors: torch.Tensor | None) -> bool:
     for CUDA tensors): CPU tensors take the reference's torch formulas, which
     its CPU tests pin, and CUDA tensors always take this library's kernels --
     a CUDA tensor never runs the torch formula, and a missing library raises."""
+    dev = next(t.device for t in tensors if t is not None)
+    if all(t is None or t.device == dev for t in tensors) and dev.type in ("cpu", "cuda"):  # the usual case
+        return dev.type == "cpu"
     devs = {t.device.type for t in tensors if t is not None}
     if devs == {"cpu"}:
         return True

@@ -979,7 +979,7 @@ int ats_int8_quantize(const void* x, int64_t x_row_stride, ats_dtype dtype, void
 }
 
 size_t ats_int8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K) {
-  if (M < 0 || N < 1 || K < 1) return 0;
+  if (M < 0 || N < 1 || K < 1 || (M == 1 && K <= kDotLongest)) return 0;  // one token is quantised where it is used
   return q_bytes(M, K) + align_up((size_t)M * sizeof(float), 256);
 }
 
@@ -998,7 +998,8 @@ int ats_int8_linear(const void* x, int64_t x_row_stride, ats_dtype dtype, const 
   if (M == 0) return ATS_OK;
   if (x == nullptr || w == nullptr || w_scale == nullptr || y == nullptr)
     return fail(ATS_EBADARG, "int8_linear: null pointer");
-  if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < ats_int8_linear_workspace_bytes(M, N, K))
+  const size_t need = ats_int8_linear_workspace_bytes(M, N, K);
+  if (need > 0 && (workspace == nullptr || !aligned16(workspace) || workspace_bytes < need))
     return fail(ATS_EBADARG, "int8_linear: workspace too small");
   int8_t* q = static_cast<int8_t*>(workspace);
   float* sx = reinterpret_cast<float*>(q + q_bytes(M, K));

@@ -174,17 +174,18 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
-def _sandwich_forward(x2, r2, wp, wn, g, rows_per_gate, residual_scale, eps, train):
-    """The forward kernel on [rows, hidden] tensors: (h, s, rstd), rstd [2, rows] kept for the backward."""
-    rows, H = x2.shape
-    s, h = torch.empty_like(x2), torch.empty_like(x2)
-    rstd = torch.empty((2, rows), dtype=torch.float32, device=x2.device) if train else None
+def _sandwich_forward(x, residual, wp, wn, g, rows_per_gate, residual_scale, eps, train):
+    """The forward kernel on contiguous tensors: (h, s, rstd), rstd [2, rows] kept for the backward."""
+    H = x.shape[-1]
+    rows = x.numel() // H
+    s, h = torch.empty_like(x), torch.empty_like(x)
+    rstd = torch.empty((2, rows), dtype=torch.float32, device=x.device) if train else None
     p = rstd.data_ptr() if train else 0
-    with _lib.device_of(x2):
-        _lib.call("ats_sandwich_norm_fwd", x2.data_ptr(), r2.data_ptr(), _lib.dtype_code(x2.dtype), wp.data_ptr(),
+    with _lib.device_of(x):
+        _lib.call("ats_sandwich_norm_fwd", x.data_ptr(), residual.data_ptr(), _lib.dtype_code(x.dtype), wp.data_ptr(),
                   wn.data_ptr(), _lib.dtype_code(wp.dtype), g.data_ptr() if g is not None else None,
                   _lib.dtype_code(g.dtype) if g is not None else 0, rows_per_gate, residual_scale, eps, s.data_ptr(),
-                  h.data_ptr(), p or None, p + 4 * rows if p else None, rows, H, _lib.stream_of(x2))
+                  h.data_ptr(), p or None, p + 4 * rows if p else None, rows, H, _lib.stream_of(x))
     return h, s, rstd
 
 
@@ -192,14 +193,13 @@ class _SandwichNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, post_weight, pre_weight, gate, rows_per_gate, residual_scale, eps):
         ctx.set_materialize_grads(False)  # an unused result's gradient arrives as None and is not read
-        H = x.shape[-1]
-        x2, r2 = x.reshape(-1, H).contiguous(), residual.reshape(-1, H).contiguous()
+        x, residual = x.contiguous(), residual.contiguous()
         wp, wn = _aligned(post_weight), _aligned(pre_weight)
         g = _aligned(gate) if gate is not None else None
-        h, s, rstd = _sandwich_forward(x2, r2, wp, wn, g, rows_per_gate, residual_scale, eps, True)
-        ctx.save_for_backward(x2, r2, wp, wn, g, rstd)
-        ctx.meta = rows_per_gate, residual_scale, x.shape, gate.shape if gate is not None else None
-        return h.view(x.shape), s.view(x.shape)
+        h, s, rstd = _sandwich_forward(x, residual, wp, wn, g, rows_per_gate, residual_scale, eps, True)
+        ctx.save_for_backward(x, residual, wp, wn, g, rstd)
+        ctx.meta = rows_per_gate, residual_scale
+        return h, s
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -207,14 +207,13 @@ class _SandwichNormFn(torch.autograd.Function):
         if dh is None and ds is None:
             return (None,) * 8
         x, r, wp, wn, g, rstd = ctx.saved_tensors
-        rows_per_gate, residual_scale, shape, gate_shape = ctx.meta
-        rows, H = x.shape
+        rows_per_gate, residual_scale = ctx.meta
+        H = x.shape[-1]
+        rows = x.numel() // H
         if rows == 0:
-            zero = x.new_zeros(shape)
-            return (zero, zero.clone(), torch.zeros_like(wp), torch.zeros_like(wn),
-                    torch.zeros(gate_shape, dtype=g.dtype, device=g.device) if g is not None else None,
-                    None, None, None)
-        dh, ds = (t.reshape(rows, H).to(x.dtype).contiguous() if t is not None else None for t in (dh, ds))
+            return (torch.zeros_like(x), torch.zeros_like(x), torch.zeros_like(wp), torch.zeros_like(wn),
+                    torch.zeros_like(g) if g is not None else None, None, None, None)
+        dh, ds = (t.to(x.dtype).contiguous() if t is not None else None for t in (dh, ds))
         dx, dr = torch.empty_like(x), torch.empty_like(r)
         dwp, dwn = torch.empty_like(wp), torch.empty_like(wn)
         dg = torch.empty_like(g) if g is not None else None
@@ -226,8 +225,7 @@ class _SandwichNormFn(torch.autograd.Function):
                       _lib.dtype_code(g.dtype) if g is not None else 0, rows_per_gate, residual_scale,
                       rstd.data_ptr(), rstd.data_ptr() + 4 * rows, dx.data_ptr(), dr.data_ptr(), dwp.data_ptr(),
                       dwn.data_ptr(), _lib.ptr(dg), ws.data_ptr(), wsb, rows, H, _lib.stream_of(x))
-        return (dx.view(shape), dr.view(shape), dwp, dwn, dg.view(gate_shape) if dg is not None else None,
-                None, None, None)
+        return dx, dr, dwp, dwn, dg, None, None, None
 
 
 def _rows_per_gate(shape: torch.Size, gate: torch.Tensor) -> int:
@@ -291,8 +289,5 @@ def fused_sandwich_norm(x: torch.Tensor, residual: torch.Tensor, post_weight: to
     tensors = (x, residual, post_weight, pre_weight, gate)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         return _SandwichNormFn.apply(*tensors, rows_per_gate, residual_scale, eps)
-    H = x.shape[-1]
-    h, s, _ = _sandwich_forward(x.reshape(-1, H).contiguous(), residual.reshape(-1, H).contiguous(),
-                                _aligned(post_weight), _aligned(pre_weight),
-                                _aligned(gate) if gate is not None else None, rows_per_gate, residual_scale, eps, False)
-    return h.view(x.shape), s.view(x.shape)
+    return _sandwich_forward(x.contiguous(), residual.contiguous(), _aligned(post_weight), _aligned(pre_weight),
+                             _aligned(gate) if gate is not None else None, rows_per_gate, residual_scale, eps, False)[:2]

@@ -159,9 +159,9 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor,
     y = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=x.device)
     with _lib.device_of(x):
         wsb = _lib.query("ats_int8_linear_workspace_bytes", M, N, K)
-        ws = torch.empty(wsb, dtype=torch.uint8, device=x.device)
+        ws = torch.empty(wsb, dtype=torch.uint8, device=x.device) if wsb else None
         _lib.call("ats_int8_linear", x2.data_ptr(), x2.stride(0), code, weight.data_ptr(), ldw,
-                  scale.data_ptr(), _lib.ptr(bias), bias_code, y.data_ptr(), M, N, K, ws.data_ptr(), wsb,
+                  scale.data_ptr(), _lib.ptr(bias), bias_code, y.data_ptr(), M, N, K, _lib.ptr(ws), wsb,
                   _lib.stream_of(x))
     return y
 
