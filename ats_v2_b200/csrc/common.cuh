@@ -105,6 +105,18 @@ __device__ __forceinline__ void store_chunk(T* p, const float (&v)[Chunk<T>::N])
   *reinterpret_cast<uint4*>(p) = raw;
 }
 
+// Round N floats to T; bf16 two at a time (one conversion for a pair).
+template <typename T, int N>
+__device__ __forceinline__ void round_n(const float* v, T* e) {
+  if constexpr (sizeof(T) == 2 && N % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) *reinterpret_cast<__nv_bfloat162*>(e + i) = __floats2bfloat162_rn(v[i], v[i + 1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) e[i] = Cvt<T>::from_f(v[i]);
+  }
+}
+
 // Load N consecutive values of T (N*sizeof(T) a multiple of 16) as floats.
 template <typename T, int N>
 __device__ __forceinline__ void load_n(const T* p, float (&v)[N]) {

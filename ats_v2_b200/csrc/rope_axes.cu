@@ -10,8 +10,8 @@
 // reduced to about [-1/2, 1/2] there, so a far position loses nothing; the sine
 // and cosine of the remainder are float32 (sincospif).  A block owns a few tokens
 // and all (or a share) of their heads: it computes the tokens' cosines and
-// sines once into shared memory, so that work is spread over the heads, and
-// then streams the heads through registers.  Every element is read once and
+// sines once into shared memory, so that work is spread over the heads; each
+// thread keeps those of its vector in registers and streams heads past them.  Every element is read once and
 // written once; HBM bounds it.
 #include "common.cuh"
 
@@ -19,10 +19,11 @@ namespace ats {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kUnroll = 4;          // rows in flight per thread
-constexpr int kItemsPerThread = 8;  // vectors a thread handles in a full block
+constexpr int kUnroll = 4;       // heads in flight per thread
+constexpr int kMostHeads = 8;    // heads a thread handles
 constexpr double kInv2PiHi = 0.15915494309189535, kInv2PiLo = -9.839338337591243e-18;  // 1 / (2 pi) in two parts
-constexpr int kTableMax = 2048;     // cosine/sine entries of a block (16 KB)
+constexpr int kTableMax = 2048;  // cosine/sine entries of a block (16 KB)
+constexpr int kPosMax = 1024;    // positions of a block (8 KB)
 
 struct AxesTensor {
   const void* in;
@@ -38,11 +39,18 @@ struct AxesArgs {
   int64_t ps_a, ps_b, ps_s;
   const float* inv_freq;
   int64_t n_tokens, S;
-  int D, pairs;
-  int tokens_per_block, heads_per_block;
+  int D, pairs, axes;
+  int tokens_per_block, group, heads_each;  // `group` threads share a token's heads, heads_each to each
   float sign;  // of the sine: +1 forward, -1 adjoint
   uint8_t axis[ATS_ROPE_MAX_PAIRS];
 };
+
+// Batch and sequence index of a token.
+__device__ __forceinline__ void split(const AxesArgs& p, int64_t tok, int64_t& b, int64_t& s) {
+  if (p.n_tokens <= 0x7fffffff) b = (unsigned)tok / (unsigned)p.S;  // S <= n_tokens
+  else b = tok / p.S;
+  s = tok - b * p.S;
+}
 
 // V consecutive elements of T moved as one access.
 template <int BYTES> struct Raw;
@@ -57,111 +65,135 @@ __device__ __forceinline__ double load_pos(const AxesArgs& p, int64_t i) {
   return (double)static_cast<const float*>(p.pos)[i];
 }
 
+// A thread owns one vector position of the pairs of one token and heads_each heads, `group` apart; consecutive threads
+// take consecutive vectors of a head's row.
 template <typename T, int V>
-__global__ void __launch_bounds__(kThreads) rope_axes_kernel(const __grid_constant__ AxesArgs p) {
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 3) rope_axes_kernel(const __grid_constant__ AxesArgs p) {
   using R = typename Raw<V * (int)sizeof(T)>::type;
-  extern __shared__ float table[];  // cosines [tokens][pairs], then sines
+  // frequencies [pairs], positions [axes][tokens], cosines [tokens][pairs], sines, axes [pairs]
+  extern __shared__ __align__(16) double2 freq_s[];
+  double* pos_s = reinterpret_cast<double*>(freq_s + p.pairs);
   const int64_t tok0 = (int64_t)blockIdx.x * p.tokens_per_block;
   const int ntok = (int)(p.n_tokens - tok0 < p.tokens_per_block ? p.n_tokens - tok0 : p.tokens_per_block);
-  const int heads_all = p.q.heads + p.k.heads;
-  const int h0 = blockIdx.y * p.heads_per_block;
-  const int nh = heads_all - h0 < p.heads_per_block ? heads_all - h0 : p.heads_per_block;
-  float* cosv = table;
-  float* sinv = table + p.tokens_per_block * p.pairs;
-  const unsigned rows = (unsigned)ntok * nh;  // (token, head) rows of this block
+  const int heads = p.q.heads + p.k.heads;
+  float* cosv = reinterpret_cast<float*>(pos_s + (p.axes * p.tokens_per_block + 1) / 2 * 2);
+  float* sinv = cosv + p.tokens_per_block * p.pairs;
+  int* axis_s = reinterpret_cast<int*>(sinv + p.tokens_per_block * p.pairs);  // [pairs] first position of the pair's axis
 
-  // address of row r (token-major): the row's first element in the input and the output
-  auto locate = [&](unsigned r, const T*& src, T*& dst, int& t) {
-    t = (int)(r / (unsigned)nh);
-    const int h = h0 + (int)(r - (unsigned)t * nh);
-    const int64_t tok = tok0 + t;
-    const int64_t b = tok / p.S, s = tok - b * p.S;
-    const bool isq = h < p.q.heads;
-    const AxesTensor& x = isq ? p.q : p.k;
-    const int hh = isq ? h : h - p.q.heads;
-    src = static_cast<const T*>(x.in) + b * x.is_b + hh * x.is_h + s * x.is_s;
-    dst = static_cast<T*>(x.out) + b * x.os_b + hh * x.os_h + s * x.os_s;
-  };
-
-  // a thread keeps one vector position of the pairs and walks the rows
   const int vecs = p.pairs / V;
-  const int rows_per_step = kThreads / vecs;
-  const int my_row = threadIdx.x / vecs;
-  const int col = (threadIdx.x - my_row * vecs) * V;
-  const bool active = my_row < rows_per_step;
+  const int rest = (int)threadIdx.x / vecs, col = ((int)threadIdx.x - rest * vecs) * V;
+  const int t = rest / p.group;
+  const int h0 = (int)blockIdx.y * p.group * p.heads_each + (rest - t * p.group);
+  const bool active = t < ntok;
+  // where head h of this thread's token begins: q's heads, then k's
+  int64_t b, s;
+  split(p, tok0 + (active ? t : 0), b, s);
+  const T* qi = static_cast<const T*>(p.q.in) + b * p.q.is_b + s * p.q.is_s;
+  const T* ki = static_cast<const T*>(p.k.in) + b * p.k.is_b + s * p.k.is_s;
+  T* qo = static_cast<T*>(p.q.out) + b * p.q.os_b + s * p.q.os_s;
+  T* ko = static_cast<T*>(p.k.out) + b * p.k.os_b + s * p.k.os_s;
+  auto source = [&](int h) {
+    return h < p.q.heads ? qi + h * p.q.is_h : ki + (h - p.q.heads) * p.k.is_h;
+  };
+  auto target = [&](int h) {
+    return h < p.q.heads ? qo + h * p.q.os_h : ko + (h - p.q.heads) * p.k.os_h;
+  };
+  const int h_end = h0 + p.group * p.heads_each < heads ? h0 + p.group * p.heads_each : heads;
   R ra[kUnroll], rb[kUnroll];
-  auto load = [&](unsigned base) {
+  auto load = [&](int first) {
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-      const unsigned r = base + u * rows_per_step;
-      if (active && r < rows) {
-        const T* src;
-        T* dst;
-        int t;
-        locate(r, src, dst, t);
-        ra[u] = *reinterpret_cast<const R*>(src + col);
-        rb[u] = *reinterpret_cast<const R*>(src + col + p.pairs);
+      const int h = first + u * p.group;
+      if (active && h < h_end) {
+        const T* src = source(h) + col;
+        ra[u] = *reinterpret_cast<const R*>(src);
+        rb[u] = *reinterpret_cast<const R*>(src + p.pairs);
       }
     }
   };
-  load(my_row);  // in flight while the table is computed
+  load(h0);  // in flight while the table is computed
 
+  // positions and frequencies first, so that the table waits for memory once and not for every entry
+  for (int i = threadIdx.x; i < p.axes * ntok; i += kThreads) {
+    const int a = i / ntok;
+    int64_t tb, ts;
+    split(p, tok0 + (i - a * ntok), tb, ts);
+    pos_s[i] = load_pos(p, a * p.ps_a + tb * p.ps_b + ts * p.ps_s);
+  }
+  for (int j = threadIdx.x; j < p.pairs; j += kThreads) {
+    // frequency / 2pi as a sum of two doubles, so that the fraction of a turn is right for every position below 2^53
+    const double f = (double)p.inv_freq[j], c = f * kInv2PiHi;
+    freq_s[j] = make_double2(c, fma(f, kInv2PiHi, -c) + f * kInv2PiLo);
+    axis_s[j] = p.axis[j] * ntok;  // neighbouring pairs read different words of the parameters: slow, so once a pair
+  }
+  __syncthreads();
   for (int i = threadIdx.x; i < ntok * p.pairs; i += kThreads) {
-    const int t = i / p.pairs, j = i - t * p.pairs;
-    const int64_t tok = tok0 + t;
-    const int64_t b = tok / p.S, s = tok - b * p.S;
-    const double pos = load_pos(p, p.axis[j] * p.ps_a + b * p.ps_b + s * p.ps_s);
-    const double f = (double)p.inv_freq[j];
-    // f / 2pi as a sum of two doubles, so that the fraction of a turn is right for every position below 2^53
-    const double c = f * kInv2PiHi, c_low = fma(f, kInv2PiHi, -c) + f * kInv2PiLo;
-    const double t_high = pos * c;
-    const float rest = (float)((t_high - rint(t_high)) + (fma(pos, c, -t_high) + pos * c_low));
-    float sn, cs;
-    sincospif(2.0f * rest, &sn, &cs);
-    cosv[i] = cs;
-    sinv[i] = sn * p.sign;
+    const int ti = (int)((unsigned)i / (unsigned)p.pairs), j = i - ti * p.pairs;
+    const double pos = pos_s[axis_s[j] + ti];
+    const double2 c = freq_s[j];
+    const double high = pos * c.x;
+    const float left = (float)((high - rint(high)) + (fma(pos, c.x, -high) + pos * c.y));
+    float sine, cosine;
+    sincospif(2.0f * left, &sine, &cosine);
+    // vectors of 8 are kept as two planes of four, so that neighbouring threads' reads do not share banks
+    const int at = V == 8 ? ti * p.pairs + (j >> 2 & 1) * (p.pairs / 2) + (j >> 3) * 4 + (j & 3) : i;
+    cosv[at] = cosine;
+    sinv[at] = sine * p.sign;
   }
   __syncthreads();
 
-  for (unsigned base = my_row; base < rows; base += kUnroll * rows_per_step) {
+  // this vector's cosines and sines: read where they are used, four at a time, which costs fewer registers than it
+  // takes to keep a third block on the SM
+  constexpr int W = V < 4 ? V : 4;
+  const float* cs = cosv + t * p.pairs + (V == 8 ? col / 2 : col);
+  const float* sn = sinv + t * p.pairs + (V == 8 ? col / 2 : col);
+  const int far = V == 8 ? p.pairs / 2 : 4;  // from the first four to the next
+  for (int first = h0; first < h_end; first += kUnroll * p.group) {
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-      const unsigned r = base + u * rows_per_step;
-      if (active && r < rows) {
-        const T* src;
-        T* dst;
-        int t;
-        locate(r, src, dst, t);
-        const float* cs = cosv + t * p.pairs + col;
-        const float* sn = sinv + t * p.pairs + col;
-        const T* a = reinterpret_cast<const T*>(&ra[u]);
-        const T* b = reinterpret_cast<const T*>(&rb[u]);
+      const int h = first + u * p.group;
+      if (active && h < h_end) {
+        const T* xa = reinterpret_cast<const T*>(&ra[u]);
+        const T* xb = reinterpret_cast<const T*>(&rb[u]);
         R oa, ob;
-        T* pa = reinterpret_cast<T*>(&oa);
-        T* pb = reinterpret_cast<T*>(&ob);
+        float fa[V], fb[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float x = Cvt<T>::to_f(a[i]), y = Cvt<T>::to_f(b[i]);
-          pa[i] = Cvt<T>::from_f(x * cs[i] - y * sn[i]);
-          pb[i] = Cvt<T>::from_f(y * cs[i] + x * sn[i]);
+        for (int w = 0; w < V; w += W) {
+          float c[W], d[W];
+          if constexpr (W == 4) {
+            *reinterpret_cast<float4*>(c) = *reinterpret_cast<const float4*>(cs + w / 4 * far);
+            *reinterpret_cast<float4*>(d) = *reinterpret_cast<const float4*>(sn + w / 4 * far);
+          } else {
+#pragma unroll
+            for (int i = 0; i < W; ++i) c[i] = cs[w + i], d[i] = sn[w + i];
+          }
+#pragma unroll
+          for (int i = 0; i < W; ++i) {
+            const float x = Cvt<T>::to_f(xa[w + i]), y = Cvt<T>::to_f(xb[w + i]);
+            fa[w + i] = x * c[i] - y * d[i];
+            fb[w + i] = y * c[i] + x * d[i];
+          }
         }
-        *reinterpret_cast<R*>(dst + col) = oa;
-        *reinterpret_cast<R*>(dst + col + p.pairs) = ob;
+        round_n<T, V>(fa, reinterpret_cast<T*>(&oa));
+        round_n<T, V>(fb, reinterpret_cast<T*>(&ob));
+        T* dst = target(h) + col;
+        *reinterpret_cast<R*>(dst) = oa;
+        *reinterpret_cast<R*>(dst + p.pairs) = ob;
       }
     }
-    load(base + kUnroll * rows_per_step);
+    load(first + kUnroll * p.group);
   }
 
-  // columns that are not rotated
-  const int rest = (p.D - 2 * p.pairs) / V;
-  for (int64_t i = threadIdx.x; i < (int64_t)rows * rest; i += kThreads) {
-    const unsigned r = (unsigned)(i / rest);
-    const int c = 2 * p.pairs + (int)(i - (int64_t)r * rest) * V;
-    const T* src;
-    T* dst;
-    int t;
-    locate(r, src, dst, t);
-    *reinterpret_cast<R*>(dst + c) = *reinterpret_cast<const R*>(src + c);
+  // columns that are not rotated: the token's threads take them vector by vector, head by head
+  const int extra = (p.D - 2 * p.pairs) / V;
+  if (active && extra > 0) {
+    const int hb = (int)blockIdx.y * p.group * p.heads_each;
+    const int nh = heads - hb < p.group * p.heads_each ? heads - hb : p.group * p.heads_each;
+    const int mine = (int)threadIdx.x - t * p.group * vecs;
+    for (int64_t i = mine; i < (int64_t)nh * extra; i += p.group * vecs) {
+      const int h = hb + (int)(i / extra), c = 2 * p.pairs + (int)(i % extra) * V;
+      *reinterpret_cast<R*>(target(h) + c) = *reinterpret_cast<const R*>(source(h) + c);
+    }
   }
 }
 
@@ -182,25 +214,33 @@ int vector_width(const AxesArgs& p, int elem) {
 
 template <typename T, int V>
 int launch_v(AxesArgs& p, cudaStream_t st) {
-  const int heads = p.q.heads + p.k.heads;
-  // Tokens per block: about kItemsPerThread vectors a thread, within the table.  The heads are split over
-  // blocks only where the tokens alone leave SMs idle.
-  const int64_t per_token = (int64_t)heads * (p.pairs / V);
-  int64_t tpb = ((int64_t)kThreads * kItemsPerThread + per_token - 1) / per_token;
+  const int heads = p.q.heads + p.k.heads, vecs = p.pairs / V;
+  const int most = kThreads / vecs;  // heads at a time
+  // Heads to a thread: as many as leave three blocks to each SM, at most kMostHeads (the cosines and sines are then
+  // computed once for many; a call of few tokens has one head to a thread and waits on latency alone).  From that
+  // down to half of it, the number that leaves the fewest threads of a block idle.
+  const double work = (double)p.n_tokens * vecs * heads / ((double)kThreads * 3 * num_sms());
+  int n = work < 1 ? 1 : work > kMostHeads ? kMostHeads : (int)work;
+  if (n > heads) n = heads;
+  int group = most < heads ? most : heads, each = n;  // where a block has no room for all the heads of a token
+  double best = 0;
+  for (int m = n; m >= 1 && 2 * m >= n; --m) {
+    const int g = (heads + m - 1) / m;
+    if (g > most) break;
+    const double full = (double)(kThreads / (vecs * g)) * vecs * heads / ((double)kThreads * m);
+    if (full > best) best = full, group = g, each = m;
+  }
+  int tpb = kThreads / (vecs * group);
   if (tpb > kTableMax / p.pairs) tpb = kTableMax / p.pairs;
-  const int64_t spread = (p.n_tokens + num_sms() - 1) / num_sms();
-  if (tpb > spread) tpb = spread;
-  if (tpb < 1) tpb = 1;
+  if (tpb > kPosMax / p.axes) tpb = kPosMax / p.axes;
+  if (tpb > p.n_tokens) tpb = (int)p.n_tokens;
+  const int64_t parts = (heads + (int64_t)group * each - 1) / ((int64_t)group * each);
   const int64_t blocks = (p.n_tokens + tpb - 1) / tpb;
-  if (blocks > 0x7fffffff) return fail(ATS_EUNSUPPORTED, "rope_axes: too many tokens");
-  int64_t parts = (num_sms() + blocks - 1) / blocks;
-  if (parts > heads) parts = heads;
-  p.tokens_per_block = (int)tpb;
-  p.heads_per_block = (int)((heads + parts - 1) / parts);
-  const unsigned gy = (unsigned)((heads + p.heads_per_block - 1) / p.heads_per_block);
-  if (gy > 65535) return fail(ATS_EUNSUPPORTED, "rope_axes: too many heads");
-  const size_t smem = (size_t)tpb * p.pairs * 2 * sizeof(float);
-  rope_axes_kernel<T, V><<<dim3((unsigned)blocks, gy), kThreads, smem, st>>>(p);
+  if (blocks > 0x7fffffff || parts > 65535) return fail(ATS_EUNSUPPORTED, "rope_axes: too many tokens or heads");
+  p.tokens_per_block = tpb, p.group = group, p.heads_each = each;
+  const size_t smem = (size_t)p.pairs * sizeof(double2) + (size_t)(tpb * p.axes + 1) / 2 * 16 +
+                      (size_t)(2 * tpb + 1) * p.pairs * sizeof(float);
+  rope_axes_kernel<T, V><<<dim3((unsigned)blocks, (unsigned)parts), kThreads, smem, st>>>(p);
   return check_launch("rope_axes_apply");
 }
 
@@ -247,6 +287,7 @@ extern "C" int ats_rope_axes_apply(const void* q_in, void* q_out, int64_t Hq, co
   p.S = S;
   p.D = (int)D;
   p.pairs = pairs;
+  p.axes = axes;
   p.sign = backward != 0 ? -1.0f : 1.0f;
   for (int j = 0; j < pairs; ++j) p.axis[j] = axis_of_pair[j];
   cudaStream_t st = (cudaStream_t)stream;

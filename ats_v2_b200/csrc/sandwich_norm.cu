@@ -180,9 +180,7 @@ struct Mine {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       R raw;
-      T* e = reinterpret_cast<T*>(&raw);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) e[i] = Cvt<T>::from_f(v[j * VEC + i]);
+      round_n<T, VEC>(v + j * VEC, reinterpret_cast<T*>(&raw));
       if (has(j)) *reinterpret_cast<R*>(static_cast<T*>(base) + at + col(j)) = raw;
     }
   }
@@ -212,9 +210,7 @@ struct Mine {
 #pragma unroll
     for (int q = 0; q < BYTES / PIECE; ++q) {
       typename Raw<PIECE>::type raw;
-      U* e = reinterpret_cast<U*>(&raw);
-#pragma unroll
-      for (int i = 0; i < N; ++i) e[i] = Cvt<U>::from_f(v[q * N + i]);
+      round_n<U, N>(v + q * N, reinterpret_cast<U*>(&raw));
       reinterpret_cast<typename Raw<PIECE>::type*>(p)[q] = raw;
     }
   }
