@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import os
 import threading
 from ctypes import POINTER, c_char_p, c_float, c_int, c_int64, c_size_t, c_void_p
@@ -259,12 +260,14 @@ def gemm_pairs(enabled: bool):
         call("ats_set_gemm_pairs", prev)
 
 
+_DTYPE_CODES = {torch.float32: ATS_F32, torch.bfloat16: ATS_BF16}
+
+
 def dtype_code(t: torch.dtype) -> int:
-    if t == torch.float32:
-        return ATS_F32
-    if t == torch.bfloat16:
-        return ATS_BF16
-    raise TypeError(f"ats_v2_b200 kernels take float32 or bfloat16 tensors, got {t}")
+    code = _DTYPE_CODES.get(t)
+    if code is None:
+        raise TypeError(f"ats_v2_b200 kernels take float32 or bfloat16 tensors, got {t}")
+    return code
 
 
 def ptr(t: torch.Tensor | None) -> int | None:
@@ -284,6 +287,19 @@ def device_of(t: torch.Tensor):
     return _SAME_DEVICE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
+def once_differentiable(backward):
+    """torch.autograd.function.once_differentiable, applied only where the backward is itself
+    recorded (create_graph): otherwise nothing could be differentiated twice, and the wrapper
+    costs several microseconds a call."""
+    wrapped = torch.autograd.function.once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        return wrapped(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return run
+
+
 def strides3(*s: int):
     return _I64x3(*s)
 
@@ -297,9 +313,9 @@ def on_cpu(name: str, *tensors: torch.Tensor | None) -> bool:
     for CUDA tensors): CPU tensors take the reference's torch formulas, which
     its CPU tests pin, and CUDA tensors always take this library's kernels --
     a CUDA tensor never runs the torch formula, and a missing library raises."""
-    dev = next(t.device for t in tensors if t is not None)
-    if all(t is None or t.device == dev for t in tensors) and dev.type in ("cpu", "cuda"):  # the usual case
-        return dev.type == "cpu"
+    dev = next((t.device for t in tensors if t is not None), None)
+    if dev is not None and dev.type in ("cpu", "cuda") and all(t is None or t.device == dev for t in tensors):
+        return dev.type == "cpu"  # the usual case: all on one device
     devs = {t.device.type for t in tensors if t is not None}
     if devs == {"cpu"}:
         return True

@@ -646,7 +646,7 @@ struct BwdPlan {
 };
 
 // Blocks of a backward on an SM, at most: those of fewer columns are smaller, and their partial rows cost less.
-int64_t most_per_sm(int64_t H) { return H >= 4096 ? 2 : H <= 512 ? 16 : 8192 / H; }
+int64_t most_per_sm(int64_t H) { return H >= 4096 ? 2 : H <= 256 ? 32 : 8192 / H; }
 
 // Row ranges (units) of the backward, none across a span, for `per_sm` blocks on each SM, but 8 rows to a block before
 // a second one on an SM: a partial row is as many bytes as a row or more.
@@ -729,11 +729,11 @@ int set_smem(F kernel, int smem, const char* what) {
   return e == cudaSuccess ? ATS_OK : fail(ATS_ECUDA, "%s: %s", what, cudaGetErrorString(e));
 }
 
-// Blocks of `threads` threads and `smem` bytes that an SM holds, 1 to 16: `regs` registers a thread.
+// Blocks of `threads` threads and `smem` bytes that an SM holds, 1 to 32: `regs` registers a thread.
 int64_t resident(int regs, int threads, int smem) {
   const int64_t by_regs = 65536 / ((int64_t)(regs + 7) / 8 * 8 * threads), by_smem = 227 * 1024 / (smem + 1536);
   const int64_t n = by_regs < by_smem ? by_regs : by_smem;
-  return n < 1 ? 1 : n > 16 ? 16 : n;
+  return n < 1 ? 1 : n > 32 ? 32 : n;
 }
 
 template <auto KERNEL>

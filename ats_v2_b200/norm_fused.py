@@ -202,7 +202,7 @@ class _SandwichNormFn(torch.autograd.Function):
         return h, s
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_lib.once_differentiable
     def backward(ctx, dh, ds):
         if dh is None and ds is None:
             return (None,) * 8

@@ -223,7 +223,7 @@ class _MultiAxisRotaryFn(torch.autograd.Function):
         return q_out, k_out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_lib.once_differentiable
     def backward(ctx, dq_out, dk_out):
         positions, inv_freq = ctx.saved_tensors
         dq_out, dk_out = (_last_dim_contig(t) if t is not None else None for t in (dq_out, dk_out))

@@ -187,3 +187,12 @@ def test_other_stream_and_graph_replay():
     held = [t.clone() for t in held]
     for a, b in zip(held, once()):
         assert torch.equal(a, b)
+
+
+def test_second_derivatives_are_refused():
+    q, _, pos, inv, _, _ = make(1, 4, 2, 1, 32, (16,), "f32")
+    q.requires_grad_()
+    out, _ = apply_multi_axis_rotary(q, None, pos, inv, (16,))
+    (dq,) = torch.autograd.grad(out.square().sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        dq.sum().backward()

@@ -185,3 +185,12 @@ def test_other_stream_and_graph_replay():
     held = [t.clone() for t in held]
     for a, b in zip(held, once()):
         assert torch.equal(a, b)
+
+
+def test_second_derivatives_are_refused():
+    x, res, wp, wn, _, _, _ = make((2, 3, 64), "f32")
+    x.requires_grad_()
+    h, s = fused_sandwich_norm(x, res, wp, wn)
+    (dx,) = torch.autograd.grad(h.sum() + s.square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        dx.sum().backward()
