@@ -190,3 +190,36 @@ def test_modules():
     qat = QuantizedLinear(64, 32, "int8")
     served = Int8Linear.from_linear(qat).cuda()
     assert served(torch.randn(2, 64, device="cuda")).shape == (2, 32)
+
+
+def test_two_streams_at_once_and_fresh_weights():
+    """Calls on two streams, each right after its weights were written on that stream."""
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for M in (1, 24, 300, 2100):
+        data = [make(M, 1536, 1024, "bf16", True, seed=M + i) for i in range(2)]
+        want = [int8_linear(*d) for d in data]
+        torch.cuda.synchronize()
+        for _ in range(4):
+            got = []
+            for st, (x, w, s, b) in zip(streams, data):
+                with torch.cuda.stream(st):
+                    w2, s2, x2 = torch.empty_like(w), torch.empty_like(s), torch.empty_like(x)
+                    x2.copy_(x)
+                    s2.copy_(s)
+                    w2.copy_(w)  # the last thing before the product reads it
+                    got.append(int8_linear(x2, w2, s2, b))
+            torch.cuda.synchronize()
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_calls_in_a_row_do_not_meet():
+    """Each call's product starts before its quantisation has ended: a chain of calls on new inputs in reused memory."""
+    for M in (1, 12, 64, 500, 2200):
+        x, w, s, _ = make(M, 1024, 1024, "bf16")
+        w = torch.where(torch.rand(w.shape, device="cuda") < 0.1, w, torch.zeros_like(w))
+        chain = [x]
+        for _ in range(6):
+            chain.append(int8_linear(chain[-1], w, s))
+        for a, b in zip(chain, chain[1:]):
+            e, mag = int8_exact(a, w, s)
+            assert_within(b, e, INT8_SLACK * mag)

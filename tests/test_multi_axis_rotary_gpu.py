@@ -196,3 +196,37 @@ def test_second_derivatives_are_refused():
     (dq,) = torch.autograd.grad(out.square().sum(), q, create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable"):
         dq.sum().backward()
+
+
+def test_no_query_heads_and_many_heads():
+    g = torch.Generator().manual_seed(6)
+    inv = (1.0 / 100.0 ** (torch.arange(8).float() / 8)).cuda()
+    pos = torch.randint(0, 99, (2, 2, 3), generator=g).cuda()
+    turn = turns_exact(pos, inv, axis_of_pairs((4, 4)))
+    for Hq, Hk in ((0, 3), (3, 0), (0, 0), (700, 1), (1, 300)):
+        q, k = (torch.randn(2, n, 3, 20, generator=g).cuda() for n in (Hq, Hk))
+        qo, ko = apply_multi_axis_rotary(q, k, pos, inv, (4, 4))
+        assert_within(qo, rotate_exact(q, turn), rotate_slack(q, 8))
+        assert_within(ko, rotate_exact(k, turn), rotate_slack(k, 8))
+
+
+def test_many_axes():
+    g = torch.Generator().manual_seed(7)
+    n = 64
+    inv = (1.0 / 100.0 ** (torch.arange(n).float() / n)).cuda()
+    pos = torch.randint(0, 99, (n, 3, 50), generator=g).cuda()
+    q = torch.randn(3, 2, 50, 2 * n, generator=g).cuda()
+    for interleaved in (False, True):
+        qo, _ = apply_multi_axis_rotary(q, None, pos, inv, (1,) * n, interleaved)
+        turn = turns_exact(pos, inv, axis_of_pairs((1,) * n, interleaved))
+        assert_within(qo, rotate_exact(q, turn), rotate_slack(q, n))
+
+
+def test_every_head_and_token_count_has_its_heads_once():
+    """The launch splits heads and tokens by rules on their numbers: small grids of both."""
+    for Hq, Hk, D, secs in ((1, 1, 64, (32,)), (5, 2, 96, (16, 16)), (33, 8, 128, (64,)), (7, 0, 12, (3, 1))):
+        for S in (1, 2, 15, 148, 400, 1500):
+            check(1, S, Hq, Hk, D, secs, "bf16", seed=S) if Hk else None
+            q, _, pos, inv, _, _ = make(1, S, Hq, 1, D, secs, "f32", seed=S + 1)
+            qo, _ = apply_multi_axis_rotary(q, None, pos, inv, secs)
+            assert_within(qo, rotate_exact(q, turns_exact(pos, inv, axis_of_pairs(secs))), rotate_slack(q, sum(secs)))

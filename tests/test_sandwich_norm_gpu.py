@@ -194,3 +194,73 @@ def test_second_derivatives_are_refused():
     (dx,) = torch.autograd.grad(h.sum() + s.square().sum(), x, create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable"):
         dx.sum().backward()
+
+
+@pytest.mark.parametrize("gate", ["channel", "sequence", "token"])
+@pytest.mark.parametrize("xd,gd", [("bf16", "f32"), ("f32", "bf16")])
+@pytest.mark.parametrize("H", [192, 1030, 1033, 4096, 6144])
+def test_gates_of_another_type(H, xd, gd, gate):
+    """A gate in another type than the rows is read in other pieces than they are."""
+    x, res, wp, wn, gt, dh, ds = make((2, 9, H), xd, "f32", gate, seed=H)
+    gt = gt.to(TD[gd])
+    leaves = [t.requires_grad_() for t in (x, res, wp, wn, gt)]
+    out = fused_sandwich_norm(x, res, wp, wn, gate=gt, residual_scale=1.2, eps=1e-5)
+    got = torch.autograd.grad(out, leaves, (dh, ds))
+    assert got[4].dtype == gt.dtype
+    e = sandwich_exact(x, res, wp, wn, gt, 1.2, 1e-5, dh, ds)
+    for name, t in zip(("h", "s", "dx", "dres", "dwp", "dwn", "dgate"), (*out, *got)):
+        slack = sandwich_slack(H, 18 if name[:2] in ("dw", "dg") else 0)
+        assert_within(t.detach(), e[name][0], slack * e[name][1], f"{name} {H} {xd} {gd} {gate}")
+
+
+def test_views_that_start_anywhere():
+    """Weights and a gate cut from larger buffers at odd elements."""
+    H = 264
+    x, res, wp, wn, gt, dh, ds = make((3, 8, H), "bf16", "f32", "token")
+    buf = torch.empty(2 * H + 3, device="cuda")
+    buf[1:H + 1], buf[H + 2:2 * H + 2] = wp, wn
+    gbuf = torch.empty(gt.numel() + 1, dtype=gt.dtype, device="cuda")
+    gbuf[1:] = gt.reshape(-1)
+    ins = [t.requires_grad_() for t in (x, res, buf[1:H + 1], buf[H + 2:2 * H + 2], gbuf[1:].view_as(gt))]
+    out = fused_sandwich_norm(*ins[:4], gate=ins[4])
+    got = torch.autograd.grad(out, ins, (dh, ds))
+    same = [t.detach().requires_grad_() for t in (x, res, wp, wn, gt)]
+    want_out = fused_sandwich_norm(*same[:4], gate=same[4])
+    want = torch.autograd.grad(want_out, same, (dh, ds))
+    for a, b in zip((*out, *got), (*want_out, *want)):
+        assert torch.equal(a, b)
+
+
+def test_one_tensor_in_several_places():
+    """x as its own residual and one weight for both norms: the gradients add up."""
+    x, _, w, _, _, dh, ds = make((2, 5, 128), "f32")
+    x.requires_grad_()
+    w.requires_grad_()
+    out = fused_sandwich_norm(x, x, w, w, residual_scale=0.5)
+    dx, dw = torch.autograd.grad(out, (x, w), (dh, ds))
+    e = sandwich_exact(x, x, w, w, None, 0.5, 1e-6, dh, ds)
+    k = sandwich_slack(128, 10)
+    assert_within(dx, e["dx"][0] + e["dres"][0], 2 * k * (e["dx"][1] + e["dres"][1]))
+    assert_within(dw, e["dwp"][0] + e["dwn"][0], 2 * k * (e["dwp"][1] + e["dwn"][1]))
+
+
+def test_two_streams_at_once():
+    ins = [make((2, 700, 1024), "bf16", "f32", "sequence", seed=i) for i in range(2)]
+    streams = [torch.cuda.Stream() for _ in ins]
+
+    def once(i):
+        x, res, wp, wn, gt, dh, ds = ins[i]
+        leaves = [t.requires_grad_() for t in (x, res, wp, wn, gt)]
+        out = fused_sandwich_norm(x, res, wp, wn, gate=gt)
+        return [o.detach() for o in out] + list(torch.autograd.grad(out, leaves, (dh, ds)))
+
+    want = [once(i) for i in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got.append(once(i))
+        torch.cuda.synchronize()
+        for a, b in zip(want[0] + want[1], got[0] + got[1]):
+            assert torch.equal(a, b)
