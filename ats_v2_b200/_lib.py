@@ -313,9 +313,16 @@ def on_cpu(name: str, *tensors: torch.Tensor | None) -> bool:
     for CUDA tensors): CPU tensors take the reference's torch formulas, which
     its CPU tests pin, and CUDA tensors always take this library's kernels --
     a CUDA tensor never runs the torch formula, and a missing library raises."""
-    dev = next((t.device for t in tensors if t is not None), None)
-    if dev is not None and dev.type in ("cpu", "cuda") and all(t is None or t.device == dev for t in tensors):
-        return dev.type == "cpu"  # the usual case: all on one device
+    dev = None
+    for t in tensors:
+        if t is not None:
+            if dev is None:
+                dev = t.device
+            elif t.device != dev:
+                break
+    else:
+        if dev is not None and dev.type in ("cpu", "cuda"):  # the usual case: all on one device
+            return dev.type == "cpu"
     devs = {t.device.type for t in tensors if t is not None}
     if devs == {"cpu"}:
         return True

@@ -7,6 +7,8 @@
 #include <stdio.h>
 #include <stdarg.h>
 
+#include <atomic>
+
 #include "../../include/ats_b200.h"
 
 namespace ats {
@@ -58,6 +60,26 @@ int int8_take_status(int* code);
 int ep_take_status(int* code);
 int gemm_ctas();  // CTAs of a persistent GEMM: num_sms() or this thread's lower limit
 bool gemm_pairs();  // expert / dense / MLA GEMMs on CTA pairs (ats_set_gemm_pairs)
+
+// Once per kernel and device: let KERNEL use all the dynamic shared memory that its static part leaves and, with
+// `carve`, prefer the largest shared-memory split of an SM (kernels that follow one another with different splits make
+// the SM drain first).
+template <auto KERNEL>
+inline int allow_smem(const char* what, bool carve = false) {
+  static std::atomic<uint64_t> done{0};  // a bit per device
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && dev >= 0 && dev < 64 && (done.load(std::memory_order_relaxed) >> dev & 1)) return ATS_OK;
+  cudaFuncAttributes a;
+  if (e == cudaSuccess) e = cudaFuncGetAttributes(&a, KERNEL);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - (int)a.sharedSizeBytes);
+  if (e == cudaSuccess && carve)
+    e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+  if (e != cudaSuccess) return fail(ATS_ECUDA, "%s: %s", what, cudaGetErrorString(e));
+  if (dev >= 0 && dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+  return ATS_OK;
+}
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 

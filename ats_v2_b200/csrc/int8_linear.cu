@@ -13,6 +13,7 @@
 #include <cudaTypedefs.h>
 
 #include <mutex>
+#include <type_traits>
 
 #include "common.cuh"
 #include "tc_ptx.cuh"
@@ -181,15 +182,9 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G) int8_quantize_kernel(const 
 
 // Launch whose prologue may start before the stream's previous kernel has ended (every kernel here waits for it with
 // wait_prerequisites), in clusters of CTAs.
-template <typename F, typename... A>
-int launch_after(F kernel, dim3 grid, int threads, int smem, dim3 cluster, cudaStream_t st, const char* what,
-                 A... args) {
-  // All with one shared-memory split: an SM that has to change it between two kernels first drains.
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
-                                       cudaSharedmemCarveoutMaxShared);
-  if (e == cudaSuccess && smem > 48 * 1024)
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return fail(ATS_ECUDA, "%s: %s", what, cudaGetErrorString(e));
+template <auto KERNEL, typename... A>
+int launch_after(dim3 grid, int threads, int smem, dim3 cluster, cudaStream_t st, const char* what, A... args) {
+  ATS_TRY(allow_smem<KERNEL>(what, true));
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -204,7 +199,7 @@ int launch_after(F kernel, dim3 grid, int threads, int smem, dim3 cluster, cudaS
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = cluster.x * cluster.y * cluster.z > 1 ? 2 : 1;
-  e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, KERNEL, args...);
   if (e != cudaSuccess) return fail(ATS_ECUDA, "%s: %s", what, cudaGetErrorString(e));
   return check_launch(what);
 }
@@ -215,11 +210,12 @@ int quantize_g(const T* x, int64_t ldx, int8_t* q, int64_t ldq, float* scale, in
   constexpr int THREADS = G < 128 ? 128 : G;
   const int64_t per = THREADS / G;
   const unsigned grid = (unsigned)((rows + per - 1) / per);
-  auto go = [&](auto kernel) {
-    return launch_after(kernel, dim3(grid), THREADS, 0, dim3(1), st, "int8_quantize", x, ldx, q, ldq, scale, rows, K);
+  auto go = [&](auto by_vec, auto by_16) {
+    return launch_after<int8_quantize_kernel<T, G, by_vec.value, by_16.value>>(
+        dim3(grid), THREADS, 0, dim3(1), st, "int8_quantize", x, ldx, q, ldq, scale, rows, K);
   };
-  if (vec) return q16 ? go(int8_quantize_kernel<T, G, true, true>) : go(int8_quantize_kernel<T, G, true, false>);
-  return q16 ? go(int8_quantize_kernel<T, G, false, true>) : go(int8_quantize_kernel<T, G, false, false>);
+  if (vec) return q16 ? go(std::true_type{}, std::true_type{}) : go(std::true_type{}, std::false_type{});
+  return q16 ? go(std::false_type{}, std::true_type{}) : go(std::false_type{}, std::false_type{});
 }
 
 // As many threads as hold the row in their registers: 32, 128 or 512 (8192x2048 bf16: 9.0 us with a warp a row,
@@ -852,13 +848,13 @@ int dot(const void* x, const int8_t* w, int64_t ldw, const Out& o, int K, cudaSt
   const int warps = kDotThreads / 32;
   const int64_t want = (o.N + warps - 1) / warps, cap = (int64_t)num_sms() * 4;
   const unsigned grid = (unsigned)(want < cap ? want : cap);
-  return launch_after(int8_dot_kernel<T>, dim3(grid), kDotThreads, (int)padded_k(K), dim3(1), st, "int8_dot",
+  return launch_after<int8_dot_kernel<T>>(dim3(grid), kDotThreads, (int)padded_k(K), dim3(1), st, "int8_dot",
                       static_cast<const T*>(x), w, ldw, o, K, aligned16(x) ? 1 : 0);
 }
 
 // Pairs of CTAs that are resident at once on the current device.
-template <typename F>
-int pairs_that_fit(F kernel, int smem, int* out) {
+template <auto KERNEL>
+int pairs_that_fit(int smem, int* out) {
   static thread_local int fit[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return fail(ATS_ECUDA, "int8_tile: no current device");
@@ -874,9 +870,9 @@ int pairs_that_fit(F kernel, int smem, int* out) {
     cfg.dynamicSmemBytes = (size_t)smem;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    ATS_TRY(allow_smem<KERNEL>("int8_tile", true));
     int n = 0;
-    if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
+    const cudaError_t e = cudaOccupancyMaxActiveClusters(&n, KERNEL, &cfg);
     if (e != cudaSuccess || n < 1) return fail(ATS_ECUDA, "int8_tile: no pair fits (%s)", cudaGetErrorString(e));
     fit[dev] = n;
   }
@@ -886,7 +882,6 @@ int pairs_that_fit(F kernel, int smem, int* out) {
 
 template <typename T>
 int tiles(const int8_t* q, int64_t ldq, const int8_t* w, int64_t ldw, const Out& o, int K, cudaStream_t st) {
-  auto kernel = int8_tile_kernel<T>;
   CUtensorMap ma, mb;
   ATS_TRY(operand_map(&ma, q, K, o.M, ldq, BM));
   ATS_TRY(operand_map(&mb, w, K, o.N, ldw, B_ROWS));
@@ -896,11 +891,11 @@ int tiles(const int8_t* q, int64_t ldq, const int8_t* w, int64_t ldw, const Out&
   if (total > 0x7fffffff - 4096) return fail(ATS_EUNSUPPORTED, "int8_linear: too many tiles");
   const int smem = 1024 + kTileStages * kTileStage + kEpiWarps * kBox;
   int pairs = 0;
-  ATS_TRY(pairs_that_fit(kernel, smem, &pairs));
+  ATS_TRY(pairs_that_fit<int8_tile_kernel<T>>(smem, &pairs));
   if (pairs > gemm_ctas() / 2) pairs = gemm_ctas() / 2;
   if (pairs > total) pairs = (int)total;
   if (pairs < 1) pairs = 1;
-  return launch_after(kernel, dim3(2 * (unsigned)pairs), kTileThreads, smem, dim3(2), st, "int8_tile", ma, mb, p);
+  return launch_after<int8_tile_kernel<T>>(dim3(2 * (unsigned)pairs), kTileThreads, smem, dim3(2), st, "int8_tile", ma, mb, p);
 }
 
 template <typename T, int TN>
@@ -910,7 +905,7 @@ int parts(const int8_t* q, int64_t ldq, const int8_t* w, int64_t ldw, const Out&
   ATS_TRY(operand_map(&mx, q, K, o.M, ldq, TN));
   const dim3 grid((unsigned)((o.N + BM - 1) / BM), (unsigned)((o.M + TN - 1) / TN), (unsigned)split);
   const int smem = 1024 + part_stages(TN) * part_stage_bytes(TN);
-  return launch_after(int8_part_kernel<T, TN>, grid, kPartThreads, smem, dim3(1, 1, (unsigned)split), st, "int8_part", mw, mx, o,
+  return launch_after<int8_part_kernel<T, TN>>(grid, kPartThreads, smem, dim3(1, 1, (unsigned)split), st, "int8_part", mw, mx, o,
                       (K + BKB - 1) / BKB, o.N % 4 == 0 && aligned16(o.y) ? 1 : 0);
 }
 

@@ -723,12 +723,6 @@ uintptr_t row_bits(const NormArgs& p) {
   return bits(p.x) | bits(p.res) | (other % 16 != 0 ? 1 : 0);
 }
 
-template <typename F>
-int set_smem(F kernel, int smem, const char* what) {
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  return e == cudaSuccess ? ATS_OK : fail(ATS_ECUDA, "%s: %s", what, cudaGetErrorString(e));
-}
-
 // Blocks of `threads` threads and `smem` bytes that an SM holds, 1 to 32: `regs` registers a thread.
 int64_t resident(int regs, int threads, int smem) {
   const int64_t by_regs = 65536 / ((int64_t)(regs + 7) / 8 * 8 * threads), by_smem = 227 * 1024 / (smem + 1536);
@@ -761,7 +755,7 @@ int fwd_t(const NormArgs& p, int gate, cudaStream_t st) {
       using M = Mine<T, vb.value, nv.value, g.value>;
       constexpr auto kernel = sandwich_fwd_kernel<T, vb.value, nv.value, g.value>;
       const int t = row_threads(p.H, M::VEC, nv.value), smem = M::smem(t, 2, stages_of<M>(2));
-      ATS_TRY(set_smem(kernel, smem, "sandwich_norm_fwd"));
+      ATS_TRY(allow_smem<kernel>("sandwich_norm_fwd"));
       const int64_t cap = num_sms() * resident(regs_of<kernel>(), t, smem);
       kernel<<<(unsigned)(p.rows < cap ? p.rows : cap), t, smem, st>>>(p);
       return check_launch("sandwich_norm_fwd");
@@ -790,7 +784,7 @@ int bwd_t(NormArgs p, int gate, float* workspace, void* dw_post, void* dw_pre, c
       using M = Mine<T, vb.value, nv.value, g.value>;
       constexpr auto kernel = sandwich_bwd_kernel<T, vb.value, nv.value, g.value>;
       const int t = row_threads(p.H, M::VEC, nv.value), smem = M::smem(t, 4, stages_of<M>(4));
-      ATS_TRY(set_smem(kernel, smem, "sandwich_norm_bwd"));
+      ATS_TRY(allow_smem<kernel>("sandwich_norm_bwd"));
       plan(resident(regs_of<kernel>(), t, smem));
       kernel<<<(unsigned)b.blocks, t, smem, st>>>(p);
       return check_launch("sandwich_norm_bwd");

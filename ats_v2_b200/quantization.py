@@ -83,7 +83,7 @@ def _torch_quantize_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
     """x [..., features] as rows whose elements are consecutive."""
-    x = x.reshape(-1, x.shape[-1])
+    x = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     return x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous()
 
 
