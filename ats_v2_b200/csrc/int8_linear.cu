@@ -49,9 +49,10 @@ __device__ __forceinline__ float row_scale(uint32_t bits, float& inv) {
   return amax / 127.0f;
 }
 
-__device__ __forceinline__ int quant(float v, float inv) {
-  const float r = rintf(v * inv);
-  return r == r ? (int)fminf(fmaxf(r, -127.f), 127.f) : 0;
+// rint(v * inv) as a byte, for |v * inv| below 2^22: adding 1.5 * 2^23 rounds to the nearest integer, ties to even, and
+// leaves it in the low bits.  |v| <= amax keeps |v * inv| within 127 (1 + 2^-22), which rounds to at most 127.
+__device__ __forceinline__ uint32_t quant(float v, float inv) {
+  return __float_as_uint(__fadd_rn(__fmul_rn(v, inv), 12582912.0f));
 }
 
 // 16 consecutive values of a row from element k, as they are stored; those at or past K are zero.
@@ -69,17 +70,27 @@ __device__ __forceinline__ void load16(const T* row, int k, int K, uint4 (&v)[si
   }
 }
 
+// The largest |value|'s bits of 16; bf16 two at a time, as the high halves of float32.
 template <typename T>
 __device__ __forceinline__ uint32_t max16(const uint4 (&v)[sizeof(T)], uint32_t m) {
-  const T* e = reinterpret_cast<const T*>(v);
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(v);
+  if constexpr (sizeof(T) == 2) {
+    uint32_t two = 0;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) m = max(m, abs_bits(Cvt<T>::to_f(e[i])));
-  return m;
+    for (int i = 0; i < 8; ++i) two = __vmaxu2(two, w[i] & 0x7fff7fffu);
+    return max(m, max(two << 16, two & 0xffff0000u));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) m = max(m, w[i] & 0x7fffffffu);
+    return m;
+  }
 }
 
+// Four bytes; zeros for a row without a finite scale (inv is 0).
 __device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d, float inv) {
-  return (uint32_t)(quant(a, inv) & 255) | (uint32_t)(quant(b, inv) & 255) << 8 |
-         (uint32_t)(quant(c, inv) & 255) << 16 | (uint32_t)(quant(d, inv) & 255) << 24;
+  const uint32_t lo = __byte_perm(quant(a, inv), quant(b, inv), 0x0040);
+  const uint32_t hi = __byte_perm(quant(c, inv), quant(d, inv), 0x0040);
+  return inv != 0.f ? __byte_perm(lo, hi, 0x5410) : 0u;
 }
 
 template <typename T>
