@@ -14,6 +14,11 @@ the reference's ``ats/model`` interfaces:
     ats/model/ffn.py          -> ats_v2_b200.ffn         (SwiGLU)
     ats/model/mla_triton.py   -> ats_v2_b200.mla_fused   (fused_mla_kv_decompress)
 
+Beside them, operators the reference does not have: ``norm_fused.fused_sandwich_norm`` (the norms
+on both sides of a block with its gate and residual scale), ``rope.apply_multi_axis_rotary`` and
+``rope.MultiAxisRotaryEmbedding`` (positions with several axes), ``quantization.int8_linear`` and
+``quantization.Int8Linear`` (the 8-bit integer projection).
+
 All compute runs on CUDA tensors; CPU tensors raise.
 """
 

