@@ -13,7 +13,7 @@
 // sines once into shared memory, so that work is spread over the heads; each
 // thread reads those of its vector there and streams heads past them.  Every element is read once and
 // written once; HBM bounds it: q [4,32,4096,128] and k [4,8,4096,128] bf16 take
-// 60 us a direction, 85% of the measured copy bandwidth (94 us with one thread
+// 58 us a direction, 88% of the measured copy bandwidth (94 us with one thread
 // per vector and head, which spent its time on indices).
 #include "common.cuh"
 
@@ -21,7 +21,9 @@ namespace ats {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kUnroll = 4;       // heads in flight per thread
+// Heads in flight per thread: with 64 registers a thread, 3 of 16 bytes in each half (2: 59 us for the q and k above,
+// 4: 60 us, spilling) or 8 of fewer.
+template <typename T, int V> struct Unroll { static constexpr int value = V * (int)sizeof(T) == 16 ? 3 : 8; };
 constexpr int kMostHeads = 8;    // heads a thread handles
 constexpr double kInv2PiHi = 0.15915494309189535, kInv2PiLo = -9.839338337591243e-18;  // 1 / (2 pi) in two parts
 constexpr int kTableMax = 2048;  // cosine/sine entries of a block (16 KB)
@@ -42,6 +44,7 @@ struct AxesArgs {
   const float* inv_freq;
   int64_t n_tokens, S;
   int D, pairs, axes;
+  int rest_vec;  // elements per access of the copied columns
   int tokens_per_block, group, heads_each;  // `group` threads share a token's heads, heads_each to each
   float sign;  // of the sine: +1 forward, -1 adjoint
   uint8_t axis[ATS_ROPE_MAX_PAIRS];
@@ -69,8 +72,9 @@ __device__ __forceinline__ double load_pos(const AxesArgs& p, int64_t i) {
 
 // A thread owns one vector position of the pairs of one token and heads_each heads, `group` apart; consecutive threads
 // take consecutive vectors of a head's row.
-template <typename T, int V>
-__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 3) rope_axes_kernel(const __grid_constant__ AxesArgs p) {
+template <typename T, int V, bool REST>  // REST: there are columns to copy
+__global__ void __launch_bounds__(kThreads, 4) rope_axes_kernel(const __grid_constant__ AxesArgs p) {
+  constexpr int kUnroll = Unroll<T, V>::value;
   using R = typename Raw<V * (int)sizeof(T)>::type;
   // frequencies [pairs], positions [axes][tokens], cosines [tokens][pairs], sines, axes [pairs]
   extern __shared__ __align__(16) double2 freq_s[];
@@ -186,23 +190,33 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 3) rope_axes_ke
     load(first + kUnroll * p.group);
   }
 
-  // columns that are not rotated: the token's threads take them vector by vector, head by head
-  const int extra = (p.D - 2 * p.pairs) / V;
-  if (active && extra > 0) {
+  // columns that are not rotated, `rest_vec` elements at a time, shared by the token's threads
+  if (REST && active) {
     const int hb = (int)blockIdx.y * p.group * p.heads_each;
     const int nh = heads - hb < p.group * p.heads_each ? heads - hb : p.group * p.heads_each;
-    const int mine = (int)threadIdx.x - t * p.group * vecs;
-    for (int64_t i = mine; i < (int64_t)nh * extra; i += p.group * vecs) {
-      const int h = hb + (int)(i / extra), c = 2 * p.pairs + (int)(i % extra) * V;
-      *reinterpret_cast<R*>(target(h) + c) = *reinterpret_cast<const R*>(source(h) + c);
-    }
+    const unsigned extra = (unsigned)((p.D - 2 * p.pairs) / p.rest_vec);
+    const unsigned team = (unsigned)(p.group * vecs);
+    const unsigned total = (unsigned)nh * extra;  // at most 256 * kMostHeads heads of 2^20 columns
+    auto copy = [&](auto raw) {
+      using C = decltype(raw);
+      for (unsigned i = threadIdx.x - (unsigned)t * team; i < total; i += team) {
+        const unsigned r = i / extra, c = i - r * extra;
+        reinterpret_cast<C*>(target(hb + (int)r) + 2 * p.pairs)[c] =
+            reinterpret_cast<const C*>(source(hb + (int)r) + 2 * p.pairs)[c];
+      }
+    };
+    const int bytes = p.rest_vec * (int)sizeof(T);
+    if (bytes == 16) copy(uint4{});
+    else if (bytes == 8) copy(uint2{});
+    else if (bytes == 4) copy(uint32_t{});
+    else copy(uint16_t{});
   }
 }
 
-// Elements one access may move: the largest power of two (at most 16 bytes) that divides the pairs, the copied
-// columns and every stride, and to which every pointer is aligned.
-int vector_width(const AxesArgs& p, int elem) {
-  int64_t bits = p.pairs | (p.D - 2 * p.pairs);
+// Elements one access may move: the largest power of two (at most 16 bytes) that divides `cols` and every stride, and
+// to which every pointer is aligned.
+int vector_width(const AxesArgs& p, int64_t cols, int elem) {
+  int64_t bits = cols;
   uintptr_t addr = 0;
   for (const AxesTensor* t : {&p.q, &p.k}) {
     if (t->heads == 0) continue;
@@ -242,7 +256,9 @@ int launch_v(AxesArgs& p, cudaStream_t st) {
   p.tokens_per_block = tpb, p.group = group, p.heads_each = each;
   const size_t smem = (size_t)p.pairs * sizeof(double2) + (size_t)(tpb * p.axes + 1) / 2 * 16 +
                       (size_t)(2 * tpb + 1) * p.pairs * sizeof(float);
-  rope_axes_kernel<T, V><<<dim3((unsigned)blocks, (unsigned)parts), kThreads, smem, st>>>(p);
+  const dim3 grid((unsigned)blocks, (unsigned)parts);
+  if (p.D > 2 * p.pairs) rope_axes_kernel<T, V, true><<<grid, kThreads, smem, st>>>(p);
+  else rope_axes_kernel<T, V, false><<<grid, kThreads, smem, st>>>(p);
   return check_launch("rope_axes_apply");
 }
 
@@ -293,15 +309,16 @@ extern "C" int ats_rope_axes_apply(const void* q_in, void* q_out, int64_t Hq, co
   p.sign = backward != 0 ? -1.0f : 1.0f;
   for (int j = 0; j < pairs; ++j) p.axis[j] = axis_of_pair[j];
   cudaStream_t st = (cudaStream_t)stream;
+  p.rest_vec = vector_width(p, 2 * (int64_t)pairs | (D - 2 * (int64_t)pairs), x_dtype == ATS_BF16 ? 2 : 4);
   if (x_dtype == ATS_BF16) {
-    switch (vector_width(p, 2)) {
+    switch (vector_width(p, pairs, 2)) {
       case 8: return launch_v<bf16, 8>(p, st);
       case 4: return launch_v<bf16, 4>(p, st);
       case 2: return launch_v<bf16, 2>(p, st);
       default: return launch_v<bf16, 1>(p, st);
     }
   }
-  switch (vector_width(p, 4)) {
+  switch (vector_width(p, pairs, 4)) {
     case 4: return launch_v<float, 4>(p, st);
     case 2: return launch_v<float, 2>(p, st);
     default: return launch_v<float, 1>(p, st);

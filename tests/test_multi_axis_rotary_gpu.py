@@ -230,3 +230,9 @@ def test_every_head_and_token_count_has_its_heads_once():
             q, _, pos, inv, _, _ = make(1, S, Hq, 1, D, secs, "f32", seed=S + 1)
             qo, _ = apply_multi_axis_rotary(q, None, pos, inv, secs)
             assert_within(qo, rotate_exact(q, turns_exact(pos, inv, axis_of_pairs(secs))), rotate_slack(q, sum(secs)))
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("D,pairs", [(96, 7), (80, 29), (190, 93), (100, 2), (67, 33), (130, 65), (77, 20), (48, 16)])
+def test_pairs_and_copied_columns_of_every_alignment(D, pairs, dt):
+    check(2, 37, 5, 3, D, (pairs,), dt, seed=D)
