@@ -13,7 +13,7 @@
 // sines once into shared memory, so that work is spread over the heads; each
 // thread reads those of its vector there and streams heads past them.  Every element is read once and
 // written once; HBM bounds it: q [4,32,4096,128] and k [4,8,4096,128] bf16 take
-// 58 us a direction, 88% of the measured copy bandwidth (94 us with one thread
+// 53 us a direction, 97% of the measured copy bandwidth (94 us with one thread
 // per vector and head, which spent its time on indices).
 #include "common.cuh"
 
@@ -21,10 +21,12 @@ namespace ats {
 namespace {
 
 constexpr int kThreads = 256;
-// Heads in flight per thread: with 64 registers a thread, 3 of 16 bytes in each half (2: 59 us for the q and k above,
-// 4: 60 us, spilling) or 8 of fewer.
-template <typename T, int V> struct Unroll { static constexpr int value = V * (int)sizeof(T) == 16 ? 3 : 8; };
-constexpr int kMostHeads = 8;    // heads a thread handles
+// Heads in flight per thread: 3 where a head is 16 bytes in each half, so that 64 registers hold them (2: 55 us for the
+// q and k above, 4: 56 us), else 4 (8 heads of 93 pairs in each of 21,244 tokens: 84 us; 2: 95 us, 3: 90 us).
+template <typename T, int V> struct Unroll { static constexpr int value = V * (int)sizeof(T) == 16 ? 3 : 4; };
+// Heads a thread handles: 16 of narrow vectors, to make up for the cost of a table (24 heads of 40 columns, 5514 tokens:
+// 20 us, with 8: 26 us), 8 of 16 bytes (the q and k above: 53 us, with 16: 55 us).
+template <typename T, int V> struct MostHeads { static constexpr int value = V * (int)sizeof(T) == 16 ? 8 : 16; };
 constexpr double kInv2PiHi = 0.15915494309189535, kInv2PiLo = -9.839338337591243e-18;  // 1 / (2 pi) in two parts
 constexpr int kTableMax = 2048;  // cosine/sine entries of a block (16 KB)
 constexpr int kPosMax = 1024;    // positions of a block (8 KB)
@@ -34,6 +36,7 @@ struct AxesTensor {
   void* out;
   int heads;
   int64_t is_b, is_h, is_s, os_b, os_h, os_s;  // strides in elements
+  int64_t i_step, o_step;  // from a thread's head to its next one
 };
 
 struct AxesArgs {
@@ -46,6 +49,7 @@ struct AxesArgs {
   int D, pairs, axes;
   int rest_vec;  // elements per access of the copied columns
   int tokens_per_block, group, heads_each;  // `group` threads share a token's heads, heads_each to each
+  unsigned by_vecs, by_group, by_pairs;  // for quotient()
   float sign;  // of the sine: +1 forward, -1 adjoint
   uint8_t axis[ATS_ROPE_MAX_PAIRS];
 };
@@ -56,6 +60,9 @@ __device__ __forceinline__ void split(const AxesArgs& p, int64_t tok, int64_t& b
   else b = tok / p.S;
   s = tok - b * p.S;
 }
+
+// i / d for i <= 2048 and d <= 256, where m = 2^20 / d + 1: m d exceeds 2^20 by at most d, and i d < 2^20.
+__device__ __forceinline__ int quotient(int i, unsigned m) { return (int)((unsigned)i * m >> 20); }
 
 // V consecutive elements of T moved as one access.
 template <int BYTES> struct Raw;
@@ -87,34 +94,37 @@ __global__ void __launch_bounds__(kThreads, 4) rope_axes_kernel(const __grid_con
   int* axis_s = reinterpret_cast<int*>(sinv + p.tokens_per_block * p.pairs);  // [pairs] first position of the pair's axis
 
   const int vecs = p.pairs / V;
-  const int rest = (int)threadIdx.x / vecs, col = ((int)threadIdx.x - rest * vecs) * V;
-  const int t = rest / p.group;
+  const int rest = quotient(threadIdx.x, p.by_vecs), col = ((int)threadIdx.x - rest * vecs) * V;
+  const int t = quotient(rest, p.by_group);
   const int h0 = (int)blockIdx.y * p.group * p.heads_each + (rest - t * p.group);
   const bool active = t < ntok;
-  // where head h of this thread's token begins: q's heads, then k's
+  // where the heads of this thread's token begin: q's, then k's
   int64_t b, s;
   split(p, tok0 + (active ? t : 0), b, s);
   const T* qi = static_cast<const T*>(p.q.in) + b * p.q.is_b + s * p.q.is_s;
-  const T* ki = static_cast<const T*>(p.k.in) + b * p.k.is_b + s * p.k.is_s;
+  const T* ki = static_cast<const T*>(p.k.in) + b * p.k.is_b + s * p.k.is_s - p.q.heads * p.k.is_h;
   T* qo = static_cast<T*>(p.q.out) + b * p.q.os_b + s * p.q.os_s;
-  T* ko = static_cast<T*>(p.k.out) + b * p.k.os_b + s * p.k.os_s;
-  auto source = [&](int h) {
-    return h < p.q.heads ? qi + h * p.q.is_h : ki + (h - p.q.heads) * p.k.is_h;
-  };
-  auto target = [&](int h) {
-    return h < p.q.heads ? qo + h * p.q.os_h : ko + (h - p.q.heads) * p.k.os_h;
-  };
-  const int h_end = h0 + p.group * p.heads_each < heads ? h0 + p.group * p.heads_each : heads;
+  T* ko = static_cast<T*>(p.k.out) + b * p.k.os_b + s * p.k.os_s - p.q.heads * p.k.os_h;
+  auto source = [&](int h) { return h < p.q.heads ? qi + h * p.q.is_h : ki + h * p.k.is_h; };
+  auto target = [&](int h) { return h < p.q.heads ? qo + h * p.q.os_h : ko + h * p.k.os_h; };
+  const int h_end = !active ? 0 : h0 + p.group * p.heads_each < heads ? h0 + p.group * p.heads_each : heads;
+  // the heads one after the other by steps, from q over to k once: an address costs a few additions, where a product
+  // for each head took most of the time of narrow vectors
+  const int k0 = h0 < p.q.heads ? h0 + (p.q.heads - h0 + p.group - 1) / p.group * p.group : h0;  // first of k
+  const T* src = source(h0) + col;
+  T* dst = target(h0) + col;
+  const T* src_k = ki + k0 * p.k.is_h + col;
+  T* dst_k = ko + k0 * p.k.os_h + col;
   R ra[kUnroll], rb[kUnroll];
   auto load = [&](int first) {
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
       const int h = first + u * p.group;
-      if (active && h < h_end) {
-        const T* src = source(h) + col;
+      if (h < h_end) {
         ra[u] = *reinterpret_cast<const R*>(src);
         rb[u] = *reinterpret_cast<const R*>(src + p.pairs);
       }
+      src = h + p.group == k0 ? src_k : src + (h < p.q.heads ? p.q.i_step : p.k.i_step);
     }
   };
   load(h0);  // in flight while the table is computed
@@ -134,7 +144,7 @@ __global__ void __launch_bounds__(kThreads, 4) rope_axes_kernel(const __grid_con
   }
   __syncthreads();
   for (int i = threadIdx.x; i < ntok * p.pairs; i += kThreads) {
-    const int ti = (int)((unsigned)i / (unsigned)p.pairs), j = i - ti * p.pairs;
+    const int ti = quotient(i, p.by_pairs), j = i - ti * p.pairs;
     const double pos = pos_s[axis_s[j] + ti];
     const double2 c = freq_s[j];
     const double high = pos * c.x;
@@ -148,8 +158,8 @@ __global__ void __launch_bounds__(kThreads, 4) rope_axes_kernel(const __grid_con
   }
   __syncthreads();
 
-  // this vector's cosines and sines: read where they are used, four at a time, which costs fewer registers than it
-  // takes to keep a third block on the SM
+  // this vector's cosines and sines: read where they are used, four at a time, which leaves registers for a fourth
+  // block on the SM
   constexpr int W = V < 4 ? V : 4;
   const float* cs = cosv + t * p.pairs + (V == 8 ? col / 2 : col);
   const float* sn = sinv + t * p.pairs + (V == 8 ? col / 2 : col);
@@ -158,7 +168,7 @@ __global__ void __launch_bounds__(kThreads, 4) rope_axes_kernel(const __grid_con
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
       const int h = first + u * p.group;
-      if (active && h < h_end) {
+      if (h < h_end) {
         const T* xa = reinterpret_cast<const T*>(&ra[u]);
         const T* xb = reinterpret_cast<const T*>(&rb[u]);
         R oa, ob;
@@ -182,12 +192,12 @@ __global__ void __launch_bounds__(kThreads, 4) rope_axes_kernel(const __grid_con
         }
         round_n<T, V>(fa, reinterpret_cast<T*>(&oa));
         round_n<T, V>(fb, reinterpret_cast<T*>(&ob));
-        T* dst = target(h) + col;
         *reinterpret_cast<R*>(dst) = oa;
         *reinterpret_cast<R*>(dst + p.pairs) = ob;
       }
+      dst = h + p.group == k0 ? dst_k : dst + (h < p.q.heads ? p.q.o_step : p.k.o_step);
     }
-    load(first + kUnroll * p.group);
+    if (first + kUnroll * p.group < h_end) load(first + kUnroll * p.group);
   }
 
   // columns that are not rotated, `rest_vec` elements at a time, shared by the token's threads
@@ -196,7 +206,7 @@ __global__ void __launch_bounds__(kThreads, 4) rope_axes_kernel(const __grid_con
     const int nh = heads - hb < p.group * p.heads_each ? heads - hb : p.group * p.heads_each;
     const unsigned extra = (unsigned)((p.D - 2 * p.pairs) / p.rest_vec);
     const unsigned team = (unsigned)(p.group * vecs);
-    const unsigned total = (unsigned)nh * extra;  // at most 256 * kMostHeads heads of 2^20 columns
+    const unsigned total = (unsigned)nh * extra;  // at most 2^30
     auto copy = [&](auto raw) {
       using C = decltype(raw);
       for (unsigned i = threadIdx.x - (unsigned)t * team; i < total; i += team) {
@@ -236,8 +246,11 @@ int launch_v(AxesArgs& p, cudaStream_t st) {
   // computed once for many; a call of few tokens has one head to a thread and waits on latency alone).  From that
   // down to half of it, the number that leaves the fewest threads of a block idle.
   const double work = (double)p.n_tokens * vecs * heads / ((double)kThreads * 3 * num_sms());
+  constexpr int kMostHeads = MostHeads<T, V>::value;
   int n = work < 1 ? 1 : work > kMostHeads ? kMostHeads : (int)work;
   if (n > heads) n = heads;
+  const int64_t copied = (int64_t)most * (p.D - 2 * p.pairs);  // of a head to each thread: at most 2^28
+  if (copied > 0 && n > (1 << 30) / copied) n = (int)((1 << 30) / copied);  // a block counts them in 32 bits
   int group = most < heads ? most : heads, each = n;  // where a block has no room for all the heads of a token
   double best = 0;
   for (int m = n; m >= 1 && 2 * m >= n; --m) {
@@ -254,6 +267,9 @@ int launch_v(AxesArgs& p, cudaStream_t st) {
   const int64_t blocks = (p.n_tokens + tpb - 1) / tpb;
   if (blocks > 0x7fffffff || parts > 65535) return fail(ATS_EUNSUPPORTED, "rope_axes: too many tokens or heads");
   p.tokens_per_block = tpb, p.group = group, p.heads_each = each;
+  for (AxesTensor* t : {&p.q, &p.k}) t->i_step = group * t->is_h, t->o_step = group * t->os_h;
+  auto inverse = [](int d) { return (1u << 20) / (unsigned)d + 1; };
+  p.by_vecs = inverse(vecs), p.by_group = inverse(group), p.by_pairs = inverse(p.pairs);
   const size_t smem = (size_t)p.pairs * sizeof(double2) + (size_t)(tpb * p.axes + 1) / 2 * 16 +
                       (size_t)(2 * tpb + 1) * p.pairs * sizeof(float);
   const dim3 grid((unsigned)blocks, (unsigned)parts);
