@@ -83,7 +83,7 @@ template <> struct Raw<2> { using type = uint16_t; };
 // Copy BYTES, or zeros where `there` is false, without a branch (one for every vector would serialise a row).
 template <int BYTES>
 __device__ __forceinline__ void copy_ahead(void* dst, const void* src, bool there) {
-  if constexpr (BYTES == 2) {  // cp.async moves 4, 8 or 16 bytes
+  if constexpr (BYTES == 2) {  // a gate's single bf16: cp.async moves 4, 8 or 16 bytes
     const uint16_t v = *static_cast<const uint16_t*>(src);
     *static_cast<uint16_t*>(dst) = there ? v : (uint16_t)0;
   } else if constexpr (BYTES == 32) {
@@ -104,27 +104,32 @@ __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_grou
 constexpr int kRowThreads = 512;  // most threads of a row block
 
 // One thread's part of the rows.
-template <typename T, int VB, int NV, int GATE>
+template <typename T, int VB, int NV, int GATE, int TENSORS>
 struct Mine {
   static constexpr int VEC = VB / (int)sizeof(T), EPT = NV * VEC;
   static_assert(EPT % 4 == 0, "whole float4s of columns");
+  // cp.async moves 4 bytes at least.  Single bf16 are loaded into registers instead, a row ahead (4096 x 4095: forward
+  // 49 us, backward 103 us; stored into the ring, which waits for every load, 62 and 132 us).
+  static constexpr bool HELD = VB == 2;
+  static constexpr int N_TENSORS = TENSORS;
   static constexpr int ROW = NV * VB;  // bytes of a row of T
   // a gate row streams beside the others, in room for float32, where a thread has few enough columns
   static constexpr bool STREAM_GATE = GATE == 2 && EPT <= 8;
-  static constexpr int BLOCKS = ROW <= 16 && GATE != 2 ? 2 : 1;  // on an SM
+  static constexpr int BLOCKS = ROW <= (HELD ? 8 : 16) && GATE != 2 ? 2 : 1;  // on an SM
   static constexpr int COLS = GATE == 2 && !STREAM_GATE ? 3 : 2;  // sets of columns kept
   using R = typename Raw<VB>::type;
   int nthr, tid, nvec;
   char* ring;
   float4* cols;
   int stage_bytes;
-  __device__ __forceinline__ Mine(int H, char* smem, int tensors, int stages)
+  mutable uint16_t held[HELD ? TENSORS : 1][HELD ? NV : 1];
+  __device__ __forceinline__ Mine(int H, char* smem, int stages)
       : nthr((int)blockDim.x), tid((int)threadIdx.x), nvec(H / VEC), ring(smem) {
-    stage_bytes = nthr * (tensors * ROW + (STREAM_GATE ? EPT * 4 : 0));
+    stage_bytes = nthr * ((HELD ? 0 : TENSORS * ROW) + (STREAM_GATE ? EPT * 4 : 0));
     cols = reinterpret_cast<float4*>(smem + stages * stage_bytes) + tid;
   }
-  static __host__ constexpr int smem(int threads, int tensors, int stages) {
-    return threads * (stages * (tensors * ROW + (STREAM_GATE ? EPT * 4 : 0)) + COLS * EPT * 4);
+  static __host__ constexpr int smem(int threads, int stages) {
+    return threads * (stages * ((HELD ? 0 : TENSORS * ROW) + (STREAM_GATE ? EPT * 4 : 0)) + COLS * EPT * 4);
   }
   __device__ __forceinline__ bool has(int j) const { return tid + j * nthr < nvec; }
   __device__ __forceinline__ int col(int j) const { return (tid + j * nthr) * VEC; }
@@ -135,34 +140,40 @@ struct Mine {
   }
   __device__ __forceinline__ void ahead(int st, int t, const void* base, int64_t at) const {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) copy_ahead<VB>(slot(st, t, j), static_cast<const T*>(base) + at + safe(j), has(j));
+    for (int j = 0; j < NV; ++j) {
+      const T* src = static_cast<const T*>(base) + at + safe(j);
+      if constexpr (HELD) held[t][j] = *reinterpret_cast<const uint16_t*>(src);
+      else copy_ahead<VB>(slot(st, t, j), src, has(j));
+    }
   }
   __device__ __forceinline__ void take(int st, int t, float (&v)[EPT]) const {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const R raw = *reinterpret_cast<const R*>(slot(st, t, j));
+      R raw;
+      if constexpr (HELD) raw = has(j) ? held[t][j] : (uint16_t)0;
+      else raw = *reinterpret_cast<const R*>(slot(st, t, j));
       const T* e = reinterpret_cast<const T*>(&raw);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) v[j * VEC + i] = Cvt<T>::to_f(e[i]);
     }
   }
   // the streamed gate: behind the `tensors` row tensors of a stage
-  __device__ __forceinline__ char* gate_slot(int st, int tensors, int j) const {
-    return ring + st * stage_bytes + tensors * ROW * nthr + (j * nthr + tid) * VEC * 4;
+  __device__ __forceinline__ char* gate_slot(int st, int j) const {
+    return ring + st * stage_bytes + (HELD ? 0 : TENSORS * ROW) * nthr + (j * nthr + tid) * VEC * 4;
   }
-  __device__ __forceinline__ void gate_ahead(int st, int tensors, const void* base, int64_t at, int is_bf16) const {
+  __device__ __forceinline__ void gate_ahead(int st, const void* base, int64_t at, int is_bf16) const {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      if (is_bf16) copy_ahead<VEC * 2>(gate_slot(st, tensors, j), static_cast<const bf16*>(base) + at + safe(j), has(j));
-      else copy_ahead<VEC * 4>(gate_slot(st, tensors, j), static_cast<const float*>(base) + at + safe(j), has(j));
+      if (is_bf16) copy_ahead<VEC * 2>(gate_slot(st, j), static_cast<const bf16*>(base) + at + safe(j), has(j));
+      else copy_ahead<VEC * 4>(gate_slot(st, j), static_cast<const float*>(base) + at + safe(j), has(j));
     }
   }
-  __device__ __forceinline__ void gate_take(int st, int tensors, int is_bf16, float (&v)[EPT]) const {
+  __device__ __forceinline__ void gate_take(int st, int is_bf16, float (&v)[EPT]) const {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       float t[VEC];
-      if (is_bf16) load_vec<bf16>(reinterpret_cast<const bf16*>(gate_slot(st, tensors, j)), t);
-      else load_vec<float>(reinterpret_cast<const float*>(gate_slot(st, tensors, j)), t);
+      if (is_bf16) load_vec<bf16>(reinterpret_cast<const bf16*>(gate_slot(st, j)), t);
+      else load_vec<float>(reinterpret_cast<const float*>(gate_slot(st, j)), t);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) v[j * VEC + i] = t[i];
     }
@@ -233,8 +244,9 @@ struct Mine {
 
 // Rows in flight: 64 KB of them for 512 threads where two such blocks share an SM, 128 KB for one alone, at most 4.
 template <typename M>
-__host__ __device__ constexpr int stages_of(int tensors) {
-  const int n = (M::BLOCKS == 2 ? 64 : 128) * 1024 / kRowThreads / (tensors * M::ROW + (M::STREAM_GATE ? M::EPT * 4 : 0));
+__host__ __device__ constexpr int stages_of() {
+  if (M::HELD) return 1;
+  const int n = (M::BLOCKS == 2 ? 64 : 128) * 1024 / kRowThreads / (M::N_TENSORS * M::ROW + (M::STREAM_GATE ? M::EPT * 4 : 0));
   return n >= 4 ? 4 : n >= 2 ? 2 : 1;
 }
 
@@ -270,19 +282,19 @@ __device__ __forceinline__ void keep_gate_post(const M& me, const NormArgs& p, b
 }
 
 template <typename T, int VB, int NV, int GATE>
-__global__ void __launch_bounds__(kRowThreads, Mine<T, VB, NV, GATE>::BLOCKS)
+__global__ void __launch_bounds__(kRowThreads, Mine<T, VB, NV, GATE, 2>::BLOCKS)
     sandwich_fwd_kernel(const __grid_constant__ NormArgs p) {
-  using M = Mine<T, VB, NV, GATE>;
-  constexpr int EPT = M::EPT, ST = stages_of<M>(2);
+  using M = Mine<T, VB, NV, GATE, 2>;
+  constexpr int EPT = M::EPT, ST = stages_of<M>();
   extern __shared__ __align__(16) char smem[];
   __shared__ float4 red[2][kRowThreads / 128];
-  const M me(p.H, smem, 2, ST);
+  const M me(p.H, smem, ST);
   const int64_t r0 = p.rows * blockIdx.x / gridDim.x, r1 = p.rows * (blockIdx.x + 1) / gridDim.x;
   auto ahead = [&](int64_t row, int st) {
     if (row < r1) {
       me.ahead(st, 0, p.x, row * p.H);
       me.ahead(st, 1, p.res, row * p.H);
-      if constexpr (M::STREAM_GATE) me.gate_ahead(st, 2, p.gate, row * p.H, p.gate_bf16);
+      if constexpr (M::STREAM_GATE) me.gate_ahead(st, p.gate, row * p.H, p.gate_bf16);
     }
     copies_commit();
   };
@@ -309,7 +321,7 @@ __global__ void __launch_bounds__(kRowThreads, Mine<T, VB, NV, GATE>::BLOCKS)
     float x[EPT], s[EPT];
     me.take(st, 0, x);
     me.take(st, 1, s);
-    if constexpr (M::STREAM_GATE) me.gate_take(st, 2, p.gate_bf16, g);
+    if constexpr (M::STREAM_GATE) me.gate_take(st, p.gate_bf16, g);
     ahead(row + ST, st);
     if (++st == ST) st = 0;
     float ss = 0.f;
@@ -342,13 +354,13 @@ __global__ void __launch_bounds__(kRowThreads, Mine<T, VB, NV, GATE>::BLOCKS)
 }
 
 template <typename T, int VB, int NV, int GATE>
-__global__ void __launch_bounds__(kRowThreads, Mine<T, VB, NV, GATE>::BLOCKS)
+__global__ void __launch_bounds__(kRowThreads, Mine<T, VB, NV, GATE, 4>::BLOCKS)
     sandwich_bwd_kernel(const __grid_constant__ NormArgs p) {
-  using M = Mine<T, VB, NV, GATE>;
-  constexpr int EPT = M::EPT, ST = stages_of<M>(4);
+  using M = Mine<T, VB, NV, GATE, 4>;
+  constexpr int EPT = M::EPT, ST = stages_of<M>();
   extern __shared__ __align__(16) char smem[];
   __shared__ float4 red[2][kRowThreads / 128];
-  const M me(p.H, smem, 4, ST);
+  const M me(p.H, smem, ST);
   tc::launch_dependents();  // the sums' kernel may be brought up; it waits for this one
   // consecutive units (row ranges inside one span): their rows are consecutive too
   const int64_t u0 = p.units * blockIdx.x / gridDim.x, u1 = p.units * (blockIdx.x + 1) / gridDim.x;
@@ -364,7 +376,7 @@ __global__ void __launch_bounds__(kRowThreads, Mine<T, VB, NV, GATE>::BLOCKS)
       me.ahead(st, 1, p.res, row * p.H);
       if (has_dh) me.ahead(st, 2, p.dh, row * p.H);
       if (has_ds) me.ahead(st, 3, p.ds, row * p.H);
-      if constexpr (M::STREAM_GATE) me.gate_ahead(st, 4, p.gate, row * p.H, p.gate_bf16);
+      if constexpr (M::STREAM_GATE) me.gate_ahead(st, p.gate, row * p.H, p.gate_bf16);
     }
     copies_commit();
   };
@@ -399,7 +411,7 @@ __global__ void __launch_bounds__(kRowThreads, Mine<T, VB, NV, GATE>::BLOCKS)
       me.kept(COL_GATE_POST, w);
       if constexpr (GATE == GATE_ROW) {
         float g[EPT];
-        if constexpr (M::STREAM_GATE) me.gate_take(st, 4, p.gate_bf16, g);
+        if constexpr (M::STREAM_GATE) me.gate_take(st, p.gate_bf16, g);
         else me.kept(COL_GATE, g);
 #pragma unroll
         for (int i = 0; i < EPT; ++i) w[i] *= g[i];
@@ -451,7 +463,7 @@ __global__ void __launch_bounds__(kRowThreads, Mine<T, VB, NV, GATE>::BLOCKS)
 #pragma unroll
       for (int i = 0; i < EPT; ++i) out[i] = w[i] * (S[i] * xr[i]);
       me.put_as(p.dgate, at, p.gate_bf16, out);
-      if constexpr (M::STREAM_GATE) me.gate_take(st, 4, p.gate_bf16, w);
+      if constexpr (M::STREAM_GATE) me.gate_take(st, p.gate_bf16, w);
       else me.kept(COL_GATE, w);
 #pragma unroll
       for (int i = 0; i < EPT; ++i) A[i] = fmaf(w[i], S[i] * xr[i], A[i]);
@@ -650,12 +662,13 @@ struct BwdPlan {
 // Blocks of a backward on an SM, at most: those of fewer columns are smaller, and their partial rows cost less.
 int64_t most_per_sm(int64_t H) { return H >= 4096 ? 2 : H <= 256 ? 32 : 8192 / H; }
 
-// Row ranges (units) of the backward, none across a span, for `per_sm` blocks on each SM, but 8 rows to a block before
-// a second one on an SM: a partial row is as many bytes as a row or more.
+// Row ranges (units) of the backward, none across a span, for `per_sm` blocks on each SM, but 4 rows to a block before
+// a second one on an SM: a partial row is as many bytes as a row or more (1674 x 3000 bf16: 25.2 us, with 8 rows 29.9 us;
+// 2232 x 371: 12.4 and 14.5 us; 3087 x 64: 10.3 us, with 2 rows 12.0 us).
 BwdPlan bwd_plan(int64_t rows, int64_t span, int64_t per_sm) {
   BwdPlan b;
   const int64_t sms = num_sms();
-  int64_t want = rows / 8 < sms ? sms : rows / 8;
+  int64_t want = rows / 4 < sms ? sms : rows / 4;
   if (want > sms * per_sm) want = sms * per_sm;
   b.spans = rows / span;
   int64_t per = b.spans >= want ? 1 : want / b.spans;
@@ -705,7 +718,7 @@ bool pick_vectors(int64_t H, uintptr_t addr, F go) {
   }
   if constexpr (sizeof(T) == 2) {
     ATS_PICK(16, 1) ATS_PICK(16, 2) ATS_PICK(8, 1) ATS_PICK(8, 2) ATS_PICK(8, 4) ATS_PICK(4, 2) ATS_PICK(4, 8)
-    ATS_PICK(2, 4) ATS_PICK(2, 16)
+    ATS_PICK(2, 4) ATS_PICK(2, 8) ATS_PICK(2, 16)
   } else {
     ATS_PICK(16, 1) ATS_PICK(16, 2) ATS_PICK(16, 4) ATS_PICK(8, 2) ATS_PICK(8, 8) ATS_PICK(4, 4) ATS_PICK(4, 16)
   }
@@ -754,9 +767,9 @@ int fwd_t(const NormArgs& p, int gate, cudaStream_t st) {
   int rc = ATS_OK;
   const bool ok = pick_vectors<T>(p.H, row_bits(p) | bits(p.s) | bits(p.h), [&](auto vb, auto nv) {
     rc = by_gate(gate, [&](auto g) {
-      using M = Mine<T, vb.value, nv.value, g.value>;
+      using M = Mine<T, vb.value, nv.value, g.value, 2>;
       constexpr auto kernel = sandwich_fwd_kernel<T, vb.value, nv.value, g.value>;
-      const int t = row_threads(p.H, M::VEC, nv.value), smem = M::smem(t, 2, stages_of<M>(2));
+      const int t = row_threads(p.H, M::VEC, nv.value), smem = M::smem(t, stages_of<M>());
       ATS_TRY(allow_smem<kernel>("sandwich_norm_fwd"));
       const int64_t cap = num_sms() * resident(regs_of<kernel>(), t, smem);
       kernel<<<(unsigned)(p.rows < cap ? p.rows : cap), t, smem, st>>>(p);
@@ -783,9 +796,9 @@ int bwd_t(NormArgs p, int gate, float* workspace, void* dw_post, void* dw_pre, c
   const uintptr_t addr = row_bits(p) | bits(p.dh) | bits(p.ds) | bits(p.dx) | bits(p.dres);
   const bool ok = pick_vectors<T>(p.H, addr, [&](auto vb, auto nv) {
     rc = by_gate(gate, [&](auto g) {
-      using M = Mine<T, vb.value, nv.value, g.value>;
+      using M = Mine<T, vb.value, nv.value, g.value, 4>;
       constexpr auto kernel = sandwich_bwd_kernel<T, vb.value, nv.value, g.value>;
-      const int t = row_threads(p.H, M::VEC, nv.value), smem = M::smem(t, 4, stages_of<M>(4));
+      const int t = row_threads(p.H, M::VEC, nv.value), smem = M::smem(t, stages_of<M>());
       ATS_TRY(allow_smem<kernel>("sandwich_norm_bwd"));
       plan(resident(regs_of<kernel>(), t, smem));
       kernel<<<(unsigned)b.blocks, t, smem, st>>>(p);
