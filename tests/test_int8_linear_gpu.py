@@ -223,3 +223,22 @@ def test_calls_in_a_row_do_not_meet():
         for a, b in zip(chain, chain[1:]):
             e, mag = int8_exact(a, w, s)
             assert_within(b, e, INT8_SLACK * mag)
+
+
+@pytest.mark.parametrize("K", [1, 2, 15, 17, 18, 511, 512, 514, 2047, 2049, 2050, 8191, 8194, 33001, 33002, 33024])
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+def test_rows_of_every_alignment(K, dt):
+    """Rows that start at any element, read 16, 4 or 2 bytes at a time, from one warp to a row to longer ones than its
+    threads hold; the largest value, or what is not finite, at the end of a row, and values past it that do not count."""
+    rows = 5
+    g = torch.Generator().manual_seed(K)
+    for start, behind in ((0, 0), (1, 0), (2, 2), (0, 1), (8, 8), (3, 5)):
+        whole = torch.randn(rows, start + K + behind, generator=g).to(TD[dt])
+        whole[:, :start] = float("nan")
+        whole[:, start + K:] = float("inf")
+        whole[0, start + K - 1] = 50.0
+        whole[1, start + K - 1] = float("nan")
+        whole[2, start] = -50.0
+        q, s = quantize_int8(whole.cuda()[:, start:start + K])
+        qc, sc = quantize_int8(whole[:, start:start + K])
+        assert torch.equal(q.cpu(), qc) and torch.equal(s.cpu().nan_to_num(-1), sc.nan_to_num(-1))
