@@ -309,7 +309,9 @@ def once_differentiable(backward):
     return run
 
 
+@functools.lru_cache(maxsize=4096)
 def strides3(*s: int):
+    """Three strides as the library reads them; equal strides share one array, which nothing writes to."""
     return _I64x3(*s)
 
 
