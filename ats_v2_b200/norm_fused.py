@@ -179,7 +179,7 @@ def _sandwich_forward(x, residual, wp, wn, g, rows_per_gate, residual_scale, eps
     H = x.shape[-1]
     rows = x.numel() // H
     s, h = torch.empty_like(x), torch.empty_like(x)
-    rstd = torch.empty((2, rows), dtype=torch.float32, device=x.device) if train else None
+    rstd = x.new_empty((2, rows), dtype=torch.float32) if train else None
     p = rstd.data_ptr() if train else 0
     with _lib.device_of(x):
         _lib.call("ats_sandwich_norm_fwd", x.data_ptr(), residual.data_ptr(), _lib.dtype_code(x.dtype), wp.data_ptr(),
@@ -219,7 +219,7 @@ class _SandwichNormFn(torch.autograd.Function):
         dg = torch.empty_like(g) if g is not None else None
         with _lib.device_of(x):
             wsb = _lib.query("ats_sandwich_norm_bwd_workspace_bytes", rows, H, rows_per_gate if g is not None else 0)
-            ws = torch.empty(wsb, dtype=torch.uint8, device=x.device)
+            ws = x.new_empty(wsb, dtype=torch.uint8)
             _lib.call("ats_sandwich_norm_bwd", _lib.ptr(dh), _lib.ptr(ds), x.data_ptr(), r.data_ptr(),
                       _lib.dtype_code(x.dtype), wp.data_ptr(), wn.data_ptr(), _lib.dtype_code(wp.dtype), _lib.ptr(g),
                       _lib.dtype_code(g.dtype) if g is not None else 0, rows_per_gate, residual_scale,

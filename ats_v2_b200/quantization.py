@@ -106,8 +106,8 @@ def quantize_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         q[:, :K], scale = _torch_quantize_int8(x2)
     else:
         code = _lib.dtype_code(x.dtype)
-        q = torch.empty((x2.shape[0], Kp), dtype=torch.int8, device=x.device)
-        scale = torch.empty(x2.shape[0], dtype=torch.float32, device=x.device)
+        q = x2.new_empty((x2.shape[0], Kp), dtype=torch.int8)
+        scale = x2.new_empty(x2.shape[0], dtype=torch.float32)
         with _lib.device_of(x):
             _lib.call("ats_int8_quantize", x2.data_ptr(), x2.stride(0), code, q.data_ptr(), Kp, scale.data_ptr(),
                       x2.shape[0], K, _lib.stream_of(x))
@@ -155,10 +155,10 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor,
         weight = torch.empty((N, ldw), dtype=torch.int8, device=weight.device)[:, :K].copy_(weight)
     scale = scale.contiguous()
     bias = bias.contiguous() if bias is not None else None
-    y = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=x.device)
+    y = x.new_empty((*x.shape[:-1], N))
     with _lib.device_of(x):
         wsb = _lib.query("ats_int8_linear_workspace_bytes", M, N, K)
-        ws = torch.empty(wsb, dtype=torch.uint8, device=x.device) if wsb else None
+        ws = x.new_empty(wsb, dtype=torch.uint8) if wsb else None
         _lib.call("ats_int8_linear", x2.data_ptr(), x2.stride(0), code, weight.data_ptr(), ldw,
                   scale.data_ptr(), _lib.ptr(bias), bias_code, y.data_ptr(), M, N, K, _lib.ptr(ws), wsb,
                   _lib.stream_of(x))

@@ -263,7 +263,7 @@ def apply_multi_axis_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: 
                          f"got {tuple(q.shape)}.")
     B, _, S, D = q.shape
     if k is not None:
-        if k.dim() != 4 or k.shape[0] != B or k.shape[2:] != q.shape[2:]:
+        if k.dim() != 4 or (k.shape[0], k.shape[2], k.shape[3]) != (B, S, D):
             raise ValueError(f"apply_multi_axis_rotary: k shape {tuple(k.shape)} incompatible with q {tuple(q.shape)}.")
         if k.dtype != q.dtype:
             raise TypeError(f"apply_multi_axis_rotary: q and k must share a dtype ({q.dtype} vs {k.dtype})")
