@@ -236,3 +236,13 @@ def test_every_head_and_token_count_has_its_heads_once():
 @pytest.mark.parametrize("D,pairs", [(96, 7), (80, 29), (190, 93), (100, 2), (67, 33), (130, 65), (77, 20), (48, 16)])
 def test_pairs_and_copied_columns_of_every_alignment(D, pairs, dt):
     check(2, 37, 5, 3, D, (pairs,), dt, seed=D)
+
+
+@pytest.mark.parametrize("B,S,Hq,Hk,D,sections,dt", [
+    (2, 4096, 13, 3, 64, (32,), "bf16"), (1, 6001, 20, 5, 96, (12, 10, 10), "bf16"), (1, 9000, 24, 6, 34, (5, 12), "bf16"),
+    (3, 3000, 1, 17, 20, (1, 3), "bf16"), (1, 5000, 18, 1, 38, (19,), "f32"), (2, 2500, 7, 9, 128, (40, 24), "f32"),
+    (1, 700, 70, 70, 32, (7, 9), "bf16")])
+@pytest.mark.parametrize("layout", ["bshd", "bhsd"])
+def test_threads_that_walk_many_heads(B, S, Hq, Hk, D, sections, dt, layout):
+    """Enough tokens that a thread takes up to 16 heads one after the other, from q over to k."""
+    check(B, S, Hq, Hk, D, sections, dt, layout=layout, seed=Hq)

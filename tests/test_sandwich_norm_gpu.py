@@ -264,3 +264,15 @@ def test_two_streams_at_once():
         torch.cuda.synchronize()
         for a, b in zip(want[0] + want[1], got[0] + got[1]):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("H,rows", [(1, 9000), (363, 2500), (2509, 1200), (4097, 900), (6, 9000), (1030, 1500)])
+@pytest.mark.parametrize("gate", [None, "channel", "sequence", "token"])
+def test_odd_widths_over_many_rows(H, rows, gate):
+    """Several rows to a block in the narrow vectors: a row ahead in registers, or in the ring."""
+    check((4, rows // 4, H), "bf16", "f32", gate, seed=H)
+
+
+@pytest.mark.parametrize("only", ["h", "s"])
+def test_odd_width_with_one_result_unused(only):
+    check((2, 600, 519), "bf16", "bf16", "token", only=only)
