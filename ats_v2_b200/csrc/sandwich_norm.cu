@@ -83,7 +83,7 @@ template <> struct Raw<2> { using type = uint16_t; };
 // Copy BYTES, or zeros where `there` is false, without a branch (one for every vector would serialise a row).
 template <int BYTES>
 __device__ __forceinline__ void copy_ahead(void* dst, const void* src, bool there) {
-  if constexpr (BYTES == 2) {  // a gate's single bf16: cp.async moves 4, 8 or 16 bytes
+  if constexpr (BYTES == 2) {  // single bf16: cp.async moves 4, 8 or 16 bytes
     const uint16_t v = *static_cast<const uint16_t*>(src);
     *static_cast<uint16_t*>(dst) = there ? v : (uint16_t)0;
   } else if constexpr (BYTES == 32) {
@@ -108,14 +108,15 @@ template <typename T, int VB, int NV, int GATE, int TENSORS>
 struct Mine {
   static constexpr int VEC = VB / (int)sizeof(T), EPT = NV * VEC;
   static_assert(EPT % 4 == 0, "whole float4s of columns");
-  // cp.async moves 4 bytes at least.  Single bf16 are loaded into registers instead, a row ahead (4096 x 4095: forward
-  // 49 us, backward 103 us; stored into the ring, which waits for every load, 62 and 132 us).
-  static constexpr bool HELD = VB == 2;
+  // cp.async moves 4 bytes at least.  Single bf16 are loaded into registers instead, a row ahead, as far as there are
+  // registers for them (4096 x 4095: forward 49 us, backward 103 us; stored into the ring, which waits for every load,
+  // 62 and 132 us; 2048 x 6001, 64 values of a backward: 150 us in registers, 134 in the ring).
+  static constexpr bool HELD = VB == 2 && NV * TENSORS <= 32;
   static constexpr int N_TENSORS = TENSORS;
   static constexpr int ROW = NV * VB;  // bytes of a row of T
   // a gate row streams beside the others, in room for float32, where a thread has few enough columns
   static constexpr bool STREAM_GATE = GATE == 2 && EPT <= 8;
-  static constexpr int BLOCKS = ROW <= (HELD ? 8 : 16) && GATE != 2 ? 2 : 1;  // on an SM
+  static constexpr int BLOCKS = ROW <= (VB == 2 ? 8 : 16) && GATE != 2 ? 2 : 1;  // on an SM
   static constexpr int COLS = GATE == 2 && !STREAM_GATE ? 3 : 2;  // sets of columns kept
   using R = typename Raw<VB>::type;
   int nthr, tid, nvec;
