@@ -376,12 +376,14 @@ __global__ void __launch_bounds__(kDotThreads, 4) int8_dot_kernel(const T* __res
 // ------------------------------------------------- tensor cores, many tokens
 // tcgen05.mma kind::i8, K in blocks of 128 bytes, 256 tokens x 256 channels on a cluster of two CTAs (cta_group::2):
 // persistent, each CTA with a TMA producer warp and eight epilogue warps (two per TMEM lane quadrant, half of the
-// columns each) that scale, round and store whole 128-byte pieces of rows through a swizzled box in shared memory;
-// CTA 0's MMA warp issues for both, into two accumulators.  Each CTA loads its 128 tokens and half of the channels,
-// 32 KB a block where a single CTA of 128 x 256 loads 48: single CTAs were held by what L2 delivers to the SMs, about
-// 15 TB/s (8192^3: 440 us against 386 in pairs, both with an earlier quantisation; 370 us now).  All loads of a block count on CTA 0's full barrier; its commits reach
-// the empty and accumulator barriers of both; both epilogues release the accumulator on CTA 0.  A block takes 509 to
-// 544 SM cycles against the 512 of its MMAs, so the clock under the power limit bounds it.
+// columns each) that scale and round into a swizzled box of shared memory, 32 rows of 128 bytes, which a TMA store
+// empties beside the next box's arithmetic (8192 x 8192 x 512 bf16: 54 us, where filling the result with a constant
+// takes 35; with the box read back and stored by the warp 58).  CTA 0's MMA warp issues for both, into two
+// accumulators.  Each CTA loads its 128 tokens and half of the channels, 32 KB a block where a single CTA of 128 x 256
+// loads 48: single CTAs were held by what L2 delivers to the SMs, about 15 TB/s (8192^3: 440 us against 386 in pairs,
+// both with an earlier quantisation; 370 us now).  All loads of a block count on CTA 0's full barrier; its commits
+// reach the empty and accumulator barriers of both; both epilogues release the accumulator on CTA 0.  A block takes
+// 509 to 544 SM cycles against the 512 of its MMAs, so the clock under the power limit bounds it.
 constexpr int BM = 128, BKB = 128;
 constexpr int kEpiWarps = 8, kTileThreads = 64 + 32 * kEpiWarps;
 constexpr int kBox = 32 * 128;  // an epilogue warp's staging: 32 rows of 128 bytes
@@ -394,7 +396,8 @@ struct TileArgs {
   Out o;
   int kb;       // K blocks
   int mt, nt;   // tiles
-  int vec_out;  // rows of y are 16-byte multiples
+  int vec_out;   // rows of y are 16-byte multiples
+  int even_out;  // 4-byte multiples
 };
 
 // Tile t: bands of kBandM M tiles, M fastest inside a band, so that the CTAs that run together share weights and
@@ -410,6 +413,7 @@ __device__ __forceinline__ void tile_of(const TileArgs& p, int t, int& m, int& n
 template <typename T>
 __global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid_constant__ CUtensorMap tmA,
                                                                    const __grid_constant__ CUtensorMap tmB,
+                                                                   const __grid_constant__ CUtensorMap tmY,
                                                                    TileArgs p) {
   constexpr int STAGE = kTileStage, NST = kTileStages;
   constexpr uint32_t IDESC = tc::idesc_i8(TM, BN);
@@ -571,7 +575,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid
         uint32_t r[BOX_COLS];
 #pragma unroll
         for (int h = 0; h < BOX_COLS; h += 16) tc::tmem_ld16_async(t_row + c + h, r + h);
-        tc::tmem_ld_wait();
+        tc::tmem_ld_wait(r);
         if (c + BOX_COLS == BN / 2) {  // the accumulator is read: the next tile's products may start
           tc::tc_fence_before();
           __syncwarp();
@@ -588,6 +592,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid
 #pragma unroll
           for (int e = 0; e < BOX_COLS; ++e)
             v[e] = __fadd_rn(v[e], __shfl_sync(0xffffffffu, bw[(c + e) / 32], (c + e) % 32));
+        if (lane == 0) tc::bulk_wait_read<0>();  // the box's last store has read it
+        __syncwarp();
 #pragma unroll
         for (int q = 0; q < 8; ++q) {  // row `lane`, 16-byte piece q at its swizzled place (conflict-free)
           float u[Chunk<T>::N];
@@ -597,35 +603,33 @@ __global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid
           pack_chunk<T>(u, w);
           *reinterpret_cast<uint4*>(box + lane * 128 + ((q ^ (lane & 7)) << 4)) = w;
         }
-        __syncwarp();
-        if (p.vec_out) {  // 8 lanes write 128 bytes of a row
-          const int q = lane & 7, col = col0 + q * Chunk<T>::N;
-          uint4 w[8];
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const int rr = k * 4 + (lane >> 3);
-            w[k] = *reinterpret_cast<const uint4*>(box + rr * 128 + ((q ^ (rr & 7)) << 4));
+        if (p.vec_out) {
+          tc::fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0 && row0 < p.o.M && col0 < p.o.N) {
+            tc::tma_store_2d(&tmY, box, col0, row0);  // what lies past the last row or column is left out
+            tc::bulk_commit();
           }
-          if (col < p.o.N) {
-            T* y = static_cast<T*>(p.o.y) + (int64_t)(row0 + (lane >> 3)) * p.o.N + col;
+        } else {  // rows of y that are not 16-byte multiples: piece by piece, along the rows (8192 x 8190: 81 us)
+          __syncwarp();
+          auto store = [&](auto piece) {
+            using P = decltype(piece);
+#pragma unroll 8
+            for (int rr = 0; rr < 32; ++rr)
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-              if (row0 + k * 4 + (lane >> 3) < p.o.M) *reinterpret_cast<uint4*>(y + (int64_t)k * 4 * p.o.N) = w[k];
-          }
-        } else {  // rows of y that are not 16-byte multiples: element by element, along the rows
-#pragma unroll 1
-          for (int rr = 0; rr < 32 && row0 + rr < p.o.M; ++rr)
-#pragma unroll
-            for (int cc = lane; cc < BOX_COLS; cc += 32) {
-              const int byte = cc * (int)sizeof(T);
-              if (col0 + cc < p.o.N)
-                static_cast<T*>(p.o.y)[(int64_t)(row0 + rr) * p.o.N + col0 + cc] =
-                    *reinterpret_cast<const T*>(box + rr * 128 + (((byte >> 4) ^ (rr & 7)) << 4) + (byte & 15));
-            }
+              for (int byte = lane * (int)sizeof(P); byte < 128; byte += 32 * (int)sizeof(P)) {
+                const int col = col0 + byte / (int)sizeof(T);
+                const P w = *reinterpret_cast<const P*>(box + rr * 128 + (((byte >> 4) ^ (rr & 7)) << 4) + (byte & 15));
+                if (row0 + rr < p.o.M && col < p.o.N)
+                  *reinterpret_cast<P*>(static_cast<T*>(p.o.y) + (int64_t)(row0 + rr) * p.o.N + col) = w;
+              }
+          };
+          if (sizeof(T) == 4 || p.even_out) store(uint32_t{});
+          else store(uint16_t{});
         }
-        __syncwarp();
       }
     }
+    if (lane == 0) tc::bulk_wait<0>();  // every store is complete before the CTA exits
   }
   tc::tc_fence_before();
   __syncthreads();
@@ -871,8 +875,10 @@ size_t q_bytes(int64_t M, int64_t K) { return align_up((size_t)(M * padded_k(K))
 PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
 std::once_flag g_encode_once;
 
-// Operand of int8 rows: boxes of 128 bytes x `box_rows`, 128-byte swizzle; bytes past K and rows past the end read as 0.
-int operand_map(CUtensorMap* m, const void* base, int64_t K, int64_t rows, int64_t ld, int box_rows) {
+// Rows [rows, cols] of `es`-byte elements: boxes of 128 bytes x `box_rows`, 128-byte swizzle; what is loaded from past an
+// end is 0, what is stored there is left out.
+int row_map(CUtensorMap* m, CUtensorMapDataType type, int es, const void* base, int64_t cols, int64_t rows, int64_t ld,
+            int box_rows) {
   std::call_once(g_encode_once, [] {
     void* fn = nullptr;
     cudaDriverEntryPointQueryResult q;
@@ -881,15 +887,19 @@ int operand_map(CUtensorMap* m, const void* base, int64_t K, int64_t rows, int64
       g_encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
   });
   if (g_encode == nullptr) return fail(ATS_ECUDA, "int8_linear: cuTensorMapEncodeTiled unavailable");
-  cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
-  cuuint64_t strides[1] = {(cuuint64_t)ld};
-  cuuint32_t box[2] = {BKB, (cuuint32_t)box_rows};
-  cuuint32_t es[2] = {1, 1};
-  CUresult r = g_encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, es,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)(ld * es)};
+  cuuint32_t box[2] = {(cuuint32_t)(BKB / es), (cuuint32_t)box_rows};
+  cuuint32_t step[2] = {1, 1};
+  CUresult r = g_encode(m, type, 2, const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(ATS_ECUDA, "int8_linear: cuTensorMapEncodeTiled failed (%d)", (int)r);
   return ATS_OK;
+}
+
+int operand_map(CUtensorMap* m, const int8_t* base, int64_t K, int64_t rows, int64_t ld, int box_rows) {
+  return row_map(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, base, K, rows, ld, box_rows);
 }
 
 template <typename T>
@@ -931,11 +941,18 @@ int pairs_that_fit(int smem, int* out) {
 
 template <typename T>
 int tiles(const int8_t* q, int64_t ldq, const int8_t* w, int64_t ldw, const Out& o, int K, cudaStream_t st) {
-  CUtensorMap ma, mb;
+  CUtensorMap ma, mb, my;
   ATS_TRY(operand_map(&ma, q, K, o.M, ldq, BM));
   ATS_TRY(operand_map(&mb, w, K, o.N, ldw, B_ROWS));
   const int vec = (int64_t)o.N * (int64_t)sizeof(T) % 16 == 0 && aligned16(o.y);
-  const TileArgs p{o, (K + BKB - 1) / BKB, (o.M + TM - 1) / TM, (o.N + BN - 1) / BN, vec};
+  if (vec) {
+    constexpr auto type = sizeof(T) == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+    ATS_TRY(row_map(&my, type, (int)sizeof(T), o.y, o.N, o.M, o.N, 32));
+  } else {
+    my = ma;  // not used
+  }
+  const TileArgs p{o, (K + BKB - 1) / BKB, (o.M + TM - 1) / TM, (o.N + BN - 1) / BN, vec,
+                   o.N % 2 == 0 && reinterpret_cast<uintptr_t>(o.y) % 4 == 0};
   const int64_t total = (int64_t)p.mt * p.nt;
   if (total > 0x7fffffff - 4096) return fail(ATS_EUNSUPPORTED, "int8_linear: too many tiles");
   const int smem = 1024 + kTileStages * kTileStage + kEpiWarps * kBox;
@@ -944,7 +961,8 @@ int tiles(const int8_t* q, int64_t ldq, const int8_t* w, int64_t ldw, const Out&
   if (pairs > gemm_ctas() / 2) pairs = gemm_ctas() / 2;
   if (pairs > total) pairs = (int)total;
   if (pairs < 1) pairs = 1;
-  return launch_after<int8_tile_kernel<T>>(dim3(2 * (unsigned)pairs), kTileThreads, smem, dim3(2), st, "int8_tile", ma, mb, p);
+  return launch_after<int8_tile_kernel<T>>(dim3(2 * (unsigned)pairs), kTileThreads, smem, dim3(2), st, "int8_tile", ma, mb,
+                                           my, p);
 }
 
 template <typename T, int TN>
