@@ -246,3 +246,11 @@ def test_pairs_and_copied_columns_of_every_alignment(D, pairs, dt):
 def test_threads_that_walk_many_heads(B, S, Hq, Hk, D, sections, dt, layout):
     """Enough tokens that a thread takes up to 16 heads one after the other, from q over to k."""
     check(B, S, Hq, Hk, D, sections, dt, layout=layout, seed=Hq)
+
+
+@pytest.mark.parametrize("D,sections,dt", [(96, (0, 2, 1, 2), "bf16"), (128, (32,), "bf16"), (80, (5,), "f32"),
+                                           (96, (0, 7), "f32"), (68, (2, 13), "bf16"), (20, (1, 3), "bf16"), (190, (81, 12), "bf16")])
+def test_copied_columns_of_many_heads(D, sections, dt):
+    """Heads with more copied columns than a thread each, and with fewer."""
+    check(2, 1500, 17, 4, D, sections, dt, seed=D)
+    check(1, 40, 3, 8, D, sections, dt, layout="bhsd", seed=D)
