@@ -660,11 +660,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid
 }
 
 // -------------------------------------------------- tensor cores, few tokens
-// The weights take the MMA's 128 rows and TN tokens its columns, and a cluster of `split` CTAs shares K: each sums
-// its part of K in TMEM, puts its int32 tile into its shared memory, and every CTA adds the parts of its share of
-// the tokens through distributed shared memory.  So a decoding batch reads the weights with every SM, and no
-// workspace or atomics are needed.  The weights' loads start before the quantisation has ended.  48 tokens through
-// 11008 x 4096: 11 us with the quantisation, 4.2 TB/s; sums over distributed shared memory cost about as much as their
+// The weights take the MMA's 128 rows and TN tokens its columns, and a cluster of `split` CTAs (1, 2, 3, 4, 6 or 8)
+// shares K: each sums its part of K in TMEM, puts its int32 tile into its shared memory, and every CTA adds the parts of
+// its share of the tokens through distributed shared memory.  So a decoding batch reads the weights with every SM, and
+// no workspace or atomics are needed.  The weights' loads start before the quantisation has ended.  48 tokens through
+// 11008 x 4096: 10.4 us with the quantisation, 4.5 TB/s; sums over distributed shared memory cost about as much as their
 // bytes at 3.3 TB/s, which is why few columns may be split further than many.
 constexpr int kPartThreads = 64 + 32 * kEpiWarps, kMaxSplit = 8;
 
@@ -853,11 +853,16 @@ __global__ void __launch_bounds__(kPartThreads, 2) int8_part_kernel(const __grid
   __syncwarp();
   if (split > 1) tc::cluster_sync();
   else __syncthreads();
-  const PartOut po{tile, sx_s, sw_s, bw_s, n0, m0, part * (TN / split), TN / split, vec_out};
-  if (split == 1) reduce_parts<T, 1>(o, po);
-  else if (split == 2) reduce_parts<T, 2>(o, po);
-  else if (split == 4) reduce_parts<T, 4>(o, po);
-  else reduce_parts<T, 8>(o, po);
+  const int each = (TN + split - 1) / split, first = part * each;
+  const PartOut po{tile, sx_s, sw_s, bw_s, n0, m0, first, TN - first < each ? TN - first : each, vec_out};
+  switch (split) {
+    case 1: reduce_parts<T, 1>(o, po); break;
+    case 2: reduce_parts<T, 2>(o, po); break;
+    case 3: reduce_parts<T, 3>(o, po); break;
+    case 4: reduce_parts<T, 4>(o, po); break;
+    case 6: reduce_parts<T, 6>(o, po); break;
+    default: reduce_parts<T, 8>(o, po);
+  }
   __syncwarp();
   // No CTA leaves while another reads its tile: what a thread read, it has used in the stores before this.
   if (split > 1) tc::cluster_sync_relaxed();
@@ -984,9 +989,7 @@ int linear(const void* x, int64_t ldx, const int8_t* w, int64_t ldw, Out o, int6
   ATS_TRY(quantize_t<T>(x, ldx, q, ldq, sx, o.M, K, st));
   o.sx = sx;
   // Few tiles of 128 channels: as many token columns as hold the tokens, at most 64, or 128 where 64 would make more
-  // than two CTAs per SM.  K is split while that gives idle SMs work (2 blocks of K to a part) or an SM a second CTA
-  // (8 blocks), and while the parts to be summed stay within 256 columns: 48 tokens 4096x11008, in us: 25.7 whole,
-  // 16.6 in 2, 12.6 in 4, 16.2 in 8; 1024^3: 7.8 whole, 8.8 in 2; 4 tokens 4096x4096: 11.8 whole, 7.4 in 4.
+  // than two CTAs per SM.
   const int64_t nt = (o.N + BM - 1) / BM, two = 2 * (int64_t)num_sms();
   const int kb = (int)((K + BKB - 1) / BKB);
   const int tn = o.M <= 16 ? 16 : o.M <= 32 ? 32 : nt * ((o.M + 63) / 64) <= two ? 64 : 128;
@@ -996,10 +999,20 @@ int linear(const void* x, int64_t ldx, const int8_t* w, int64_t ldw, Out o, int6
   const int64_t pair_tiles = ((o.M + TM - 1) / TM) * ((o.N + BN - 1) / (int64_t)BN);
   const bool one_round = ctas > num_sms() && tn == 128 && 8 * pair_tiles >= 3 * (int64_t)num_sms();
   if (ctas > two || mt > 65535 || one_round) return tiles<T>(q, ldq, w, ldw, o, (int)K, st);
+  // K is split so that the fullest SM, of one or two CTAs, has the least to do, where each part has 2 blocks of K, or 8
+  // where SMs have two parts, and at most 256 columns are summed; for the same load into more parts where each still
+  // has 16 blocks.  In us: 48 tokens 4096x11008 25.7 whole, 16.6 in 2, 12.6 in 4, 16.2 in 8; 48 tokens 11008x4096 14.3
+  // in 2, 12.9 in 3; 200 tokens 2048x8192 14.5 in 2, 13.2 in 4; 500 tokens 2048x2048 8.6 whole, 9.3 in 2.  Clusters of 3
+  // or 6 leave places free that others fill: 288 CTAs in clusters of 3 did not fit on 148 SMs at once (100 tokens
+  // 6144x4096: 16.7 in 3, 12.3 in 2), so they get nine tenths of the places.
   int split = 1;
-  while (split < kMaxSplit && 2 * split * tn <= 256 && 2 * split * ctas <= two &&
-         kb >= 2 * split * (2 * split * ctas <= num_sms() ? 2 : 8))
-    split *= 2;
+  double load = (double)((ctas + num_sms() - 1) / num_sms());  // in whole tiles
+  for (int n : {2, 3, 4, 6, 8}) {
+    const int64_t all = n * ctas;
+    if (n * tn > 256 || all > ((n & (n - 1)) == 0 ? two : two * 9 / 10) || kb < n * (all <= num_sms() ? 2 : 8)) continue;
+    const double l = (double)((all + num_sms() - 1) / num_sms()) / n;
+    if (l < load || (l == load && kb >= 16 * n)) load = l, split = n;
+  }
   switch (tn) {
     case 16: return parts<T, 16>(q, ldq, w, ldw, o, (int)K, split, st);
     case 32: return parts<T, 32>(q, ldq, w, ldw, o, (int)K, split, st);

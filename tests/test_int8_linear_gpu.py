@@ -242,3 +242,11 @@ def test_rows_of_every_alignment(K, dt):
         q, s = quantize_int8(whole.cuda()[:, start:start + K])
         qc, sc = quantize_int8(whole[:, start:start + K])
         assert torch.equal(q.cpu(), qc) and torch.equal(s.cpu().nan_to_num(-1), sc.nan_to_num(-1))
+
+
+@pytest.mark.parametrize("M,N,K", [(5, 10000, 3200), (30, 10000, 3201), (48, 11008, 4096), (64, 10120, 3300), (20, 2900, 1600),
+                                   (10, 5000, 6200), (31, 2999, 1700), (40, 4096, 8192), (2, 2900, 1600)])
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+def test_clusters_of_every_size(M, N, K, dt):
+    """K in 3, 4, 6 and 8 parts on 148 SMs, tokens that the parts share unevenly."""
+    check(M, N, K, dt, bias=True, seed=M)
