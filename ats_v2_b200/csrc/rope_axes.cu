@@ -48,8 +48,9 @@ struct AxesArgs {
   int64_t n_tokens, S;
   int D, pairs, axes;
   int rest_vec;  // elements per access of the copied columns
+  int width;     // threads to a head
   int tokens_per_block, group, heads_each;  // `group` threads share a token's heads, heads_each to each
-  unsigned by_vecs, by_group, by_pairs;  // for quotient()
+  unsigned by_width, by_group, by_pairs;  // for quotient()
   float sign;  // of the sine: +1 forward, -1 adjoint
   uint8_t axis[ATS_ROPE_MAX_PAIRS];
 };
@@ -93,8 +94,9 @@ __global__ void __launch_bounds__(kThreads, 4) rope_axes_kernel(const __grid_con
   float* sinv = cosv + p.tokens_per_block * p.pairs;
   int* axis_s = reinterpret_cast<int*>(sinv + p.tokens_per_block * p.pairs);  // [pairs] first position of the pair's axis
 
-  const int vecs = p.pairs / V;
-  const int rest = quotient(threadIdx.x, p.by_vecs), col = ((int)threadIdx.x - rest * vecs) * V;
+  const int vecs = p.pairs / V, width = REST ? p.width : vecs;
+  const int rest = quotient(threadIdx.x, p.by_width), vec = (int)threadIdx.x - rest * width;
+  const int col = !REST || vec < vecs ? vec * V : 0;
   const int t = quotient(rest, p.by_group);
   const int h0 = (int)blockIdx.y * p.group * p.heads_each + (rest - t * p.group);
   const bool active = t < ntok;
@@ -115,12 +117,13 @@ __global__ void __launch_bounds__(kThreads, 4) rope_axes_kernel(const __grid_con
   T* dst = target(h0) + col;
   const T* src_k = ki + k0 * p.k.is_h + col;
   T* dst_k = ko + k0 * p.k.os_h + col;
+  const int h_turn = !REST || vec < vecs ? h_end : 0;  // threads past the pairs' only copy
   R ra[kUnroll], rb[kUnroll];
   auto load = [&](int first) {
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
       const int h = first + u * p.group;
-      if (h < h_end) {
+      if (h < h_turn) {
         ra[u] = *reinterpret_cast<const R*>(src);
         rb[u] = *reinterpret_cast<const R*>(src + p.pairs);
       }
@@ -164,11 +167,11 @@ __global__ void __launch_bounds__(kThreads, 4) rope_axes_kernel(const __grid_con
   const float* cs = cosv + t * p.pairs + (V == 8 ? col / 2 : col);
   const float* sn = sinv + t * p.pairs + (V == 8 ? col / 2 : col);
   const int far = V == 8 ? p.pairs / 2 : 4;  // from the first four to the next
-  for (int first = h0; first < h_end; first += kUnroll * p.group) {
+  for (int first = h0; first < h_turn; first += kUnroll * p.group) {
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
       const int h = first + u * p.group;
-      if (h < h_end) {
+      if (h < h_turn) {
         const T* xa = reinterpret_cast<const T*>(&ra[u]);
         const T* xb = reinterpret_cast<const T*>(&rb[u]);
         R oa, ob;
@@ -197,14 +200,14 @@ __global__ void __launch_bounds__(kThreads, 4) rope_axes_kernel(const __grid_con
       }
       dst = h + p.group == k0 ? dst_k : dst + (h < p.q.heads ? p.q.o_step : p.k.o_step);
     }
-    if (first + kUnroll * p.group < h_end) load(first + kUnroll * p.group);
+    if (first + kUnroll * p.group < h_turn) load(first + kUnroll * p.group);
   }
 
   // Columns that are not rotated, `rest_vec` elements at a time.  Where a head has a piece for each of its threads they
-  // walk the heads as above (40 heads of 96 columns, 10 turned, of 7074 tokens: 39 us, dealt out 60), else
+  // walk the heads as above (40 heads of 96 columns, 10 turned, of 7074 tokens: 33 us, dealt out 60), else
   // all of the token's pieces are dealt out to its threads (8 heads of 190 columns, 186 turned: 83 us, walked 97).
   if (REST && active) {
-    const int vec = (int)threadIdx.x - rest * vecs, extra = (p.D - 2 * p.pairs) / p.rest_vec;
+    const int extra = (p.D - 2 * p.pairs) / p.rest_vec;
     auto walk = [&](auto raw) {
       using C = decltype(raw);
       constexpr int U = 4;  // heads in flight
@@ -221,7 +224,7 @@ __global__ void __launch_bounds__(kThreads, 4) rope_axes_kernel(const __grid_con
           src = h + p.group == k0 ? src_k : src + (h < p.q.heads ? p.q.i_step : p.k.i_step);
           dst = h + p.group == k0 ? dst_k : dst + (h < p.q.heads ? p.q.o_step : p.k.o_step);
         }
-        for (int c = vec; c < extra; c += vecs) {
+        for (int c = vec; c < extra; c += width) {
           C v[U];
 #pragma unroll
           for (int u = 0; u < U; ++u)
@@ -236,7 +239,7 @@ __global__ void __launch_bounds__(kThreads, 4) rope_axes_kernel(const __grid_con
       using C = decltype(raw);
       const int hb = (int)blockIdx.y * p.group * p.heads_each;
       const int nh = heads - hb < p.group * p.heads_each ? heads - hb : p.group * p.heads_each;
-      const int team = p.group * vecs;  // pieces: at most 256 of a head, of 4096 heads
+      const int team = p.group * width;  // pieces: at most 256 of a head, of 4096 heads
       for (int i = (int)threadIdx.x - t * team; i < nh * extra; i += team) {
         const int r = (int)((unsigned)i / (unsigned)extra), c = i - r * extra;
         reinterpret_cast<C*>(target(hb + r) + 2 * p.pairs)[c] =
@@ -244,7 +247,7 @@ __global__ void __launch_bounds__(kThreads, 4) rope_axes_kernel(const __grid_con
       }
     };
     auto copy = [&](auto raw) {
-      if (extra >= vecs) walk(raw);
+      if (extra >= width) walk(raw);
       else deal(raw);
     };
     const int bytes = p.rest_vec * (int)sizeof(T);
@@ -273,11 +276,17 @@ int vector_width(const AxesArgs& p, int64_t cols, int elem) {
 template <typename T, int V>
 int launch_v(AxesArgs& p, cudaStream_t st) {
   const int heads = p.q.heads + p.k.heads, vecs = p.pairs / V;
-  const int most = kThreads / vecs;  // heads at a time
+  // Threads to a head: one for each vector of pairs, but 8 where that is fewer and four times as many pieces are only
+  // copied, so that neighbours copy neighbours (10 heads of 128 columns, 12 turned, of 51456 tokens: 92 us, with three
+  // threads to a head 210; 40 heads of 96 columns, 10 turned, of 7074 tokens: 33 us, with five 39, with 32 61).
+  const int extra = (p.D - 2 * p.pairs) / p.rest_vec;
+  p.width = extra >= 4 * vecs ? (extra < 8 ? extra : 8) : vecs;
+  if (p.width < vecs) p.width = vecs;
+  const int most = kThreads / p.width;  // heads at a time
   // Heads to a thread: as many as leave three blocks to each SM, at most kMostHeads (the cosines and sines are then
   // computed once for many; a call of few tokens has one head to a thread and waits on latency alone).  From that
   // down to half of it, the number that leaves the fewest threads of a block idle.
-  const double work = (double)p.n_tokens * vecs * heads / ((double)kThreads * 3 * num_sms());
+  const double work = (double)p.n_tokens * p.width * heads / ((double)kThreads * 3 * num_sms());
   constexpr int kMostHeads = MostHeads<T, V>::value;
   int n = work < 1 ? 1 : work > kMostHeads ? kMostHeads : (int)work;
   if (n > heads) n = heads;
@@ -286,10 +295,10 @@ int launch_v(AxesArgs& p, cudaStream_t st) {
   for (int m = n; m >= 1 && 2 * m >= n; --m) {
     const int g = (heads + m - 1) / m;
     if (g > most) break;
-    const double full = (double)(kThreads / (vecs * g)) * vecs * heads / ((double)kThreads * m);
+    const double full = (double)(kThreads / (p.width * g)) * p.width * heads / ((double)kThreads * m);
     if (full > best) best = full, group = g, each = m;
   }
-  int tpb = kThreads / (vecs * group);
+  int tpb = kThreads / (p.width * group);
   if (tpb > kTableMax / p.pairs) tpb = kTableMax / p.pairs;
   if (tpb > kPosMax / p.axes) tpb = kPosMax / p.axes;
   if (tpb > p.n_tokens) tpb = (int)p.n_tokens;
@@ -299,7 +308,7 @@ int launch_v(AxesArgs& p, cudaStream_t st) {
   p.tokens_per_block = tpb, p.group = group, p.heads_each = each;
   for (AxesTensor* t : {&p.q, &p.k}) t->i_step = group * t->is_h, t->o_step = group * t->os_h;
   auto inverse = [](int d) { return (1u << 20) / (unsigned)d + 1; };
-  p.by_vecs = inverse(vecs), p.by_group = inverse(group), p.by_pairs = inverse(p.pairs);
+  p.by_width = inverse(p.width), p.by_group = inverse(group), p.by_pairs = inverse(p.pairs);
   const size_t smem = (size_t)p.pairs * sizeof(double2) + (size_t)(tpb * p.axes + 1) / 2 * 16 +
                       (size_t)(2 * tpb + 1) * p.pairs * sizeof(float);
   const dim3 grid((unsigned)blocks, (unsigned)parts);

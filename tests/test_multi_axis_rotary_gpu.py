@@ -249,7 +249,8 @@ def test_threads_that_walk_many_heads(B, S, Hq, Hk, D, sections, dt, layout):
 
 
 @pytest.mark.parametrize("D,sections,dt", [(96, (0, 2, 1, 2), "bf16"), (128, (32,), "bf16"), (80, (5,), "f32"),
-                                           (96, (0, 7), "f32"), (68, (2, 13), "bf16"), (20, (1, 3), "bf16"), (190, (81, 12), "bf16")])
+                                           (96, (0, 7), "f32"), (68, (2, 13), "bf16"), (20, (1, 3), "bf16"),
+                                           (190, (81, 12), "bf16"), (128, (6,), "bf16"), (128, (8,), "bf16"), (40, (1,), "f32")])
 def test_copied_columns_of_many_heads(D, sections, dt):
     """Heads with more copied columns than a thread each, and with fewer."""
     check(2, 1500, 17, 4, D, sections, dt, seed=D)
