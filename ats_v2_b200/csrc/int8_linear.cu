@@ -679,7 +679,9 @@ struct PartOut {
 };
 
 // Add the S parts of this CTA's tokens and write them: a warp takes tokens, a lane four channels, with 8 reads in
-// flight (a read of another CTA's shared memory takes hundreds of cycles).
+// flight, 6 where S is 3 or 6 (a read of another CTA's shared memory takes hundreds of cycles).  Each thread arrives
+// at the cluster's closing barrier between its last read of another CTA's tile and the stores that use it: the reads
+// are done with before any CTA may leave, and the barrier does not wait for these stores.
 template <typename T, int S>
 __device__ __forceinline__ void reduce_parts(const Out& o, const PartOut& p) {
   constexpr int U = kMaxSplit / S, W = kPartThreads / 32;
@@ -694,16 +696,20 @@ __device__ __forceinline__ void reduce_parts(const Out& o, const PartOut& p) {
   }
   const int left = o.M - p.m0 - p.first;
   const int share = p.share < left ? p.share : left;
+  if (S > 1 && warp >= share) tc::cluster_arrive();  // nothing to read
   for (int i0 = warp; i0 < share; i0 += U * W) {
     int4 b[U][S];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int i = i0 + u * W < share ? i0 + u * W : i0;
+      const int i = i0 + u * W;
+      const bool there = i < share && n < o.N;  // what is read is stored
 #pragma unroll
-      for (int z = 0; z < S; ++z)
-        b[u][z] = S == 1 ? *reinterpret_cast<const int4*>(p.tile + (p.first + i) * BM + r4)
-                         : tc::ld_cluster_v4(base[z] + (uint32_t)i * BM * 4u);
+      for (int z = 0; z < S; ++z) {
+        if constexpr (S > 1) b[u][z] = tc::ld_cluster_v4(base[z] + (uint32_t)i * BM * 4u, there);
+        else b[u][z] = there ? *reinterpret_cast<const int4*>(p.tile + (p.first + i) * BM + r4) : make_int4(0, 0, 0, 0);
+      }
     }
+    if (S > 1 && i0 + U * W >= share) tc::cluster_arrive();
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int i = i0 + u * W;
@@ -838,7 +844,7 @@ __global__ void __launch_bounds__(kPartThreads, 2) int8_part_kernel(const __grid
     tc::wait_prerequisites();  // the tokens' scales
     if (r < TN) sx_s[r] = m0 + r < o.M ? o.sx[m0 + r] : 0.f;
   }
-  if (!tc::mbar_wait(&tfull_bar, 0u, nullptr, kWaitBudget)) atomicCAS(&g_int8_status, 0, 44);
+  if (!tc::mbar_wait_warp(&tfull_bar, 0u, nullptr, kWaitBudget)) atomicCAS(&g_int8_status, 0, 44);
   tc::tc_fence_after();
   int* tile = reinterpret_cast<int*>(ring);  // [TN][128]: the ring is no longer read or written
   if (warp >= 2) {
@@ -864,8 +870,7 @@ __global__ void __launch_bounds__(kPartThreads, 2) int8_part_kernel(const __grid
     default: reduce_parts<T, 8>(o, po);
   }
   __syncwarp();
-  // No CTA leaves while another reads its tile: what a thread read, it has used in the stores before this.
-  if (split > 1) tc::cluster_sync_relaxed();
+  if (split > 1) tc::cluster_wait();  // no CTA leaves while another reads its tile
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();

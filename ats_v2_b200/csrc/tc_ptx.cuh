@@ -286,6 +286,11 @@ __device__ __forceinline__ void cluster_sync_relaxed() {
   asm volatile("barrier.cluster.arrive.relaxed;\n\tbarrier.cluster.wait;" ::: "memory");
 }
 
+// The two halves of cluster_sync: what a thread read and wrote before its arrival is done with before any thread of
+// the cluster leaves the wait.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+
 // Address, in the cluster's shared window, of this CTA's shared object at `saddr` as it sits in CTA `rank`.
 __device__ __forceinline__ uint32_t cluster_addr(uint32_t saddr, uint32_t rank) {
   uint32_t r;
@@ -389,13 +394,18 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, v
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_prerequisites() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
-// 16 bytes of shared memory of any CTA of the cluster (address from cluster_addr).
-__device__ __forceinline__ int4 ld_cluster_v4(uint32_t caddr) {
+// 16 bytes of shared memory of any CTA of the cluster (address from cluster_addr); zeros, and no access, where `there`
+// is false.
+__device__ __forceinline__ int4 ld_cluster_v4(uint32_t caddr, bool there) {
   int4 v;
-  asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "r"(caddr)
-               : "memory");
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "mov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
+      "@p ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];\n\t}"
+      : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w)
+      : "r"(caddr), "r"((uint32_t)there)
+      : "memory");
   return v;
 }
 
