@@ -424,6 +424,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid
   __shared__ __align__(8) uint64_t full_bar[NST], empty_bar[NST], tfull_bar[2], tempty_bar[2], done_bar;
   __shared__ uint32_t tmem_base_s;
   __shared__ int peer_issued_s;  // CTA 0: blocks that CTA 1 loaded
+  __shared__ int used_s, tiles_s;  // blocks multiplied and accumulators handed over, by CTA 0 for both
   __shared__ volatile int abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long budget = g_int8_wait_budget;
@@ -457,13 +458,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid
   tc::cluster_sync();  // both CTAs' barriers exist before either signals the other's
   tc::tc_fence_after();
   const uint32_t tmem_base = tmem_base_s;
-  // every load issued lands before the CTA may exit: the last phase of each stage of the first `issued` blocks
-  auto drain = [&](int issued) {
-    for (int s = 0; s < NST && s < issued; ++s) {
-      const int last = s + (issued - 1 - s) / NST * NST;
-      if (!tc::mbar_wait(&full_bar[s], (uint32_t)((last / NST) & 1), nullptr, kWaitBudget))
-        atomicCAS(&g_int8_status, 0, 35);
+  // Waits for the last phase of each of `depth` barriers that n arrivals went round: true where all have landed.
+  auto landed = [&](uint64_t* bar, int depth, int n) {
+    bool ok = true;
+    for (int s = 0; s < depth && s < n; ++s) {
+      const int last = s + (n - 1 - s) / depth * depth;
+      if (!tc::mbar_wait(&bar[s], (uint32_t)((last / depth) & 1), nullptr, kWaitBudget)) ok = false;
     }
+    return ok;
   };
   int issued_blocks = 0;
   tc::wait_prerequisites();  // the quantised tokens and their scales
@@ -506,9 +508,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid
         tc::mma_commit_pair(tc::cluster_addr(tc::smem_u32(bar), 0u));
         tc::mma_commit_pair(tc::cluster_addr(tc::smem_u32(bar), 1u));
       };
-      int stage = 0, i = 0;
+      int stage = 0, i = 0, used = 0, tiles = 0;
       uint32_t phase = 0;
-      bool issued = false, ok = true;
+      bool ok = true;
       for (int t = t_first; t < total && ok; t += t_step, ++i) {
         const int acc = i & 1;
         ok = tc::mbar_wait_warp(&tempty_bar[acc], ((uint32_t)(i >> 1) & 1u) ^ 1u, &abort_flag, budget);
@@ -534,16 +536,21 @@ __global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid
             commit(&empty_bar[stage]);
             if (kb == p.kb - 1) commit(&tfull_bar[acc]);
           }
-          issued = true;
+          ++used;
+          if (kb == p.kb - 1) ++tiles;
           if (++stage == NST) {
             stage = 0;
             phase ^= 1u;
           }
         }
       }
-      if (issued) {  // all MMAs complete before TMEM is freed
-        if (tc::elect_one()) commit(&done_bar);
-        if (!tc::mbar_wait(&done_bar, 0u, nullptr, kWaitBudget)) atomicCAS(&g_int8_status, 0, 36);
+      if (used > 0) {  // all MMAs complete before TMEM is freed
+        if (tc::elect_one()) tc::mma_commit_pair(tc::cluster_addr(tc::smem_u32(&done_bar), 0u));
+        if (!tc::mbar_wait_warp(&done_bar, 0u, nullptr, kWaitBudget)) atomicCAS(&g_int8_status, 0, 36);
+      }
+      if (lane < 2) {
+        tc::st_cluster_u32(tc::cluster_addr(tc::smem_u32(&used_s), (uint32_t)lane), (uint32_t)used);
+        tc::st_cluster_u32(tc::cluster_addr(tc::smem_u32(&tiles_s), (uint32_t)lane), (uint32_t)tiles);
       }
     }
   } else {
@@ -633,22 +640,28 @@ __global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid
   }
   tc::tc_fence_before();
   __syncthreads();
-  // CTA 0's MMAs read CTA 1's ring and write its TMEM, and CTA 1's loads and epilogue signal CTA 0's barriers.  After
-  // the first barrier CTA 0 knows how many blocks each loaded.  Where only one of them loaded a block (the other gave
-  // up) it settles that block's count -- the half that never came counted as done, the half on its way expected -- and
-  // waits for every phase, so no load is in flight when the second barrier lets both exit.
+  // CTA 0's MMAs read CTA 1's ring and write its TMEM, its commits signal the barriers of both, and CTA 1's loads and
+  // epilogue signal CTA 0's.  After the first barrier each knows how many blocks were loaded and multiplied, and waits
+  // for the commits' last arrivals at its own barriers: at most one is due at each, since a stage or an accumulator is
+  // used again only after both CTAs have seen the last one.  Where only one of them loaded a block (the other gave up)
+  // CTA 0 settles that block's count -- the half that never came counted as done, the half on its way expected -- and
+  // waits for every phase.  So no load and no arrival is in flight when the second barrier lets both exit.
   tc::cluster_sync();
-  if (cta == 0 && warp == 0 && lane == 0) {
-    const int own = issued_blocks, peer = peer_issued_s;
-    const int lo = own < peer ? own : peer, hi = own < peer ? peer : own;
-    if (hi - lo > NST) {  // cannot happen: a stage is loaded again only after both halves of its last load
-      atomicCAS(&g_int8_status, 0, 37);
-    } else {
-      for (int k = lo; k < hi; ++k) {
-        if (k < own) tc::mbar_complete_tx(&full_bar[k % NST], STAGE);
-        else tc::mbar_arrive_expect_tx(&full_bar[k % NST], STAGE);
+  if (warp == 0 && lane == 0) {
+    const bool empties = landed(empty_bar, NST, used_s), accs = landed(tfull_bar, 2, tiles_s);
+    if (!empties || !accs) atomicCAS(&g_int8_status, 0, 38);
+    if (cta == 0) {
+      const int own = issued_blocks, peer = peer_issued_s;
+      const int lo = own < peer ? own : peer, hi = own < peer ? peer : own;
+      if (hi - lo > NST) {  // cannot happen: a stage is loaded again only after both halves of its last load
+        atomicCAS(&g_int8_status, 0, 37);
+      } else {
+        for (int k = lo; k < hi; ++k) {
+          if (k < own) tc::mbar_complete_tx(&full_bar[k % NST], STAGE);
+          else tc::mbar_arrive_expect_tx(&full_bar[k % NST], STAGE);
+        }
+        if (!landed(full_bar, NST, hi)) atomicCAS(&g_int8_status, 0, 35);
       }
-      drain(hi);
     }
   }
   __syncwarp();

@@ -36,3 +36,10 @@ def repeated(M, N, K, calls=60):
                                    (200, 2048, 8192)])
 def test_parts_of_k_with_uneven_shares_of_the_tokens(M, N, K):
     repeated(M, N, K)
+
+
+@pytest.mark.parametrize("M,N,K", [(2304, 4096, 16), (2304, 4096, 130), (5001, 1003, 260), (1200, 8000, 900),
+                                   (4500, 4500, 64), (2200, 4096, 2048)])
+def test_pairs_whose_barriers_are_passed_once_or_often(M, N, K):
+    """One block of K, fewer blocks than stages, more than twice as many; one tile to a pair, and several."""
+    repeated(M, N, K, calls=30)
