@@ -557,7 +557,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid
     const int quad = warp & 3, chalf = (warp - 2) >> 2;
     uint8_t* box = staging + (warp - 2) * kBox;
     int i = 0;
-    for (int t = t_first; t < total && !abort_flag; t += t_step, ++i) {
+    // the whole warp goes on or leaves: the flag may be set while its lanes read it
+    for (int t = t_first; t < total && !__any_sync(0xffffffffu, abort_flag); t += t_step, ++i) {
       int m, n;
       tile_of(p, t, m, n);
       const int acc = i & 1;
@@ -634,6 +635,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid
           if (sizeof(T) == 4 || p.even_out) store(uint32_t{});
           else store(uint16_t{});
         }
+        __syncwarp();  // the accumulator is read, and the flag voted on, by whole warps
       }
     }
     if (lane == 0) tc::bulk_wait<0>();  // every store is complete before the CTA exits
