@@ -16,6 +16,7 @@ from ctypes import POINTER, c_char_p, c_float, c_int, c_int64, c_size_t, c_void_
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 LIB_PATH = Path(__file__).resolve().parent / "libats_b200.so"
 
@@ -287,8 +288,18 @@ def device_of(t: torch.Tensor):
     return _SAME_DEVICE if t.device.index == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
 
 
+def refuse_tangents(*tensors: torch.Tensor | None) -> None:
+    """The kernels have no forward-mode derivative, and a result without a tangent reads as a derivative of zero."""
+    if forward_ad._current_level >= 0:  # a dual level is open: elsewhere this costs one comparison
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError("ats_v2_b200 kernels do not compute forward-mode derivatives. Fix: use "
+                                          "reverse mode, or pass the primal of a dual tensor.")
+
+
 def wants_grad(*tensors: torch.Tensor | None) -> bool:
-    """Whether a call on these tensors is to be recorded for a backward."""
+    """Whether a call on these tensors is to be recorded for a backward; forward-mode duals are refused."""
+    refuse_tangents(*tensors)
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
@@ -304,6 +315,7 @@ def once_differentiable(backward):
 
     @functools.wraps(backward)
     def run(ctx, *grads):
+        refuse_tangents(*grads)
         return wrapped(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
 
     return run

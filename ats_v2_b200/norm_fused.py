@@ -269,7 +269,8 @@ def fused_sandwich_norm(x: torch.Tensor, residual: torch.Tensor, post_weight: to
     last axes before hidden, e.g. [batch, 1, hidden] (per sequence).  The arithmetic is
     float32 and each result is rounded once.  CUDA tensors run one kernel forward and
     two backward (sums over rows in a fixed order: results repeat bit for bit);
-    differentiable once, in every tensor argument."""
+    differentiable once, in every tensor argument, and in reverse mode only (duals are
+    refused)."""
     shape = x.shape
     if len(shape) < 1 or shape[-1] < 1:
         raise ValueError(f"fused_sandwich_norm expected x of shape [..., hidden], got {tuple(shape)}.")

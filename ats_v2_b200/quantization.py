@@ -94,9 +94,10 @@ def quantize_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     ``amax`` is the row's largest magnitude (at least 2^-100).  A row that holds an infinity or
     NaN gets zeros and a NaN scale.  For a weight [out_features, in_features] the scales are per
     output channel.  Rows of the result start at multiples of 16 bytes, as ``int8_linear`` reads
-    them.  Not differentiable."""
+    them.  Not differentiable: the results have no graph, and forward-mode duals are refused."""
     if x.dim() < 1 or not 1 <= x.shape[-1] <= INT8_MAX_FEATURES:
         raise ValueError(f"quantize_int8: x must be [..., 1 to {INT8_MAX_FEATURES} features], got {tuple(x.shape)}.")
+    _lib.refuse_tangents(x)
     lead, K = x.shape[:-1], x.shape[-1]
     x2 = _rows(x.detach())
     Kp = (K + 15) // 16 * 16
@@ -123,7 +124,7 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor,
     exactly in int32, then scaled in float32 and rounded once to x's dtype.  A token that holds
     an infinity or NaN gives NaN outputs.  Weight rows should start at multiples of 16 bytes, as
     ``quantize_int8`` lays them out; others are copied on every call.  Inference only: tensors
-    that need a gradient are refused."""
+    that need a gradient and forward-mode duals are refused."""
     if weight.dim() != 2 or weight.dtype != torch.int8:
         raise TypeError(f"int8_linear: weight must be int8 [out_features, in_features], got {weight.dtype} "
                         f"{tuple(weight.shape)}. Fix: pass quantize_int8(weight).")

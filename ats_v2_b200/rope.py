@@ -255,7 +255,8 @@ def apply_multi_axis_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: 
     float32 [sum(sections)]).  Columns from 2*sum(sections) on pass unchanged.  The angles are
     reduced in 64 bits, so far positions keep their accuracy; the rest is float32, rounded once.
     Any batch, head and sequence strides; the results of dense inputs are laid out like them.
-    One launch each way on CUDA tensors; differentiable once, in q and k."""
+    One launch each way on CUDA tensors; differentiable once, in q and k, and in reverse mode only
+    (duals are refused)."""
     axes = axis_of_pairs(tuple(sections), bool(interleaved))
     n_axes = len(sections)
     if q.dim() != 4 or q.shape[-1] < 2 * len(axes):
@@ -280,6 +281,7 @@ def apply_multi_axis_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: 
     if _lib.on_cpu("apply_multi_axis_rotary", q, k, positions, inv_freq):
         return (_torch_multi_axis(q, positions, inv_freq, axes),
                 _torch_multi_axis(k, positions, inv_freq, axes) if k is not None else None)
+    _lib.refuse_tangents(positions, inv_freq)
     q = _last_dim_contig(q)
     k = _last_dim_contig(k) if k is not None else None
     inv_freq = inv_freq.contiguous()
