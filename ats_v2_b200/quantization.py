@@ -202,9 +202,10 @@ class Int8Linear(nn.Module):
         return new
 
     def _apply(self, fn, recurse=True):  # moves keep the scales float32 and the rows aligned
-        scale = self.scale
+        old = self.scale
         super()._apply(fn, recurse)
-        self.scale = scale.to(device=self.scale.device)
+        if self.scale.dtype != torch.float32:
+            self.scale = self.scale.float() if old.is_meta else old.to(device=self.scale.device)
         self.weight = self._laid_out(self.weight)
         return self
 

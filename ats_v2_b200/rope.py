@@ -307,13 +307,19 @@ class MultiAxisRotaryEmbedding(nn.Module):
         self.theta = theta
         self.interleaved = bool(interleaved)
         self.inv_freq: torch.Tensor
-        self.register_buffer("inv_freq", 1.0 / (theta ** (torch.arange(0, dim, 2, dtype=torch.float32) / dim)),
-                             persistent=False)
+        self.register_buffer("inv_freq", self._frequencies(), persistent=False)
 
-    def _apply(self, fn, recurse=True):  # .to(dtype) must not round the frequencies
-        inv_freq = self.inv_freq
+    def _frequencies(self, device: torch.device | None = None) -> torch.Tensor:
+        return 1.0 / (self.theta ** (torch.arange(0, self.dim, 2, dtype=torch.float32, device=device) / self.dim))
+
+    def _apply(self, fn, recurse=True):
+        old = self.inv_freq
         super()._apply(fn, recurse)
-        self.inv_freq = inv_freq.to(device=self.inv_freq.device)
+        new = self.inv_freq
+        if old.is_meta and not new.is_meta:  # to_empty: no state dict holds what belongs there
+            self.inv_freq = self._frequencies(new.device)
+        elif new.dtype != torch.float32:  # .to(dtype) must not round the frequencies
+            self.inv_freq = old.to(device=new.device)
         return self
 
     def forward(self, q: torch.Tensor, k: torch.Tensor | None,

@@ -1,0 +1,59 @@
+"""The block operators' modules as a model's loading code treats them: made without memory, materialised, cast, loaded."""
+
+from __future__ import annotations
+
+import copy
+
+import pytest
+import torch
+
+from ats_v2_b200.quantization import Int8Linear
+from ats_v2_b200.rope import MultiAxisRotaryEmbedding
+
+
+@pytest.mark.parametrize("cast", [None, torch.bfloat16, torch.float64])
+def test_rotary_made_on_the_meta_device(cast):
+    want = MultiAxisRotaryEmbedding(16, (5, 3), theta=500.0)
+    with torch.device("meta"):
+        emb = MultiAxisRotaryEmbedding(16, (5, 3), theta=500.0)
+    assert emb.inv_freq.is_meta
+    if cast is not None:
+        emb = emb.to(cast)
+        assert emb.inv_freq.is_meta and emb.inv_freq.dtype == torch.float32
+    emb = torch.nn.ModuleList([emb]).to_empty(device="cpu")[0]
+    assert torch.equal(emb.inv_freq, want.inv_freq)  # in no state dict: it is there without one
+    q, pos = torch.randn(2, 3, 4, 16), torch.randint(0, 50, (2, 2, 4))
+    assert torch.equal(emb(q, None, pos)[0], want(q, None, pos)[0])
+
+
+def test_rotary_casts_keep_its_frequencies():
+    emb = MultiAxisRotaryEmbedding(16, (5, 3))
+    want = emb.inv_freq.clone()
+    for m in (emb.half(), copy.deepcopy(emb).bfloat16(), emb.double(), emb.to("cpu")):
+        assert m.inv_freq.dtype == torch.float32 and torch.equal(m.inv_freq, want)
+
+
+@pytest.mark.parametrize("K", [33, 48])
+@pytest.mark.parametrize("cast", [None, torch.bfloat16])
+def test_int8_linear_made_on_the_meta_device(K, cast):
+    want = Int8Linear.from_linear(torch.nn.Linear(K, 5))
+    with torch.device("meta"):
+        lin = Int8Linear(K, 5, bias=True)
+    if cast is not None:
+        lin = lin.to(cast)
+        assert lin.scale.is_meta and lin.scale.dtype == torch.float32
+    lin = torch.nn.ModuleList([lin]).to_empty(device="cpu")[0]
+    assert not lin.weight.is_meta and lin.weight.stride() == (48, 1)
+    lin.load_state_dict(want.state_dict())
+    x = torch.randn(3, K)
+    assert lin.scale.dtype == torch.float32
+    assert torch.equal(lin(x), want(x)) or cast is not None  # a cast rounds the bias, as it does a Linear's
+    assert torch.equal(lin.weight, want.weight) and torch.equal(lin.scale, want.scale)
+
+
+def test_int8_linear_casts_keep_its_scales():
+    lin = Int8Linear.from_linear(torch.nn.Linear(40, 5))
+    scale, weight = lin.scale.clone(), lin.weight.clone()
+    for m in (lin.half(), copy.deepcopy(lin).bfloat16(), lin.double(), lin.to("cpu")):
+        assert m.scale.dtype == torch.float32 and torch.equal(m.scale, scale) and torch.equal(m.weight, weight)
+        assert m.weight.stride(0) % 16 == 0
