@@ -188,7 +188,8 @@ class Int8Linear(nn.Module):
     def _laid_out(weight: torch.Tensor) -> torch.Tensor:
         """weight with rows that start at multiples of 16 bytes."""
         N, K = weight.shape
-        if weight.stride(1) == 1 and weight.stride(0) % 16 == 0 and weight.stride(0) >= K:
+        if weight.stride(1) == 1 and weight.stride(0) % 16 == 0 and weight.stride(0) >= K and \
+                weight.data_ptr() % 16 == 0:
             return weight
         return torch.zeros((N, (K + 15) // 16 * 16), dtype=torch.int8, device=weight.device)[:, :K].copy_(weight)
 
@@ -208,6 +209,10 @@ class Int8Linear(nn.Module):
             self.scale = self.scale.float() if old.is_meta else old.to(device=self.scale.device)
         self.weight = self._laid_out(self.weight)
         return self
+
+    def _load_from_state_dict(self, *args, **kwargs):  # assign=True takes a weight laid out in any way
+        super()._load_from_state_dict(*args, **kwargs)
+        self.weight = self._laid_out(self.weight)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         return int8_linear(x, self.weight, self.scale, self.bias)

@@ -57,3 +57,27 @@ def test_int8_linear_casts_keep_its_scales():
     for m in (lin.half(), copy.deepcopy(lin).bfloat16(), lin.double(), lin.to("cpu")):
         assert m.scale.dtype == torch.float32 and torch.equal(m.scale, scale) and torch.equal(m.weight, weight)
         assert m.weight.stride(0) % 16 == 0
+
+
+@pytest.mark.parametrize("meta", [False, True])
+def test_an_assigned_weight_is_laid_out_once(meta):
+    """int8_linear copies a weight whose rows do not start at multiples of 16 bytes: not on every call of a module."""
+    want = Int8Linear.from_linear(torch.nn.Linear(33, 7))
+    buf = torch.empty(7 * 33 + 1, dtype=torch.int8)[1:].view(7, 33)
+    wide = torch.empty(7 * 48 + 1, dtype=torch.int8)[1:].view(7, 48)[:, :33]  # rows of 48 bytes from an odd address
+    for weight in (want.weight.contiguous(), want.weight.t().contiguous().t(), buf.copy_(want.weight),
+                   wide.copy_(want.weight)):
+        with torch.device("meta" if meta else "cpu"):
+            lin = Int8Linear(33, 7, bias=True)
+        lin.load_state_dict({**want.state_dict(), "weight": weight}, assign=True)
+        assert lin.weight.stride() == (48, 1) and lin.weight.data_ptr() % 16 == 0
+        assert torch.equal(lin.weight, want.weight)
+        x = torch.randn(3, 33)
+        assert torch.equal(lin(x), want(x))
+        assert set(lin.state_dict()) == {"weight", "scale", "bias"}
+    lin = Int8Linear(33, 7, bias=True)
+    aligned = want.weight
+    lin.load_state_dict({**want.state_dict(), "weight": aligned}, assign=True)
+    assert lin.weight.data_ptr() == aligned.data_ptr()  # already so: taken as it is
+    with pytest.raises(RuntimeError, match="size mismatch"):
+        lin.load_state_dict({**want.state_dict(), "weight": aligned[:, :32]}, assign=True)
