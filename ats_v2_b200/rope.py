@@ -88,6 +88,13 @@ def _last_dim_contig(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 else t.contiguous()
 
 
+def _out_like(t: torch.Tensor) -> torch.Tensor:
+    """An empty tensor laid out like t, its last axis consecutive as the kernels write it: empty_like moves another
+    axis of an overlapping view (windows of a longer sequence, say) inside of it."""
+    out = torch.empty_like(t)
+    return out if out.stride(-1) == 1 else t.new_empty(t.shape)
+
+
 def _table(t: torch.Tensor, D: int, S: int, name: str) -> tuple[torch.Tensor, int]:
     if t.dim() != 2 or t.shape[-1] != D or t.shape[0] not in (S, 1):
         raise ValueError(f"{name}: cos/sin must be [seq_len={S} (or 1), {D}], got {tuple(t.shape)}")
@@ -111,8 +118,8 @@ class _RopeFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, cos, sin, cs_stride):
         ctx.set_materialize_grads(False)  # an unused output's gradient arrives as None, not zeros
-        q_out = torch.empty_like(q)
-        k_out = torch.empty_like(k) if k is not None else None
+        q_out = _out_like(q)
+        k_out = _out_like(k) if k is not None else None
         _launch(q, q_out, k, k_out, cos, sin, cs_stride, False)
         ctx.save_for_backward(cos, sin)
         ctx.cs_stride = cs_stride
@@ -126,15 +133,15 @@ class _RopeFn(torch.autograd.Function):
             return None, None, None, None, None
         if dq_out is None:  # only k was used downstream: run its adjoint alone
             dk_out = _last_dim_contig(dk_out)
-            dk = torch.empty_like(dk_out)
+            dk = _out_like(dk_out)
             _launch(dk_out, dk, None, None, cos, sin, ctx.cs_stride, True)
             return None, dk, None, None, None
         dq_out = _last_dim_contig(dq_out)
-        dq = torch.empty_like(dq_out)
+        dq = _out_like(dq_out)
         dk = None
         if ctx.has_k and dk_out is not None:
             dk_out = _last_dim_contig(dk_out)
-            dk = torch.empty_like(dk_out)
+            dk = _out_like(dk_out)
         _launch(dq_out, dq, dk_out if dk is not None else None, dk, cos, sin, ctx.cs_stride, True)
         return dq, dk, None, None, None
 
@@ -215,8 +222,8 @@ class _MultiAxisRotaryFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, positions, inv_freq, axes, n_axes):
         ctx.set_materialize_grads(False)  # an unused output's gradient arrives as None, not zeros
-        q_out = torch.empty_like(q)
-        k_out = torch.empty_like(k) if k is not None else None
+        q_out = _out_like(q)
+        k_out = _out_like(k) if k is not None else None
         _launch_axes(q, q_out, k, k_out, positions, inv_freq, axes, n_axes, False)
         ctx.save_for_backward(positions, inv_freq)
         ctx.axes = axes, n_axes
@@ -227,7 +234,7 @@ class _MultiAxisRotaryFn(torch.autograd.Function):
     def backward(ctx, dq_out, dk_out):
         positions, inv_freq = ctx.saved_tensors
         dq_out, dk_out = (_last_dim_contig(t) if t is not None else None for t in (dq_out, dk_out))
-        dq, dk = (torch.empty_like(t) if t is not None else None for t in (dq_out, dk_out))
+        dq, dk = (_out_like(t) if t is not None else None for t in (dq_out, dk_out))
         if dq is not None or dk is not None:
             _launch_axes(dq_out, dq, dk_out, dk, positions, inv_freq, *ctx.axes, True)
         return dq, dk, None, None, None, None
@@ -287,7 +294,7 @@ def apply_multi_axis_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: 
     inv_freq = inv_freq.contiguous()
     if _lib.wants_grad(q, k):
         return _MultiAxisRotaryFn.apply(q, k, positions, inv_freq, axes, n_axes)
-    q_out, k_out = torch.empty_like(q), torch.empty_like(k) if k is not None else None
+    q_out, k_out = _out_like(q), _out_like(k) if k is not None else None
     _launch_axes(q, q_out, k, k_out, positions, inv_freq, axes, n_axes, False)
     return q_out, k_out
 
