@@ -188,11 +188,15 @@ def apply_rotary_pos_emb(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor,
     return _RopeFn.apply(q, k, cos, sin, cs)
 
 
-@functools.lru_cache(maxsize=64)
 def axis_of_pairs(sections: tuple[int, ...], interleaved: bool = False) -> bytes:
     """The position axis of each rotated pair.  ``sections[a]`` pairs follow axis a:
     section after section, or (``interleaved``) dealt out one by one to the axes that
     have pairs left."""
+    return _axis_of_pairs(bool(interleaved), *sections)
+
+
+@functools.lru_cache(maxsize=64, typed=True)  # by the counts' types too: 2.0 is refused whether or not 2 was seen
+def _axis_of_pairs(interleaved: bool, *sections: int) -> bytes:
     if not sections or any(not isinstance(n, int) or n < 0 for n in sections) or len(sections) > 256 or \
             not 1 <= sum(sections) <= _lib.ATS_ROPE_MAX_PAIRS:
         raise ValueError(f"multi-axis rotary: sections {sections} must be counts of pairs, one per axis, 1 to "
