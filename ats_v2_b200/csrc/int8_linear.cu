@@ -930,7 +930,8 @@ int operand_map(CUtensorMap* m, const int8_t* base, int64_t K, int64_t rows, int
 template <typename T>
 int dot(const void* x, const int8_t* w, int64_t ldw, const Out& o, int K, cudaStream_t st) {
   const int warps = kDotThreads / 32;
-  const int64_t want = (o.N + warps - 1) / warps, cap = (int64_t)num_sms() * 4;
+  // a limit on the GEMMs' SMs leaves one block to each
+  const int64_t want = (o.N + warps - 1) / warps, cap = gemm_ctas() < num_sms() ? gemm_ctas() : (int64_t)num_sms() * 4;
   const unsigned grid = (unsigned)(want < cap ? want : cap);
   return launch_after<int8_dot_kernel<T>>(dim3(grid), kDotThreads, (int)padded_k(K), dim3(1), st, "int8_dot",
                       static_cast<const T*>(x), w, ldw, o, K, aligned16(x) ? 1 : 0);
@@ -1010,14 +1011,16 @@ int linear(const void* x, int64_t ldx, const int8_t* w, int64_t ldw, Out o, int6
   o.sx = sx;
   // Few tiles of 128 channels: as many token columns as hold the tokens, at most 64, or 128 where 64 would make more
   // than two CTAs per SM.
-  const int64_t nt = (o.N + BM - 1) / BM, two = 2 * (int64_t)num_sms();
+  // Under a limit on the GEMMs' SMs the parts get one CTA to an SM, and what does not fit takes the persistent pairs.
+  const int sms = gemm_ctas();
+  const int64_t nt = (o.N + BM - 1) / BM, two = sms < num_sms() ? sms : 2 * (int64_t)sms;
   const int kb = (int)((K + BKB - 1) / BKB);
   const int tn = o.M <= 16 ? 16 : o.M <= 32 ? 32 : nt * ((o.M + 63) / 64) <= two ? 64 : 128;
   const int64_t mt = (o.M + tn - 1) / tn, ctas = nt * mt;
   // One round of pair tiles beats two CTAs to an SM where it keeps three quarters of the pairs busy (2000^3: 16.8 us
   // against 20.4; 3000 x 1000 x 1000, 48 tiles: 13.7 against 14.3; 1024 x 2048 x 4096, 32 tiles: 19.0 against 15.6).
   const int64_t pair_tiles = ((o.M + TM - 1) / TM) * ((o.N + BN - 1) / (int64_t)BN);
-  const bool one_round = ctas > num_sms() && tn == 128 && 8 * pair_tiles >= 3 * (int64_t)num_sms();
+  const bool one_round = ctas > sms && tn == 128 && 8 * pair_tiles >= 3 * (int64_t)sms;
   if (ctas > two || mt > 65535 || one_round) return tiles<T>(q, ldq, w, ldw, o, (int)K, st);
   // K is split so that the fullest SM, of one or two CTAs, has the least to do, where each part has 2 blocks of K, or 8
   // where SMs have two parts, and at most 256 columns are summed; for the same load into more parts where each still
@@ -1026,11 +1029,11 @@ int linear(const void* x, int64_t ldx, const int8_t* w, int64_t ldw, Out o, int6
   // or 6 leave places free that others fill: 288 CTAs in clusters of 3 did not fit on 148 SMs at once (100 tokens
   // 6144x4096: 16.7 in 3, 12.3 in 2), so they get nine tenths of the places.
   int split = 1;
-  double load = (double)((ctas + num_sms() - 1) / num_sms());  // in whole tiles
+  double load = (double)((ctas + sms - 1) / sms);  // in whole tiles
   for (int n : {2, 3, 4, 6, 8}) {
     const int64_t all = n * ctas;
-    if (n * tn > 256 || all > ((n & (n - 1)) == 0 ? two : two * 9 / 10) || kb < n * (all <= num_sms() ? 2 : 8)) continue;
-    const double l = (double)((all + num_sms() - 1) / num_sms()) / n;
+    if (n * tn > 256 || all > ((n & (n - 1)) == 0 ? two : two * 9 / 10) || kb < n * (all <= sms ? 2 : 8)) continue;
+    const double l = (double)((all + sms - 1) / sms) / n;
     if (l < load || (l == load && kb >= 16 * n)) load = l, split = n;
   }
   switch (tn) {

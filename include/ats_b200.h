@@ -597,7 +597,9 @@ ATS_API int ats_moe_router_status(const void* workspace, size_t workspace_bytes,
  * the sum exact in int32, the rest float32, rounded once to dtype.  w: int8
  * [N, K], 16-byte aligned rows (w_row_stride a multiple of 16 bytes); bytes past K are not used.  bias
  * [N] may be NULL.  y [M, N] contiguous.  workspace: 16-byte aligned,
- * ats_int8_linear_workspace_bytes(M, N, K) (0: none).  The reference's quantized Linear
+ * ats_int8_linear_workspace_bytes(M, N, K) (0: none).  Under
+ * ats_set_gemm_sm_limit the product's CTAs are at most that many (two where the
+ * limit is one); the quantisation's blocks are not limited.  The reference's quantized Linear
  * (ats/model/quantization.py:40-193) only imitates int8 in float. */
 ATS_API int ats_int8_quantize(const void* x, int64_t x_row_stride, ats_dtype dtype, void* q, int64_t q_row_stride,
                               float* scale, int64_t rows, int64_t K, void* stream);
