@@ -18,7 +18,9 @@ For inference, ``Int8Linear`` holds the weight in 8-bit integers and multiplies
 integers: ``quantize_int8`` gives int8 rows with a float32 scale each, and
 ``int8_linear`` quantises its input per token and runs the integer product on
 the sm_100a kernels (not in the reference, whose int8 mode imitates the
-rounding in floating point).
+rounding in floating point).  Its scales are finer than those that
+``QuantizedLinear`` trains with (see ``Int8Linear``): serving a trained layer
+this way is a quantisation of its float weights, not the trained rounding.
 """
 
 from __future__ import annotations
@@ -169,7 +171,12 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor,
 class Int8Linear(nn.Module):
     """A Linear for inference with 8-bit weights: buffers ``weight`` (int8), ``scale`` (float32,
     per output channel) and ``bias``; ``forward`` is ``int8_linear``.  ``from_linear`` quantises
-    an ``nn.Linear`` (a ``QuantizedLinear`` trained with fake quantisation included)."""
+    the float weight of an ``nn.Linear``.
+
+    A ``QuantizedLinear`` is an ``nn.Linear`` too, but the result does not round as its training
+    did: here each output channel and each token has a symmetric scale of its own, where it
+    imitates one symmetric scale for the whole weight and one affine range, observed over many
+    batches, for all activations.  Its observers are dropped."""
 
     def __init__(self, in_features: int, out_features: int, bias: bool = False) -> None:
         super().__init__()

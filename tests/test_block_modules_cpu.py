@@ -7,7 +7,7 @@ import copy
 import pytest
 import torch
 
-from ats_v2_b200.quantization import Int8Linear
+from ats_v2_b200.quantization import Int8Linear, QuantizedLinear
 from ats_v2_b200.rope import MultiAxisRotaryEmbedding
 
 
@@ -81,3 +81,21 @@ def test_an_assigned_weight_is_laid_out_once(meta):
     assert lin.weight.data_ptr() == aligned.data_ptr()  # already so: taken as it is
     with pytest.raises(RuntimeError, match="size mismatch"):
         lin.load_state_dict({**want.state_dict(), "weight": aligned[:, :32]}, assign=True)
+
+
+def test_a_fake_quantised_layer_is_served_by_its_float_weight():
+    """Not by the rounding it trained with: scales per channel and token, the observed ranges unused."""
+    qat = QuantizedLinear(40, 6, "int8", bias=True)
+    with torch.no_grad():
+        qat.weight[0] *= 100  # the one scale of the whole weight, in training
+    qat.train()
+    for _ in range(3):
+        qat(50 * torch.randn(8, 40))  # moves the observed ranges
+    plain = torch.nn.Linear(40, 6)
+    plain.load_state_dict({"weight": qat.weight, "bias": qat.bias})
+    served, want = Int8Linear.from_linear(qat), Int8Linear.from_linear(plain)
+    x = torch.randn(3, 40)
+    assert torch.equal(served(x), want(x)) and set(served.state_dict()) == {"weight", "scale", "bias"}
+    off = (served.weight.double() * served.scale.double()[:, None] - qat.weight.detach().double()).abs()
+    assert bool((off <= 0.5001 * served.scale.double()[:, None]).all())  # half a step of each channel's own scale
+    assert float(served.scale[1:].max()) < 0.1 * float(served.scale[0])
