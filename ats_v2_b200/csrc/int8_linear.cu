@@ -694,12 +694,13 @@ struct PartOut {
 };
 
 // Add the S parts of this CTA's tokens and write them: a warp takes tokens, a lane four channels, with 8 reads in
-// flight, 6 where S is 3 or 6 (a read of another CTA's shared memory takes hundreds of cycles).  Each thread arrives
-// at the cluster's closing barrier between its last read of another CTA's tile and the stores that use it: the reads
-// are done with before any CTA may leave, and the barrier does not wait for these stores.
+// flight, 9 where S is 3 and 6 where it is 6 (a read of another CTA's shared memory takes hundreds of cycles).  Each
+// thread arrives at the cluster's closing barrier between its last read of another CTA's tile and the stores that use
+// it: the reads are done with before any CTA may leave, and the barrier does not wait for these stores.  It does wait
+// for the stores of a round before, which a third token at a time saves the parts in threes of up to 30 tokens each.
 template <typename T, int S>
 __device__ __forceinline__ void reduce_parts(const Out& o, const PartOut& p) {
-  constexpr int U = kMaxSplit / S, W = kPartThreads / 32;
+  constexpr int U = S == 3 ? 3 : kMaxSplit / S, W = kPartThreads / 32;
   const int warp = threadIdx.x >> 5, r4 = (threadIdx.x & 31) * 4, n = p.n0 + r4;
   const float4 sw = *reinterpret_cast<const float4*>(p.sw_s + r4), bw = *reinterpret_cast<const float4*>(p.bw_s + r4);
   const bool whole = p.vec_out && n + 4 <= o.N;
