@@ -299,7 +299,8 @@ def refuse_tangents(*tensors: torch.Tensor | None) -> None:
 
 def wants_grad(*tensors: torch.Tensor | None) -> bool:
     """Whether a call on these tensors is to be recorded for a backward; forward-mode duals are refused."""
-    refuse_tangents(*tensors)
+    if forward_ad._current_level >= 0:
+        refuse_tangents(*tensors)
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
@@ -315,7 +316,8 @@ def once_differentiable(backward):
 
     @functools.wraps(backward)
     def run(ctx, *grads):
-        refuse_tangents(*grads)
+        if forward_ad._current_level >= 0:
+            refuse_tangents(*grads)
         return wrapped(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
 
     return run

@@ -292,11 +292,10 @@ def apply_multi_axis_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: 
     if _lib.on_cpu("apply_multi_axis_rotary", q, k, positions, inv_freq):
         return (_torch_multi_axis(q, positions, inv_freq, axes),
                 _torch_multi_axis(k, positions, inv_freq, axes) if k is not None else None)
-    _lib.refuse_tangents(positions, inv_freq)
     q = _last_dim_contig(q)
     k = _last_dim_contig(k) if k is not None else None
     inv_freq = inv_freq.contiguous()
-    if _lib.wants_grad(q, k):
+    if _lib.wants_grad(q, k, positions, inv_freq):  # the last two need none: they may be duals
         return _MultiAxisRotaryFn.apply(q, k, positions, inv_freq, axes, n_axes)
     q_out, k_out = _out_like(q), _out_like(k) if k is not None else None
     _launch_axes(q, q_out, k, k_out, positions, inv_freq, axes, n_axes, False)
