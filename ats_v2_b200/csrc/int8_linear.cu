@@ -458,14 +458,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid
   tc::cluster_sync();  // both CTAs' barriers exist before either signals the other's
   tc::tc_fence_after();
   const uint32_t tmem_base = tmem_base_s;
-  // Waits for the last phase of each of `depth` barriers that n arrivals went round: true where all have landed.
+  // By a whole warp, a lane to each of `depth` barriers that n arrivals went round: waits for the last phase of every
+  // one; true where all have landed.
   auto landed = [&](uint64_t* bar, int depth, int n) {
     bool ok = true;
-    for (int s = 0; s < depth && s < n; ++s) {
-      const int last = s + (n - 1 - s) / depth * depth;
-      if (!tc::mbar_wait(&bar[s], (uint32_t)((last / depth) & 1), nullptr, kWaitBudget)) ok = false;
+    if (lane < depth && lane < n) {
+      const int last = lane + (n - 1 - lane) / depth * depth;
+      ok = tc::mbar_wait(&bar[lane], (uint32_t)((last / depth) & 1), nullptr, kWaitBudget);
     }
-    return ok;
+    return __all_sync(0xffffffffu, ok) != 0;
   };
   int issued_blocks = 0;
   tc::wait_prerequisites();  // the quantised tokens and their scales
@@ -649,22 +650,24 @@ __global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid
   // CTA 0 settles that block's count -- the half that never came counted as done, the half on its way expected -- and
   // waits for every phase.  So no load and no arrival is in flight when the second barrier lets both exit.
   tc::cluster_sync();
-  if (warp == 0 && lane == 0) {
-    const bool empties = landed(empty_bar, NST, used_s), accs = landed(tfull_bar, 2, tiles_s);
-    if (!empties || !accs) atomicCAS(&g_int8_status, 0, 38);
+  if (warp == 0) {
+    int bad = landed(empty_bar, NST, used_s) && landed(tfull_bar, 2, tiles_s) ? 0 : 38;
     if (cta == 0) {
       const int own = issued_blocks, peer = peer_issued_s;
       const int lo = own < peer ? own : peer, hi = own < peer ? peer : own;
       if (hi - lo > NST) {  // cannot happen: a stage is loaded again only after both halves of its last load
-        atomicCAS(&g_int8_status, 0, 37);
+        bad = 37;
       } else {
-        for (int k = lo; k < hi; ++k) {
-          if (k < own) tc::mbar_complete_tx(&full_bar[k % NST], STAGE);
-          else tc::mbar_arrive_expect_tx(&full_bar[k % NST], STAGE);
-        }
-        if (!landed(full_bar, NST, hi)) atomicCAS(&g_int8_status, 0, 35);
+        if (lane == 0)
+          for (int k = lo; k < hi; ++k) {
+            if (k < own) tc::mbar_complete_tx(&full_bar[k % NST], STAGE);
+            else tc::mbar_arrive_expect_tx(&full_bar[k % NST], STAGE);
+          }
+        __syncwarp();
+        if (!landed(full_bar, NST, hi)) bad = 35;
       }
     }
+    if (bad != 0 && lane == 0) atomicCAS(&g_int8_status, 0, bad);
   }
   __syncwarp();
   tc::cluster_sync_relaxed();
