@@ -88,11 +88,15 @@ def _last_dim_contig(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 else t.contiguous()
 
 
-def _out_like(t: torch.Tensor) -> torch.Tensor:
-    """An empty tensor laid out like t, its last axis consecutive as the kernels write it: empty_like moves another
-    axis of an overlapping view (windows of a longer sequence, say) inside of it."""
+def _out_like(t: torch.Tensor):
+    """An empty tensor laid out like t, its last axis consecutive as the kernels write it, and its other strides:
+    empty_like moves another axis of an overlapping view (windows of a longer sequence, say) inside of the last."""
     out = torch.empty_like(t)
-    return out if out.stride(-1) == 1 else t.new_empty(t.shape)
+    s = out.stride()
+    if s[3] != 1:
+        out = t.new_empty(t.shape)
+        s = out.stride()
+    return out, _lib.strides3(s[0], s[1], s[2])
 
 
 def _table(t: torch.Tensor, D: int, S: int, name: str) -> tuple[torch.Tensor, int]:
@@ -102,25 +106,26 @@ def _table(t: torch.Tensor, D: int, S: int, name: str) -> tuple[torch.Tensor, in
     return t, (0 if t.shape[0] == 1 else t.stride(0))
 
 
-def _launch(q_in, q_out, k_in, k_out, cos, sin, cs_stride, backward: bool) -> None:
+def _launch(q_in, k_in, cos, sin, cs_stride, backward: bool):
+    """The rotation of q_in and (unless None) k_in: (q_out, k_out)."""
     B, Hq, S, D = q_in.shape
-    Hk = k_in.shape[1] if k_in is not None else 0
+    q_out, qo = _out_like(q_in)
     qs = _lib.strides3(q_in.stride(0), q_in.stride(1), q_in.stride(2))
-    qo = _lib.strides3(q_out.stride(0), q_out.stride(1), q_out.stride(2))
-    ks = _lib.strides3(k_in.stride(0), k_in.stride(1), k_in.stride(2)) if k_in is not None else None
-    ko = _lib.strides3(k_out.stride(0), k_out.stride(1), k_out.stride(2)) if k_in is not None else None
+    k_out, Hk, ks, ko = None, 0, None, None
+    if k_in is not None:
+        k_out, ko = _out_like(k_in)
+        Hk, ks = k_in.shape[1], _lib.strides3(k_in.stride(0), k_in.stride(1), k_in.stride(2))
     _lib.call("ats_rope_apply", q_in.data_ptr(), q_out.data_ptr(), Hq, qs, qo,
               _lib.ptr(k_in), _lib.ptr(k_out), Hk, ks, ko, cos.data_ptr(), sin.data_ptr(), cs_stride,
               B, S, D, _lib.dtype_code(q_in.dtype), 1 if backward else 0, _lib.stream_of(q_in))
+    return q_out, k_out
 
 
 class _RopeFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, cos, sin, cs_stride):
         ctx.set_materialize_grads(False)  # an unused output's gradient arrives as None, not zeros
-        q_out = _out_like(q)
-        k_out = _out_like(k) if k is not None else None
-        _launch(q, q_out, k, k_out, cos, sin, cs_stride, False)
+        q_out, k_out = _launch(q, k, cos, sin, cs_stride, False)
         ctx.save_for_backward(cos, sin)
         ctx.cs_stride = cs_stride
         ctx.has_k = k is not None
@@ -132,17 +137,10 @@ class _RopeFn(torch.autograd.Function):
         if dq_out is None and (dk_out is None or not ctx.has_k):
             return None, None, None, None, None
         if dq_out is None:  # only k was used downstream: run its adjoint alone
-            dk_out = _last_dim_contig(dk_out)
-            dk = _out_like(dk_out)
-            _launch(dk_out, dk, None, None, cos, sin, ctx.cs_stride, True)
+            dk, _ = _launch(_last_dim_contig(dk_out), None, cos, sin, ctx.cs_stride, True)
             return None, dk, None, None, None
-        dq_out = _last_dim_contig(dq_out)
-        dq = _out_like(dq_out)
-        dk = None
-        if ctx.has_k and dk_out is not None:
-            dk_out = _last_dim_contig(dk_out)
-            dk = _out_like(dk_out)
-        _launch(dq_out, dq, dk_out if dk is not None else None, dk, cos, sin, ctx.cs_stride, True)
+        dk_out = _last_dim_contig(dk_out) if ctx.has_k and dk_out is not None else None
+        dq, dk = _launch(_last_dim_contig(dq_out), dk_out, cos, sin, ctx.cs_stride, True)
         return dq, dk, None, None, None
 
 
@@ -205,30 +203,30 @@ def _axis_of_pairs(interleaved: bool, *sections: int) -> bytes:
     return bytes(a for _, a in (sorted(pairs) if interleaved else pairs))
 
 
-def _launch_axes(q, q_out, k, k_out, positions, inv_freq, axes: bytes, n_axes: int, backward: bool) -> None:
-    if q is None:
-        q, q_out, k, k_out = k, k_out, None, None
-    B, H, S, D = q.shape
+def _launch_axes(q, k, positions, inv_freq, axes: bytes, n_axes: int, backward: bool):
+    """The rotation of q and k, of which one may be None: (q_out, k_out)."""
+    first, second = (q, k) if q is not None else (k, None)
+    B, H, S, D = first.shape
     s3 = _lib.strides3
     pos = positions.stride()
-    if k is not None:
-        kargs = (k.data_ptr(), k_out.data_ptr(), k.shape[1], s3(*k.stride()[:3]), s3(*k_out.stride()[:3]))
-    else:
-        kargs = (None, None, 0, None, None)
-    with _lib.device_of(q):
-        _lib.call("ats_rope_axes_apply", q.data_ptr(), q_out.data_ptr(), H, s3(*q.stride()[:3]),
-                  s3(*q_out.stride()[:3]), *kargs, positions.data_ptr(), _lib.ATS_POS_TYPES[positions.dtype],
+    out, out3 = _out_like(first)
+    k_out, kargs = None, (None, None, 0, None, None)
+    if second is not None:
+        k_out, k3 = _out_like(second)
+        kargs = (second.data_ptr(), k_out.data_ptr(), second.shape[1], s3(*second.stride()[:3]), k3)
+    with _lib.device_of(first):
+        _lib.call("ats_rope_axes_apply", first.data_ptr(), out.data_ptr(), H, s3(*first.stride()[:3]), out3, *kargs,
+                  positions.data_ptr(), _lib.ATS_POS_TYPES[positions.dtype],
                   s3(pos[0], pos[1] if len(pos) == 3 else 0, pos[-1]), n_axes, inv_freq.data_ptr(), axes, len(axes),
-                  B, S, D, _lib.dtype_code(q.dtype), 1 if backward else 0, _lib.stream_of(q))
+                  B, S, D, _lib.dtype_code(first.dtype), 1 if backward else 0, _lib.stream_of(first))
+    return (out, k_out) if q is not None else (None, out)
 
 
 class _MultiAxisRotaryFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, positions, inv_freq, axes, n_axes):
         ctx.set_materialize_grads(False)  # an unused output's gradient arrives as None, not zeros
-        q_out = _out_like(q)
-        k_out = _out_like(k) if k is not None else None
-        _launch_axes(q, q_out, k, k_out, positions, inv_freq, axes, n_axes, False)
+        q_out, k_out = _launch_axes(q, k, positions, inv_freq, axes, n_axes, False)
         ctx.save_for_backward(positions, inv_freq)
         ctx.axes = axes, n_axes
         return q_out, k_out
@@ -238,10 +236,9 @@ class _MultiAxisRotaryFn(torch.autograd.Function):
     def backward(ctx, dq_out, dk_out):
         positions, inv_freq = ctx.saved_tensors
         dq_out, dk_out = (_last_dim_contig(t) if t is not None else None for t in (dq_out, dk_out))
-        dq, dk = (_out_like(t) if t is not None else None for t in (dq_out, dk_out))
-        if dq is not None or dk is not None:
-            _launch_axes(dq_out, dq, dk_out, dk, positions, inv_freq, *ctx.axes, True)
-        return dq, dk, None, None, None, None
+        if dq_out is None and dk_out is None:
+            return (None,) * 6
+        return *_launch_axes(dq_out, dk_out, positions, inv_freq, *ctx.axes, True), None, None, None, None
 
 
 def _torch_multi_axis(x: torch.Tensor, positions, inv_freq, axes: bytes) -> torch.Tensor:
@@ -268,7 +265,7 @@ def apply_multi_axis_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: 
     Any batch, head and sequence strides; the results of dense inputs are laid out like them.
     One launch each way on CUDA tensors; differentiable once, in q and k, and in reverse mode only
     (duals are refused)."""
-    axes = axis_of_pairs(tuple(sections), bool(interleaved))
+    axes = _axis_of_pairs(bool(interleaved), *sections)
     n_axes = len(sections)
     if q.dim() != 4 or q.shape[-1] < 2 * len(axes):
         raise ValueError(f"apply_multi_axis_rotary: q must be [batch, heads, seq_len, head_dim >= {2 * len(axes)}], "
@@ -297,9 +294,7 @@ def apply_multi_axis_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: 
     inv_freq = inv_freq.contiguous()
     if _lib.wants_grad(q, k, positions, inv_freq):  # the last two need none: they may be duals
         return _MultiAxisRotaryFn.apply(q, k, positions, inv_freq, axes, n_axes)
-    q_out, k_out = _out_like(q), _out_like(k) if k is not None else None
-    _launch_axes(q, q_out, k, k_out, positions, inv_freq, axes, n_axes, False)
-    return q_out, k_out
+    return _launch_axes(q, k, positions, inv_freq, axes, n_axes, False)
 
 
 class MultiAxisRotaryEmbedding(nn.Module):

@@ -2,6 +2,8 @@
 
 from __future__ import annotations
 
+import contextlib
+
 import pytest
 import torch
 
@@ -23,10 +25,13 @@ def view(name):
 @pytest.mark.parametrize("axes", ["one", "several"])
 def test_inputs_and_results_have_consecutive_heads(monkeypatch, axes, name, grad):
     seen = []
-    monkeypatch.setattr(_lib, "on_cpu", lambda *a: False)
-    monkeypatch.setattr(_lib, "require_cuda", lambda *a: None)
-    for fn in ("_launch", "_launch_axes"):  # (q, q_out, k, k_out, ...)
-        monkeypatch.setattr(rope, fn, lambda *a: seen.extend(zip(a[0:4:2], a[1:4:2])))
+
+    def call(name, q, q_out, heads, q_strides, q_out_strides, k, k_out, k_heads, k_strides, k_out_strides, *rest):
+        seen.extend([(q_out, tuple(q_strides), tuple(q_out_strides)), (k_out, tuple(k_strides), tuple(k_out_strides))])
+
+    for what, stub in (("on_cpu", lambda *a: False), ("require_cuda", lambda *a: None), ("call", call),
+                       ("stream_of", lambda t: 0), ("device_of", lambda t: contextlib.nullcontext())):
+        monkeypatch.setattr(_lib, what, stub)
     q, k = view(name), view(name)
     if grad:
         q, k = q.requires_grad_(), k.requires_grad_()
@@ -35,11 +40,13 @@ def test_inputs_and_results_have_consecutive_heads(monkeypatch, axes, name, grad
     else:
         out = rope.apply_multi_axis_rotary(q, k, torch.zeros(2, 4, dtype=torch.int64), torch.ones(4), (2, 2))
     if grad:
-        torch.autograd.backward(out, (view(name), view(name)))
-    assert len(seen) == (4 if grad else 2)
-    for src, dst in seen:
-        assert src.shape == dst.shape == (2, 3, 4, 8) and src.stride(-1) == dst.stride(-1) == 1
+        out += torch.autograd.grad(out, (q, k), (view(name), view(name)))
+    assert len(out) == len(seen) == (4 if grad else 2)
+    for dst, (ptr, src_strides, dst_strides) in zip(out, seen):
+        assert dst.data_ptr() == ptr and dst.stride() == (*dst_strides, 1)
         places = (torch.tensor(dst.stride()) * torch.cartesian_prod(*map(torch.arange, dst.shape))).sum(1)
         assert places.unique().numel() == dst.numel()  # every value has a place of its own
+        if VIEWS[name][3] == 1:
+            assert src_strides == VIEWS[name][:3]  # read where it is
         if name in ("dense", "heads inside"):
-            assert dst.stride() == src.stride()
+            assert dst_strides == src_strides
