@@ -106,26 +106,25 @@ def _table(t: torch.Tensor, D: int, S: int, name: str) -> tuple[torch.Tensor, in
     return t, (0 if t.shape[0] == 1 else t.stride(0))
 
 
-def _launch(q_in, k_in, cos, sin, cs_stride, backward: bool):
-    """The rotation of q_in and (unless None) k_in: (q_out, k_out)."""
+def _launch(q_in, q_out, k_in, k_out, cos, sin, cs_stride, backward: bool) -> None:
     B, Hq, S, D = q_in.shape
-    q_out, qo = _out_like(q_in)
+    Hk = k_in.shape[1] if k_in is not None else 0
     qs = _lib.strides3(q_in.stride(0), q_in.stride(1), q_in.stride(2))
-    k_out, Hk, ks, ko = None, 0, None, None
-    if k_in is not None:
-        k_out, ko = _out_like(k_in)
-        Hk, ks = k_in.shape[1], _lib.strides3(k_in.stride(0), k_in.stride(1), k_in.stride(2))
+    qo = _lib.strides3(q_out.stride(0), q_out.stride(1), q_out.stride(2))
+    ks = _lib.strides3(k_in.stride(0), k_in.stride(1), k_in.stride(2)) if k_in is not None else None
+    ko = _lib.strides3(k_out.stride(0), k_out.stride(1), k_out.stride(2)) if k_in is not None else None
     _lib.call("ats_rope_apply", q_in.data_ptr(), q_out.data_ptr(), Hq, qs, qo,
               _lib.ptr(k_in), _lib.ptr(k_out), Hk, ks, ko, cos.data_ptr(), sin.data_ptr(), cs_stride,
               B, S, D, _lib.dtype_code(q_in.dtype), 1 if backward else 0, _lib.stream_of(q_in))
-    return q_out, k_out
 
 
 class _RopeFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, cos, sin, cs_stride):
         ctx.set_materialize_grads(False)  # an unused output's gradient arrives as None, not zeros
-        q_out, k_out = _launch(q, k, cos, sin, cs_stride, False)
+        q_out = _out_like(q)[0]
+        k_out = _out_like(k)[0] if k is not None else None
+        _launch(q, q_out, k, k_out, cos, sin, cs_stride, False)
         ctx.save_for_backward(cos, sin)
         ctx.cs_stride = cs_stride
         ctx.has_k = k is not None
@@ -137,10 +136,17 @@ class _RopeFn(torch.autograd.Function):
         if dq_out is None and (dk_out is None or not ctx.has_k):
             return None, None, None, None, None
         if dq_out is None:  # only k was used downstream: run its adjoint alone
-            dk, _ = _launch(_last_dim_contig(dk_out), None, cos, sin, ctx.cs_stride, True)
+            dk_out = _last_dim_contig(dk_out)
+            dk = _out_like(dk_out)[0]
+            _launch(dk_out, dk, None, None, cos, sin, ctx.cs_stride, True)
             return None, dk, None, None, None
-        dk_out = _last_dim_contig(dk_out) if ctx.has_k and dk_out is not None else None
-        dq, dk = _launch(_last_dim_contig(dq_out), dk_out, cos, sin, ctx.cs_stride, True)
+        dq_out = _last_dim_contig(dq_out)
+        dq = _out_like(dq_out)[0]
+        dk = None
+        if ctx.has_k and dk_out is not None:
+            dk_out = _last_dim_contig(dk_out)
+            dk = _out_like(dk_out)[0]
+        _launch(dq_out, dq, dk_out if dk is not None else None, dk, cos, sin, ctx.cs_stride, True)
         return dq, dk, None, None, None
 
 
