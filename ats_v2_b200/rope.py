@@ -88,15 +88,11 @@ def _last_dim_contig(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 else t.contiguous()
 
 
-def _out_like(t: torch.Tensor):
-    """An empty tensor laid out like t, its last axis consecutive as the kernels write it, and its other strides:
-    empty_like moves another axis of an overlapping view (windows of a longer sequence, say) inside of the last."""
+def _out_like(t: torch.Tensor) -> torch.Tensor:
+    """An empty tensor laid out like t, its last axis consecutive as the kernels write it: empty_like moves another
+    axis of an overlapping view (windows of a longer sequence, say) inside of it."""
     out = torch.empty_like(t)
-    s = out.stride()
-    if s[3] != 1:
-        out = t.new_empty(t.shape)
-        s = out.stride()
-    return out, _lib.strides3(s[0], s[1], s[2])
+    return out if out.stride()[3] == 1 else t.new_empty(t.shape)
 
 
 def _table(t: torch.Tensor, D: int, S: int, name: str) -> tuple[torch.Tensor, int]:
@@ -122,8 +118,8 @@ class _RopeFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, cos, sin, cs_stride):
         ctx.set_materialize_grads(False)  # an unused output's gradient arrives as None, not zeros
-        q_out = _out_like(q)[0]
-        k_out = _out_like(k)[0] if k is not None else None
+        q_out = _out_like(q)
+        k_out = _out_like(k) if k is not None else None
         _launch(q, q_out, k, k_out, cos, sin, cs_stride, False)
         ctx.save_for_backward(cos, sin)
         ctx.cs_stride = cs_stride
@@ -137,15 +133,15 @@ class _RopeFn(torch.autograd.Function):
             return None, None, None, None, None
         if dq_out is None:  # only k was used downstream: run its adjoint alone
             dk_out = _last_dim_contig(dk_out)
-            dk = _out_like(dk_out)[0]
+            dk = _out_like(dk_out)
             _launch(dk_out, dk, None, None, cos, sin, ctx.cs_stride, True)
             return None, dk, None, None, None
         dq_out = _last_dim_contig(dq_out)
-        dq = _out_like(dq_out)[0]
+        dq = _out_like(dq_out)
         dk = None
         if ctx.has_k and dk_out is not None:
             dk_out = _last_dim_contig(dk_out)
-            dk = _out_like(dk_out)[0]
+            dk = _out_like(dk_out)
         _launch(dq_out, dq, dk_out if dk is not None else None, dk, cos, sin, ctx.cs_stride, True)
         return dq, dk, None, None, None
 
@@ -215,17 +211,27 @@ def _launch_axes(q, k, positions, inv_freq, axes: bytes, n_axes: int, backward: 
     B, H, S, D = first.shape
     s3 = _lib.strides3
     pos = positions.stride()
-    out, out3 = _out_like(first)
-    k_out, kargs = None, (None, None, 0, None, None)
+    ib, ih, is_, _ = first.stride()
+    out = torch.empty_like(first)
+    ob, oh, os_, od = out.stride()
+    if od != 1:
+        out = _out_like(first)
+        ob, oh, os_, _ = out.stride()
+    out2, kargs = None, (None, None, 0, None, None)
     if second is not None:
-        k_out, k3 = _out_like(second)
-        kargs = (second.data_ptr(), k_out.data_ptr(), second.shape[1], s3(*second.stride()[:3]), k3)
+        kb, kh, ks, _ = second.stride()
+        out2 = torch.empty_like(second)
+        cb, ch, cs, cd = out2.stride()
+        if cd != 1:
+            out2 = _out_like(second)
+            cb, ch, cs, _ = out2.stride()
+        kargs = (second.data_ptr(), out2.data_ptr(), second.shape[1], s3(kb, kh, ks), s3(cb, ch, cs))
     with _lib.device_of(first):
-        _lib.call("ats_rope_axes_apply", first.data_ptr(), out.data_ptr(), H, s3(*first.stride()[:3]), out3, *kargs,
+        _lib.call("ats_rope_axes_apply", first.data_ptr(), out.data_ptr(), H, s3(ib, ih, is_), s3(ob, oh, os_), *kargs,
                   positions.data_ptr(), _lib.ATS_POS_TYPES[positions.dtype],
                   s3(pos[0], pos[1] if len(pos) == 3 else 0, pos[-1]), n_axes, inv_freq.data_ptr(), axes, len(axes),
                   B, S, D, _lib.dtype_code(first.dtype), 1 if backward else 0, _lib.stream_of(first))
-    return (out, k_out) if q is not None else (None, out)
+    return (out, out2) if q is not None else (None, out)
 
 
 class _MultiAxisRotaryFn(torch.autograd.Function):
