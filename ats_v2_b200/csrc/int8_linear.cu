@@ -71,8 +71,8 @@ __device__ __forceinline__ void load16(const T* row, int k, int K, uint4 (&v)[si
 }
 
 // The same of a row aligned to P only, of which K is whole pieces: G threads load their G * 16 values from `base` on side
-// by side and pass them through `stage`, where thread t finds its 16.  8192 x 2047 bf16: 12.2 us, 2046: 8.8 us;
-// 16 loads by each thread for itself took 20.4 us.
+// by side and pass them through `stage`, where thread t finds its 16.  8192 x 2047 bf16, the same rows again from L2:
+// 12.2 us, 2046: 8.8 us; 16 loads by each thread for itself took 20.4 us.  (From HBM 18 to 23 and 11 us.)
 template <typename T, int G, typename P>
 __device__ __forceinline__ void stage16(const T* row, int base, int t, int K, char* stage, uint4 (&v)[sizeof(T)]) {
   constexpr int E = (int)(sizeof(P) / sizeof(T)), N = 16 / E;
@@ -260,8 +260,8 @@ int quantize_g(const T* x, int64_t ldx, int8_t* q, int64_t ldq, float* scale, in
   return go(uint32_t{});
 }
 
-// As many threads as hold the row in their registers: 32, 128 or 512 (8192x2048 bf16: 6.7 us with a warp a row; 256
-// threads, half of them idle there, took 18.4).
+// As many threads as hold the row in their registers: 32, 128 or 512 (8192x2048 bf16, the same rows again from L2: 6.7
+// us with a warp a row; 256 threads, half of them idle there, took 18.4.  From HBM a warp a row takes 10 to 12).
 template <typename T>
 int quantize_t(const void* x, int64_t ldx, void* q, int64_t ldq, float* scale, int64_t rows, int64_t K,
                cudaStream_t st) {
@@ -294,8 +294,8 @@ __device__ __forceinline__ float bias_at(const Out& o, int n) {
 // --------------------------------------------------------------- one token
 // One launch: every block quantises the token into its shared memory (it comes from L2), with the first weights of
 // its warps already in flight, then a warp takes an output channel at a time: 16 weights per lane and step against
-// the token's integers.  The weights are read once; latency bounds it at this size (4096 x 4096: 5.4 us, 3.1 TB/s; the
-// tensor-core kernel below takes 6.6 us with its quantisation).
+// the token's integers.  The weights are read once; latency bounds it at this size (4096 x 4096: 7.1 us with the weights
+// from HBM, 2.4 TB/s; 5.2 from L2, where the tensor-core kernel below takes 6.6 with its quantisation).
 constexpr int kDotThreads = 256, kDotStep = 8;
 constexpr int kDotLongest = 16384;  // a warp walks its channels 4 KB at a time: longer rows are split over SMs instead
 
@@ -378,12 +378,13 @@ __global__ void __launch_bounds__(kDotThreads, 4) int8_dot_kernel(const T* __res
 // persistent, each CTA with a TMA producer warp and eight epilogue warps (two per TMEM lane quadrant, half of the
 // columns each) that scale and round into a swizzled box of shared memory, 32 rows of 128 bytes, which a TMA store
 // empties beside the next box's arithmetic (8192 x 8192 x 512 bf16: 54 us, where filling the result with a constant
-// takes 35; with the box read back and stored by the warp 58).  CTA 0's MMA warp issues for both, into two
+// takes 35; with the box read back and stored by the warp 58, both before the last waits took a lane to each barrier).  CTA 0's MMA warp issues for both, into two
 // accumulators.  Each CTA loads its 128 tokens and half of the channels, 32 KB a block where a single CTA of 128 x 256
 // loads 48: single CTAs were held by what L2 delivers to the SMs, about 15 TB/s (8192^3: 440 us against 386 in pairs,
-// both with an earlier quantisation; 370 us now).  All loads of a block count on CTA 0's full barrier; its commits
-// reach the empty and accumulator barriers of both; both epilogues release the accumulator on CTA 0.  A block takes
-// 509 to 544 SM cycles against the 512 of its MMAs, so the clock under the power limit bounds it.
+// both with an earlier quantisation; 355 to 375 us now).  All loads of a block count on CTA 0's full barrier; its commits
+// reach the empty and accumulator barriers of both; both epilogues release the accumulator on CTA 0.  From one
+// commit of the MMA warp to the next it is 509 to 544 SM cycles, about the 512 that a block's MMAs take (the commits
+// themselves jitter), so the clock under the power limit bounds it.
 constexpr int BM = 128, BKB = 128;
 constexpr int kEpiWarps = 8, kTileThreads = 64 + 32 * kEpiWarps;
 constexpr int kBox = 32 * 128;  // an epilogue warp's staging: 32 rows of 128 bytes
@@ -459,7 +460,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid
   tc::tc_fence_after();
   const uint32_t tmem_base = tmem_base_s;
   // By a whole warp, a lane to each of `depth` barriers that n arrivals went round: waits for the last phase of every
-  // one; true where all have landed.
+  // one; true where all have landed.  One barrier after the other took 1.5 us of every call (2000^3: 17.4 us, so 16.0).
   auto landed = [&](uint64_t* bar, int depth, int n) {
     bool ok = true;
     if (lane < depth && lane < n) {
@@ -619,7 +620,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid
             tc::tma_store_2d(&tmY, box, col0, row0);  // what lies past the last row or column is left out
             tc::bulk_commit();
           }
-        } else {  // rows of y that are not 16-byte multiples: piece by piece, along the rows (8192 x 8190: 81 us)
+        } else {  // rows of y that are not 16-byte multiples: piece by piece, along the rows (8192 x 8190: 79 us)
           __syncwarp();
           auto store = [&](auto piece) {
             using P = decltype(piece);
@@ -682,8 +683,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid
 // shares K: each sums its part of K in TMEM, puts its int32 tile into its shared memory, and every CTA adds the parts of
 // its share of the tokens through distributed shared memory.  So a decoding batch reads the weights with every SM, and
 // no workspace or atomics are needed.  The weights' loads start before the quantisation has ended.  48 tokens through
-// 11008 x 4096: 10.4 us with the quantisation, 4.5 TB/s; sums over distributed shared memory cost about as much as their
-// bytes at 3.3 TB/s, which is why few columns may be split further than many.
+// 11008 x 4096, in 3 parts: 13.7 us with the quantisation and the weights from HBM, 3.4 TB/s; sums over distributed
+// shared memory cost about as much as their bytes at 3.3 TB/s, which is why few columns may be split further than many.
 constexpr int kPartThreads = 64 + 32 * kEpiWarps, kMaxSplit = 8;
 
 // Two CTAs share an SM, with half of its shared memory each.
@@ -1021,15 +1022,18 @@ int linear(const void* x, int64_t ldx, const int8_t* w, int64_t ldw, Out o, int6
   const int kb = (int)((K + BKB - 1) / BKB);
   const int tn = o.M <= 16 ? 16 : o.M <= 32 ? 32 : nt * ((o.M + 63) / 64) <= two ? 64 : 128;
   const int64_t mt = (o.M + tn - 1) / tn, ctas = nt * mt;
-  // One round of pair tiles beats two CTAs to an SM where it keeps three quarters of the pairs busy (2000^3: 16.8 us
-  // against 20.4; 3000 x 1000 x 1000, 48 tiles: 13.7 against 14.3; 1024 x 2048 x 4096, 32 tiles: 19.0 against 15.6).
+  // One round of pair tiles beats two CTAs to an SM where it keeps three quarters of the pairs busy (from L2,
+  // 2000^3: 16.8 us against 20.4; 3000 x 1000 x 1000, 48 tiles: 13.7 against 14.3; 1024 x 2048 x 4096, 32 tiles: 19.0
+  // against 15.6; the pair tiles' last waits have since become shorter, 2000^3 16.0).
   const int64_t pair_tiles = ((o.M + TM - 1) / TM) * ((o.N + BN - 1) / (int64_t)BN);
   const bool one_round = ctas > sms && tn == 128 && 8 * pair_tiles >= 3 * (int64_t)sms;
   if (ctas > two || mt > 65535 || one_round) return tiles<T>(q, ldq, w, ldw, o, (int)K, st);
   // K is split so that the fullest SM, of one or two CTAs, has the least to do, where each part has 2 blocks of K, or 8
   // where SMs have two parts, and at most 256 columns are summed; for the same load into more parts where each still
-  // has 16 blocks.  In us: 48 tokens 4096x11008 25.7 whole, 16.6 in 2, 12.6 in 4, 16.2 in 8; 48 tokens 11008x4096 14.3
-  // in 2, 12.9 in 3; 200 tokens 2048x8192 14.5 in 2, 13.2 in 4; 500 tokens 2048x2048 8.6 whole, 9.3 in 2.  Clusters of 3
+  // has 16 blocks.  In us, one sweep of the same tokens: 48 tokens 4096x11008 25.7 whole, 16.6 in 2, 12.6 in 4, 16.2
+  // in 8; 48 tokens 11008x4096 14.3 in 2, 12.9 in 3; 200 tokens 2048x8192 14.5 in 2, 13.2 in 4; 500 tokens 2048x2048 8.6
+  // whole, 9.3 in 2.  (Those chosen, each call with tokens and weights of its own from HBM: 14.1 to 14.7, 13.7, 13.5 and
+  // 9.3 to 9.6.)  Clusters of 3
   // or 6 leave places free that others fill: 288 CTAs in clusters of 3 did not fit on 148 SMs at once (100 tokens
   // 6144x4096: 16.7 in 3, 12.3 in 2), so they get nine tenths of the places.
   int split = 1;

@@ -56,7 +56,8 @@ ATS_API uint64_t ats_kernel_launches(void);
  * with, for launches made later by the calling host thread; 0 (the default)
  * means every SM.  A caller that overlaps a collective on another stream with
  * the expert GEMMs leaves SMs free for it: a GEMM CTA occupies a whole SM, so
- * a collective launched beside a full-width GEMM would wait for its end.
+ * a collective launched beside a full-width GEMM would wait for its end.  The
+ * 8-bit product (ats_int8_linear) keeps to it as well.
  * No reference counterpart (DeepSpeed's all-to-all does not overlap). */
 ATS_API int ats_set_gemm_sm_limit(int sms);
 ATS_API int ats_gemm_sm_limit(void);
