@@ -378,13 +378,13 @@ __global__ void __launch_bounds__(kDotThreads, 4) int8_dot_kernel(const T* __res
 // persistent, each CTA with a TMA producer warp and eight epilogue warps (two per TMEM lane quadrant, half of the
 // columns each) that scale and round into a swizzled box of shared memory, 32 rows of 128 bytes, which a TMA store
 // empties beside the next box's arithmetic (8192 x 8192 x 512 bf16: 54 us, where filling the result with a constant
-// takes 35; with the box read back and stored by the warp 58, both before the last waits took a lane to each barrier).  CTA 0's MMA warp issues for both, into two
-// accumulators.  Each CTA loads its 128 tokens and half of the channels, 32 KB a block where a single CTA of 128 x 256
-// loads 48: single CTAs were held by what L2 delivers to the SMs, about 15 TB/s (8192^3: 440 us against 386 in pairs,
-// both with an earlier quantisation; 355 to 375 us now).  All loads of a block count on CTA 0's full barrier; its commits
-// reach the empty and accumulator barriers of both; both epilogues release the accumulator on CTA 0.  From one
-// commit of the MMA warp to the next it is 509 to 544 SM cycles, about the 512 that a block's MMAs take (the commits
-// themselves jitter), so the clock under the power limit bounds it.
+// takes 35; with the box read back and stored by the warp 58, before the last waits took a lane to each barrier).  CTA
+// 0's MMA warp issues for both, into two accumulators.  Each CTA loads its 128 tokens and half of the channels, 32 KB
+// a block where a single CTA of 128 x 256 loads 48: single CTAs were held by what L2 delivers to the SMs, about 15
+// TB/s (8192^3: 440 us against 386 in pairs, both with an earlier quantisation; 355 to 375 us now).  All loads of a
+// block count on CTA 0's full barrier; its commits reach the empty and accumulator barriers of both; both epilogues
+// release the accumulator on CTA 0.  From one commit of the MMA warp to the next it is 509 to 544 SM cycles, about the
+// 512 that a block's MMAs take (the commits themselves jitter), so the clock under the power limit bounds it.
 constexpr int BM = 128, BKB = 128;
 constexpr int kEpiWarps = 8, kTileThreads = 64 + 32 * kEpiWarps;
 constexpr int kBox = 32 * 128;  // an epilogue warp's staging: 32 rows of 128 bytes

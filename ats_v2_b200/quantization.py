@@ -198,7 +198,7 @@ class Int8Linear(nn.Module):
         if weight.stride(1) == 1 and weight.stride(0) % 16 == 0 and weight.stride(0) >= K and \
                 weight.data_ptr() % 16 == 0:
             return weight
-        return torch.zeros((N, (K + 15) // 16 * 16), dtype=torch.int8, device=weight.device)[:, :K].copy_(weight)
+        return torch.zeros((N, (K + 15) // 16 * 16), dtype=weight.dtype, device=weight.device)[:, :K].copy_(weight)
 
     @classmethod
     def from_linear(cls, linear: nn.Linear) -> "Int8Linear":
@@ -212,8 +212,7 @@ class Int8Linear(nn.Module):
     def _apply(self, fn, recurse=True):  # moves keep the scales float32 and the rows aligned
         old = self.scale
         super()._apply(fn, recurse)
-        if self.scale.dtype != torch.float32:
-            self.scale = self.scale.float() if old.is_meta else old.to(device=self.scale.device)
+        self.scale = self.scale.float() if old.is_meta else old.to(device=self.scale.device)
         self.weight = self._laid_out(self.weight)
         return self
 

@@ -333,9 +333,9 @@ class MultiAxisRotaryEmbedding(nn.Module):
         old = self.inv_freq
         super()._apply(fn, recurse)
         new = self.inv_freq
-        if old.is_meta and not new.is_meta:  # to_empty: no state dict holds what belongs there
+        if old.is_meta and not new.is_meta:  # no state dict holds what belongs there
             self.inv_freq = self._frequencies(new.device)
-        elif new.dtype != torch.float32:  # .to(dtype) must not round the frequencies
+        else:  # .to(dtype) must not round the frequencies, nor to_empty lose them
             self.inv_freq = old.to(device=new.device)
         return self
 

@@ -28,8 +28,9 @@ def test_rotary_made_on_the_meta_device(cast):
 
 def test_rotary_casts_keep_its_frequencies():
     emb = MultiAxisRotaryEmbedding(16, (5, 3))
+    emb.inv_freq *= 0.5  # values of the user's own
     want = emb.inv_freq.clone()
-    for m in (emb.half(), copy.deepcopy(emb).bfloat16(), emb.double(), emb.to("cpu")):
+    for m in (emb.half(), copy.deepcopy(emb).bfloat16(), emb.double(), emb.to("cpu"), emb.to_empty(device="cpu")):
         assert m.inv_freq.dtype == torch.float32 and torch.equal(m.inv_freq, want)
 
 
@@ -79,6 +80,11 @@ def test_an_assigned_weight_is_laid_out_once(meta):
     aligned = want.weight
     lin.load_state_dict({**want.state_dict(), "weight": aligned}, assign=True)
     assert lin.weight.data_ptr() == aligned.data_ptr()  # already so: taken as it is
+    for floats in (torch.rand(7, 33), torch.rand(7, 48)[:, :33]):  # not an 8-bit weight: refused, never truncated
+        wrong = Int8Linear(33, 7, bias=True)
+        wrong.load_state_dict({**want.state_dict(), "weight": floats}, assign=True)
+        with pytest.raises(TypeError, match="must be int8"):
+            wrong(torch.randn(3, 33))
     with pytest.raises(RuntimeError, match="size mismatch"):
         lin.load_state_dict({**want.state_dict(), "weight": aligned[:, :32]}, assign=True)
 
